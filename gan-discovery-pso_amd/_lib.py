@@ -84,6 +84,18 @@ _PROTOTYPES = {
     "gdpso_vq_nearest": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t]),
     "gdpso_vq_lookup": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "gdpso_vq_nearest_static": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gdpso_code_logits": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, c_void_p, c_int, c_float, c_void_p]),
+    "gdpso_code_logits_grad_workspace_bytes": (c_size_t, [c_int] * 3),
+    "gdpso_code_logits_grad": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p] * 3 + [c_int, c_float] + [c_void_p] * 3 + [c_size_t]),
+    "gdpso_balance_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "gdpso_balance": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, C.c_longlong, c_int, c_void_p, c_int, c_void_p, c_float] + [c_void_p] * 5
+                      + [c_size_t]),
+    "gdpso_balance_grad": (c_int, [c_void_p, c_int, c_int, c_void_p, C.c_longlong, c_int] + [c_void_p] * 4),
+    "gdpso_distill_workspace_bytes": (c_size_t, [c_int] * 3),
+    "gdpso_distill": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, C.c_longlong, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_float, c_float]
+                      + [c_void_p] * 5 + [c_size_t]),
+    "gdpso_distill_grad": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, C.c_longlong, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_float]
+                           + [c_void_p] * 3),
     "gdpso_swarm_scratch_bytes": (c_size_t, [c_int]),
     "gdpso_swarm_reset": (c_int, [C.POINTER(SwarmDesc), c_void_p, c_double]),
     "gdpso_swarm_local_best": (c_int, [C.POINTER(SwarmDesc), c_void_p, c_int, c_int]),

@@ -366,6 +366,191 @@ def vq_seed_codebook(codebook: torch.Tensor, positions: torch.Tensor, row0: int 
         check(_lib.lib().gdpso_vq_seed_codebook(_lib.stream_handle(device), ptr(codebook), k, d, int(row0), ptr(pos), pos.shape[0]))
 
 
+# -------------------------------------------------- soft code assignment and losses over it
+_LOGIT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _code_args(inputs: torch.Tensor, codebook: torch.Tensor):
+    device = _device_guard(codebook.device)
+    _same_device(device, inputs=inputs)
+    if codebook.dim() != 2 or codebook.shape[0] == 0 or codebook.shape[1] == 0:
+        raise ValueError("codebook must be [K, D]")
+    if inputs.dim() == 0 or inputs.shape[-1] != codebook.shape[1]:
+        raise ValueError(f"inputs must be [..., {codebook.shape[1]}], got {tuple(inputs.shape)}")
+    if inputs.dtype not in _LOGIT_TYPES or codebook.dtype != inputs.dtype:
+        raise ValueError(f"inputs and codebook must share one of float32, bfloat16, float16 (got {inputs.dtype} and {codebook.dtype})")
+    return device, inputs.detach().reshape(-1, inputs.shape[-1]).contiguous(), codebook.detach().contiguous()
+
+
+def code_logits(inputs: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+    """Logits of the soft assignment of ``inputs`` [..., D] to the rows of ``codebook`` [K, D] (gdpso_code_logits):
+    (2 <x, code> - |code|^2) / temperature, float32 [..., K], whatever the type of the inputs."""
+    device, x, cb = _code_args(inputs, codebook)
+    (n, d), k = x.shape, cb.shape[0]
+    out = torch.empty(n, k, dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        check(_lib.lib().gdpso_code_logits(_lib.stream_handle(device), n, d, k, ptr(x), ptr(cb), _dtype_code(x.dtype), temperature, ptr(out)))
+    return out.reshape(*inputs.shape[:-1], k)
+
+
+def code_logits_grad(grad_logits: torch.Tensor, inputs: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.0, want_inputs=True,
+                     want_codebook=True):
+    """Gradients of ``code_logits`` for ``grad_logits`` float32 [..., K] (gdpso_code_logits_grad): (gradient of the inputs or
+    None, gradient of the codebook or None), in their type."""
+    device, x, cb = _code_args(inputs, codebook)
+    (n, d), k = x.shape, cb.shape[0]
+    _same_device(device, grad_logits=grad_logits)
+    if grad_logits.dtype != torch.float32 or grad_logits.shape != (*inputs.shape[:-1], k):
+        raise ValueError(f"grad_logits must be float32 {(*inputs.shape[:-1], k)}, got {grad_logits.dtype} {tuple(grad_logits.shape)}")
+    g = grad_logits.detach().reshape(n, k).contiguous()
+    dx = torch.empty_like(x) if want_inputs else None
+    dcb = torch.empty_like(cb) if want_codebook else None
+    L = _lib.lib()
+    with torch.cuda.device(device):
+        ws = torch.empty(L.gdpso_code_logits_grad_workspace_bytes(n, d, k), dtype=torch.uint8, device=device) if want_codebook else None
+        check(L.gdpso_code_logits_grad(_lib.stream_handle(device), n, d, k, ptr(g), ptr(x), ptr(cb), _dtype_code(x.dtype), temperature, ptr(dx), ptr(dcb),
+                                       ptr(ws), 0 if ws is None else ws.numel()))
+    return None if dx is None else dx.reshape(inputs.shape), dcb
+
+
+def _loss_rows(logits: torch.Tensor, mask):
+    """Rows [n, E] of ``logits`` [..., E] with consecutive columns (a view where the strides allow it) and the mask's bytes."""
+    device = _device_guard(logits.device)
+    if logits.dtype not in _LOGIT_TYPES:
+        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be [..., E] with E > 0, got {tuple(logits.shape)}")
+    e = logits.shape[-1]
+    rows = logits.detach().reshape(logits.numel() // e, e)
+    if rows.stride(1) != 1 and e > 1:
+        rows = rows.contiguous()
+    if mask is not None:
+        _same_device(device, mask=mask)
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape[:-1]:
+            raise ValueError(f"mask must be bool {tuple(logits.shape[:-1])}, got {mask.dtype} {tuple(mask.shape)}")
+        mask = mask.detach().reshape(-1).contiguous()
+    return device, rows, mask
+
+
+def _row_indices(indices: torch.Tensor, lead, device, what):
+    """indices [..., k], or [...] for one a row -> contiguous [n, k]."""
+    _same_device(device, **{what: indices})
+    if indices.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what} must be int64 or int32, got {indices.dtype}")
+    if indices.shape == lead:
+        indices = indices.unsqueeze(-1)
+    if indices.shape[:-1] != lead or indices.shape[-1] == 0:
+        raise ValueError(f"{what} must be {(*lead, 'k')}, got {tuple(indices.shape)}")
+    return indices.detach().reshape(lead.numel(), indices.shape[-1]).contiguous()
+
+
+def _row_stride(rows):
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+
+
+def _balance(logits, indices, mask, grad_scale):
+    device, rows, mask = _loss_rows(logits, mask)
+    n, e = rows.shape
+    idx = _row_indices(indices, logits.shape[:-1], device, "indices")
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    counts = torch.empty(e + 2, dtype=torch.int64, device=device)
+    mean_prob = torch.empty(e, dtype=torch.float32, device=device)
+    grad = None if grad_scale is None else torch.empty(n, e, dtype=rows.dtype, device=device)
+    L = _lib.lib()
+    with torch.cuda.device(device):
+        ws = torch.empty(L.gdpso_balance_workspace_bytes(n, e), dtype=torch.uint8, device=device)
+        check(L.gdpso_balance(_lib.stream_handle(device), n, e, idx.shape[1], ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(idx),
+                              idx.element_size(), ptr(mask), 0.0 if grad_scale is None else grad_scale, ptr(loss), ptr(counts), ptr(mean_prob),
+                              ptr(grad), ptr(ws), ws.numel()))
+    return loss, counts, mean_prob, None if grad is None else grad.reshape(logits.shape)
+
+
+def balance(logits: torch.Tensor, indices: torch.Tensor, mask=None, grad_scale=None):
+    """Balance loss of the choices ``indices`` [..., k] (or [...]: one a row) made from ``logits`` [..., E] (gdpso_balance):
+    E * sum_c f[c] P[c], f the share of the choices that fell on c, P the mean softmax.  ``mask`` bool [...]: rows to leave
+    out are False.  An index outside [0, E) is a choice that is not counted.  Returns (loss, choices per expert int64 [E], P
+    float32 [E], gradient of ``grad_scale`` * loss by the logits, or None without a ``grad_scale``)."""
+    loss, counts, mean_prob, grad = _balance(logits, indices, mask, grad_scale)
+    return loss, counts[:-2], mean_prob, grad
+
+
+def balance_grad(logits: torch.Tensor, counts: torch.Tensor, upstream: torch.Tensor, mask=None) -> torch.Tensor:
+    """Gradient of ``upstream`` (a float32 scalar on the device) * balance loss by the logits (gdpso_balance_grad); ``counts``
+    int64 [E + 2] as gdpso_balance leaves them: choices per expert, rows kept, choices counted."""
+    device, rows, mask = _loss_rows(logits, mask)
+    n, e = rows.shape
+    _same_device(device, counts=counts, upstream=upstream)
+    if counts.dtype != torch.int64 or counts.shape != (e + 2,) or not counts.is_contiguous():
+        raise ValueError(f"counts must be contiguous int64 [{e + 2}]")
+    if upstream.dtype != torch.float32 or upstream.numel() != 1:
+        raise ValueError("upstream must be a float32 scalar")
+    grad = torch.empty(n, e, dtype=rows.dtype, device=device)
+    with torch.cuda.device(device):
+        check(_lib.lib().gdpso_balance_grad(_lib.stream_handle(device), n, e, ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(mask), ptr(counts),
+                                            ptr(upstream), ptr(grad)))
+    return grad.reshape(logits.shape)
+
+
+def _distill_args(logits, teacher_logits, teacher_indices, mask):
+    device, rows, mask = _loss_rows(logits, mask)
+    idx = _row_indices(teacher_indices, logits.shape[:-1], device, "teacher_indices")
+    _same_device(device, teacher_logits=teacher_logits)
+    if teacher_logits.dtype not in _LOGIT_TYPES or teacher_logits.shape != teacher_indices.shape:
+        raise ValueError(f"teacher_logits must be floating point of the shape of teacher_indices {tuple(teacher_indices.shape)}, got "
+                         f"{teacher_logits.dtype} {tuple(teacher_logits.shape)}")
+    return device, rows, mask, idx, teacher_logits.detach().reshape(idx.shape).contiguous()
+
+
+def _distill(logits, teacher_logits, teacher_indices, mask, temperature, grad_scale):
+    device, rows, mask, idx, t = _distill_args(logits, teacher_logits, teacher_indices, mask)
+    (n, v), k = rows.shape, idx.shape[1]
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    row_loss = torch.empty(n, dtype=torch.float32, device=device)
+    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=device)
+    grad = None if grad_scale is None else torch.empty(n, v, dtype=rows.dtype, device=device)
+    L = _lib.lib()
+    with torch.cuda.device(device):
+        ws = torch.empty(L.gdpso_distill_workspace_bytes(n, v, k), dtype=torch.uint8, device=device)
+        check(L.gdpso_distill(_lib.stream_handle(device), n, v, k, ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(t), _dtype_code(t.dtype),
+                              ptr(idx), idx.element_size(), ptr(mask), temperature, 0.0 if grad_scale is None else grad_scale, ptr(loss), ptr(row_loss),
+                              ptr(stats), ptr(grad), ptr(ws), ws.numel()))
+    return loss, row_loss.reshape(logits.shape[:-1]), None if grad is None else grad.reshape(logits.shape), stats
+
+
+def distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, mask=None, temperature: float = 1.0, grad_scale=None):
+    """Distillation of a student's ``logits`` [..., V] from the k highest logits of a teacher (gdpso_distill):
+    ``teacher_logits`` and ``teacher_indices`` [..., k]; temperature^2 * KL(softmax of the teacher's kept logits || softmax of the
+    student's row), both over the temperature, averaged over the rows ``mask`` (bool [...]) keeps.  An index outside
+    [0, V) is an absent entry.  Returns (loss, loss of every row float32 [...], gradient of ``grad_scale`` * loss by the logits,
+    or None without a ``grad_scale``)."""
+    return _distill(logits, teacher_logits, teacher_indices, mask, temperature, grad_scale)[:3]
+
+
+def distill_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, row_stats: torch.Tensor, upstream: torch.Tensor,
+                 mask=None, temperature: float = 1.0) -> torch.Tensor:
+    """Gradient of ``upstream`` (a float32 scalar on the device) * distillation loss by the logits (gdpso_distill_grad);
+    ``row_stats`` float32 [2 n + 1] as gdpso_distill leaves them for the same logits and temperature."""
+    device, rows, mask, idx, t = _distill_args(logits, teacher_logits, teacher_indices, mask)
+    (n, v), k = rows.shape, idx.shape[1]
+    _same_device(device, row_stats=row_stats, upstream=upstream)
+    if row_stats.dtype != torch.float32 or row_stats.shape != (2 * n + 1,) or not row_stats.is_contiguous():
+        raise ValueError(f"row_stats must be contiguous float32 [{2 * n + 1}]")
+    if upstream.dtype != torch.float32 or upstream.numel() != 1:
+        raise ValueError("upstream must be a float32 scalar")
+    grad = torch.empty(n, v, dtype=rows.dtype, device=device)
+    with torch.cuda.device(device):
+        check(_lib.lib().gdpso_distill_grad(_lib.stream_handle(device), n, v, k, ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(t),
+                                            _dtype_code(t.dtype), ptr(idx), idx.element_size(), ptr(mask), temperature, ptr(row_stats), ptr(upstream),
+                                            ptr(grad)))
+    return grad.reshape(logits.shape)
+
+
 # -------------------------------------------------------------------- fitness settings
 @dataclass
 class FitnessSpec:

@@ -79,6 +79,24 @@ class VQEmbedding(nn.Module):
         z_q_x_bar = z_q_x_bar_.permute(0, 3, 1, 2).contiguous()
         return z_q_x, z_q_x_bar
 
+    def code_logits(self, z_e_x, temperature=1.0):
+        """z_e_x [B, D, H, W] -> float32 logits [B, H, W, K] of the soft assignment, differentiable in latents and codebook
+        (no counterpart in the reference, like the two losses below)."""
+        weight = self.embedding.weight
+        dtype = weight.dtype if weight.dtype in (torch.bfloat16, torch.float16) else torch.float32  # seeding may leave float64
+        return util_function.code_logits(z_e_x.permute(0, 2, 3, 1).to(dtype), weight.to(dtype), temperature)
+
+    def balance(self, z_e_x, temperature=1.0, mask=None):
+        """How evenly the latents use the codebook: (balance loss of the nearest codes under the soft assignment, int64 latents
+        per code [K], mean soft assignment [K]); the loss is 1 for an even use and reaches latents and codebook.
+        ``mask`` bool [B, H, W]: positions to leave out are False."""
+        return util_function.balance(self.code_logits(z_e_x, temperature), self(z_e_x), mask)
+
+    def distill(self, z_e_x, teacher_logits, teacher_indices, temperature=1.0, mask=None):
+        """Distillation loss of the soft assignment from a teacher's top code logits [B, H, W, k] (e.g. the ``topk`` of another
+        encoder's ``code_logits`` over the same codes)."""
+        return util_function.distill(self.code_logits(z_e_x), teacher_logits, teacher_indices, mask, temperature)
+
 
 class _SubNet(nn.Module):
     """Container for one sub-network's parameters that is callable like the reference's

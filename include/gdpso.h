@@ -355,6 +355,68 @@ int gdpso_vq_lookup(void *stream, int n, int d, int k, const float *codebook, co
 int gdpso_vq_nearest_static(void *stream, int n, int d, int k, const float *inputs, const float *codebook,
                             long long *indices, float *codes, float *best_dist);
 
+/* ------------------------------------------- soft assignment to codes, and losses over it
+ * The differentiable side of the vector quantisation above, for what is trained behind a swarm: latents against a
+ * codebook, a student against a teacher.  The reference trains its VQ-VAE through the hard assignment only
+ * (src/inverter/utils_vq_vae/util_function.py:6-70); these entry points have no counterpart there.  All buffers on the
+ * device, row-major; `dtype` (GDPSO_DTYPE_*) is the type of latents and codebook, or of the logits and their gradient.
+ * Sums, softmax statistics and code logits are fp32; a gradient is rounded once, when it is stored.  No call
+ * allocates, synchronises or reads anything back, so all can be captured into a HIP graph; results do not depend on the
+ * order in which workgroups run.
+ *
+ * gdpso_code_logits: logits[i,c] = (2 <x_i, code_c> - |code_c|^2) / temperature, fp32 [n, k]: minus the squared distance
+ * over the temperature up to a constant per row, so softmax over the codes is the soft assignment whose maximum
+ * gdpso_vq_nearest finds.  gdpso_code_logits_grad: given d loss / d logits (fp32 [n, k]), the gradients
+ *   grad_inputs[i]   = (2 / t) sum_c g[i,c] code_c
+ *   grad_codebook[c] = (2 / t) (sum_i g[i,c] x_i - code_c sum_i g[i,c])
+ * in `dtype`; either may be NULL.  d <= 4096, k <= 2^20, temperature in [1e-6, 1e6].  The workspace
+ * (gdpso_code_logits_grad_workspace_bytes) is needed for grad_codebook only. */
+int gdpso_code_logits(void *stream, int n, int d, int k, const void *inputs, const void *codebook, int dtype, float temperature,
+                      float *logits);
+size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k);
+int gdpso_code_logits_grad(void *stream, int n, int d, int k, const float *grad_logits, const void *inputs, const void *codebook,
+                           int dtype, float temperature, void *grad_inputs, void *grad_codebook, void *workspace,
+                           size_t workspace_bytes);
+
+/* Balance loss of n choices among e codes (experts, classes): with p_i = softmax(logits row i), P[c] = mean of p_i[c]
+ * over the rows kept, f[c] = share of the choices that fell on c,
+ *   loss = e * sum_c f[c] P[c]                          (1 when choices and probabilities are spread evenly)
+ *   grad[i,c] = grad_scale * (e / rows kept) * p_i[c] * (f[c] - sum_j f[j] p_i[j])
+ * (the choices themselves have no gradient).  row_stride: elements from one row of logits to the next; the gradient is
+ * contiguous.  indices [n, k]: int64 (index_bytes 8) or int32 (4); one outside [0, e) is not counted (a dropped
+ * choice).  mask [n] or NULL: rows whose byte is 0 are left out whatever they hold; their gradient is 0.  A kept row
+ * without a finite logit has p = 0 (its choices count); NaN and +inf propagate.  No row kept, or no choice counted: loss 0.
+ * Outputs: loss [1], counts int64 [e + 2] (choices per code, then the rows kept, then the choices counted), mean_prob
+ * [e] = P, grad [n, e] in `dtype` or NULL.  1 <= e <= GDPSO_BALANCE_MAX_E.  n == 0 is allowed.
+ * gdpso_balance_grad: the gradient alone from the counts of an earlier call, times the DEVICE scalar *upstream. */
+#define GDPSO_BALANCE_MAX_E 16384
+size_t gdpso_balance_workspace_bytes(int n, int e);
+int gdpso_balance(void *stream, int n, int e, int k, const void *logits, long long row_stride, int dtype, const void *indices,
+                  int index_bytes, const unsigned char *mask, float grad_scale, float *loss, long long *counts, float *mean_prob,
+                  void *grad, void *workspace, size_t workspace_bytes);
+int gdpso_balance_grad(void *stream, int n, int e, const void *logits, long long row_stride, int dtype, const unsigned char *mask,
+                       const long long *counts, const float *upstream, void *grad);
+
+/* Distillation from a teacher's top logits: q_i = softmax of the row's k teacher logits / t, p_i = softmax of the student's
+ * row of v logits / t,
+ *   row_loss[i] = t^2 sum_j q_ij (log q_ij - log p_i[index_ij]),   loss = mean of row_loss over the rows kept
+ *   grad[i,c] = grad_scale * (t / rows kept) * (p_i[c] - sum of q_ij over the j with index_ij == c)
+ * t_logits [n, k] of type t_dtype, t_indices [n, k] int64 or int32.  An entry whose index lies outside [0, v) is
+ * absent (rows with fewer than k entries); an index that appears twice adds up.  A row without an entry, or without a finite
+ * student logit, has loss 0 and gradient 0 but counts as kept; a teacher's entry on a column at -inf makes the loss
+ * +inf; NaN propagates.  mask as for gdpso_balance.  1 <= k <= GDPSO_DISTILL_MAX_K, temperature in [1e-6, 1e6].
+ * Outputs: loss [1], row_loss [n] (0 for rows left out), row_stats [2 n + 1] (what gdpso_distill_grad needs: maximum and
+ * sum of exponentials of every row, then one over the rows kept), grad [n, v] in `dtype`, contiguous, or NULL.
+ * gdpso_distill_grad: the gradient alone, times the DEVICE scalar *upstream. */
+#define GDPSO_DISTILL_MAX_K 1024
+size_t gdpso_distill_workspace_bytes(int n, int v, int k);
+int gdpso_distill(void *stream, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits,
+                  int t_dtype, const void *t_indices, int index_bytes, const unsigned char *mask, float temperature, float grad_scale,
+                  float *loss, float *row_loss, float *row_stats, void *grad, void *workspace, size_t workspace_bytes);
+int gdpso_distill_grad(void *stream, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits,
+                       int t_dtype, const void *t_indices, int index_bytes, const unsigned char *mask, float temperature,
+                       const float *row_stats, const float *upstream, void *grad);
+
 /* -------------------------------------------------------------------- measurement
  * No counterpart in the reference: a hook for benchmarks.  Between begin and end, every
  * launch of the implicit-GEMM convolution kernel (generator, assessor and encoder

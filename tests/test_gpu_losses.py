@@ -1,0 +1,504 @@
+"""Soft code assignment, balance loss and distillation on the GPU against their definitions in 64 bits
+(tests/loss_utils.py derives the bounds), at the sizes, strides and masks where they can go wrong."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from loss_utils import assert_within, balance64, code_logits64, distill64, store_error
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def eng():
+    return importlib.import_module("gan-discovery-pso_amd.engine")
+
+
+@pytest.fixture(scope="module")
+def fn():
+    return importlib.import_module("gan-discovery-pso_amd.inverter.utils_vq_vae.util_function")
+
+
+@pytest.fixture(scope="module")
+def model():
+    return importlib.import_module("gan-discovery-pso_amd.inverter.utils_vq_vae.util_model")
+
+
+def rand(seed, *shape, scale=1.0, dtype=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=gen) * scale).to(dtype).to(DEV)
+
+
+def randint(seed, lo, hi, *shape, dtype=torch.int64):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randint(lo, hi, shape, generator=gen).to(dtype).to(DEV)
+
+
+def check_balance(out, logits, idx, mask, scale):
+    loss, counts, mean_prob, grad = out
+    want = balance64(logits, idx, mask, 1.0 if scale is None else scale)
+    assert loss.dtype == mean_prob.dtype == torch.float32 and counts.dtype == torch.int64
+    assert torch.equal(counts.cpu(), want[1])
+    assert_within(mean_prob, want[2], want[5] + store_error(want[2], torch.float32), "mean_prob")
+    assert_within(loss, want[0], want[4] + store_error(want[0], torch.float32), "loss")
+    if scale is None:
+        assert grad is None
+    else:
+        assert grad.dtype == logits.dtype and grad.shape == logits.shape and grad.is_contiguous()
+        assert_within(grad, want[3], want[6] + store_error(want[3], logits.dtype), "grad")
+
+
+def check_distill(out, logits, t_logits, t_idx, mask, t, scale):
+    loss, row, grad = out
+    want = distill64(logits, t_logits, t_idx, mask, t, 1.0 if scale is None else scale)
+    assert loss.dtype == row.dtype == torch.float32
+    assert_within(row, want[1], want[4] + store_error(want[1], torch.float32), "row_loss")
+    assert_within(loss, want[0], want[3] + store_error(want[0], torch.float32), "loss")
+    if scale is None:
+        assert grad is None
+    else:
+        assert grad.dtype == logits.dtype and grad.shape == logits.shape and grad.is_contiguous()
+        assert_within(grad, want[2], want[5] + store_error(want[2], logits.dtype), "grad")
+
+
+# ------------------------------------------------------------------------------------------------- code logits
+CODE_SIZES = [(1, 1, 1), (1, 512, 64), (5, 37, 3), (512, 256, 100), (67, 130, 257), (33, 1000, 16), (130, 8, 1030), (1025, 65, 33),
+              (2049, 128, 128), (300, 129, 40), (7, 64, 4096)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k,d", CODE_SIZES)
+def test_code_logits(eng, n, k, d, dtype):
+    x, code = rand(n, n, d, dtype=dtype), rand(k + 1, k, d, dtype=dtype)
+    s = eng.code_logits(x, code, temperature=1.7)
+    want, bound = code_logits64(x, code, 1.7)
+    assert s.dtype == torch.float32 and tuple(s.shape) == (n, k)
+    assert_within(s, want, bound + store_error(want, torch.float32))
+    g = rand(d + 2, n, k)
+    dx, dcode = eng.code_logits_grad(g, x, code, temperature=1.7)
+    wx, bx, wc, bc = code_logits64(x, code, 1.7, g)
+    assert dx.dtype == dcode.dtype == dtype and dx.shape == x.shape and dcode.shape == code.shape
+    assert_within(dx, wx, bx + store_error(wx, dtype), "dx")
+    assert_within(dcode, wc, bc + store_error(wc, dtype), "dcode")
+    only_x, none = eng.code_logits_grad(g, x, code, temperature=1.7, want_codebook=False)
+    none2, only_c = eng.code_logits_grad(g, x, code, temperature=1.7, want_inputs=False)
+    assert none is None and none2 is None and torch.equal(only_x, dx) and torch.equal(only_c, dcode)
+
+
+def test_code_logits_shapes(eng):
+    code = rand(1, 37, 16)
+    nchw = rand(2, 2, 16, 5, 3)
+    x = nchw.permute(0, 2, 3, 1)  # channels last by strides only
+    s = eng.code_logits(x, code)
+    assert tuple(s.shape) == (2, 5, 3, 37)
+    assert torch.equal(s, eng.code_logits(x.contiguous(), code))
+    wide = rand(3, 37, 40)[:, 7:23]  # codebook with gaps between rows, off alignment
+    assert torch.equal(eng.code_logits(x, wide), eng.code_logits(x, wide.contiguous()))
+    odd = rand(4, 1 + 30 * 16)[1:].reshape(30, 16)  # base address off 16 bytes
+    assert torch.equal(eng.code_logits(odd, code), eng.code_logits(odd.clone(), code))
+    g = rand(5, 37, 30).t()
+    a, b = eng.code_logits_grad(g, odd, code), eng.code_logits_grad(g.contiguous(), odd.clone(), code)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for lead in [(0,), (3, 0)]:
+        empty = torch.empty(*lead, 16, device=DEV)
+        s = eng.code_logits(empty, code)
+        assert tuple(s.shape) == (*lead, 37)
+        dx, dcode = eng.code_logits_grad(s, empty, code)
+        assert dx.shape == empty.shape and torch.equal(dcode, torch.zeros_like(code))
+
+
+def test_code_logits_rank_the_nearest_code(eng):
+    x, code = rand(1, 4099, 100), rand(2, 256, 100)
+    idx = eng.vq_nearest(x, code)[0]
+    s = eng.code_logits(x, code)
+    best = s.amax(dim=1)
+    chosen = s.gather(1, idx[:, None])[:, 0]
+    _, bound = code_logits64(x, code, 1.0)
+    scale = 4 * bound.amax(dim=1).to(DEV).float() + 1e-5 * (x * x).sum(dim=1)  # both searches round
+    assert bool((best - chosen <= scale).all())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_code_logits_keep_bad_values_to_their_rows(eng, bad):
+    x, code = rand(1, 70, 24), rand(2, 40, 24)
+    clean = eng.code_logits(x, code)
+    x2 = x.clone()
+    x2[33, 5] = bad
+    s = eng.code_logits(x2, code)
+    rows = torch.arange(70, device=DEV) != 33
+    assert torch.equal(s[rows], clean[rows]) and not bool(s[33].isfinite().any())
+
+
+# ------------------------------------------------------------------------------------------------- balance loss
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,e,k", [(1, 1, 1), (1, 8, 2), (3, 2, 1), (1, 256, 1), (515, 7, 3), (512, 8, 8), (64, 37, 2), (1000, 64, 2), (77, 100, 1),
+                                   (512, 256, 1), (131, 257, 4), (513, 512, 1), (40, 1001, 2), (33, 1024, 1), (65, 2048, 3), (9, 2050, 1), (5, 5000, 2),
+                                   (3, 16384, 8), (5000, 16, 2), (20000, 5, 1)])
+def test_balance(eng, n, e, k, dtype):
+    logits = rand(n + e, n, e, scale=2.0, dtype=dtype)
+    idx = randint(k, 0, e, n, k)
+    mask = randint(n, 0, 4, n) > 0
+    check_balance(eng.balance(logits, idx), logits, idx, None, None)
+    check_balance(eng.balance(logits, idx, grad_scale=3.0), logits, idx, None, 3.0)
+    check_balance(eng.balance(logits, idx, mask=mask, grad_scale=float(n)), logits, idx, mask, float(n))
+
+
+def test_balance_of_an_even_use_is_one(eng):
+    out = eng.balance(torch.zeros(64, 16, device=DEV), torch.arange(64, device=DEV) % 16, grad_scale=1.0)
+    assert float(out[0]) == 1.0 and out[1].tolist() == [4] * 16 and not bool(out[3].any())
+
+
+@pytest.mark.parametrize("e", [8, 100, 513, 3000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_balance_masks(eng, e, dtype):
+    n, k = 70, 2
+    logits = rand(e, n, e, dtype=dtype)
+    logits[0] = -math.inf                       # no finite logit: p = 0, its choices count
+    logits[1, 1:] = -math.inf                   # one expert left
+    logits[2] = torch.finfo(dtype).min          # a mask of the type's lowest value: even
+    logits[3, : e // 2] = torch.finfo(dtype).min
+    logits[4] = torch.finfo(dtype).max
+    idx = randint(3, 0, e, n, k)
+    idx[5, 0], idx[6, 1], idx[7, 0], idx[8, 0] = -1, e, 2 ** 40, -(2 ** 40)  # choices that are dropped
+    check_balance(eng.balance(logits, idx, grad_scale=1.0), logits, idx, None, 1.0)
+    check_balance(eng.balance(logits, idx.clamp(-1, e).int(), grad_scale=1.0), logits, idx, None, 1.0)  # int32
+    mask = torch.ones(n, dtype=torch.bool, device=DEV)
+    mask[9:13] = False
+    dirty, clean = logits.clone(), logits.clone()
+    dirty[9], dirty[10], dirty[11] = math.nan, math.inf, -math.inf
+    clean[9:12] = 0
+    a, b = eng.balance(dirty, idx, mask=mask, grad_scale=1.0), eng.balance(clean, idx, mask=mask, grad_scale=1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and not bool(a[3][9:13].any())
+    check_balance(a, clean, idx, mask, 1.0)
+    none = eng.balance(dirty, idx, mask=torch.zeros_like(mask), grad_scale=1.0)
+    assert float(none[0]) == 0 and not any(bool(t.any()) for t in none[1:])
+    no_choice = eng.balance(clean, torch.full_like(idx, -1), grad_scale=1.0)
+    assert float(no_choice[0]) == 0 and not bool(no_choice[1].any()) and not bool(no_choice[3].any())
+
+
+@pytest.mark.parametrize("e", [6, 200, 5000])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_balance_propagates(eng, e, bad):
+    logits = rand(1, 12, e)
+    idx = randint(2, 0, e, 12)
+    logits[3, 2] = bad
+    loss, counts, mean_prob, grad = eng.balance(logits, idx, grad_scale=1.0)
+    assert math.isnan(float(loss)) and int(counts.sum()) == 12 and bool(mean_prob.isnan().any())
+    rows = torch.arange(12, device=DEV) != 3
+    assert bool(grad[3].isnan().any()) and bool(grad[rows].isfinite().all())
+    all_nan = torch.full((2, e), math.nan, device=DEV)
+    assert math.isnan(float(eng.balance(all_nan, idx[:2])[0]))
+
+
+def test_balance_strides_and_shapes(eng):
+    for dtype in DTYPES:
+        wide = rand(1, 40, 77, dtype=dtype)
+        idx = randint(2, 0, 50, 40)
+        for view in (wide[:, 3:53], wide[:, :50], wide[::2, 1:51]):
+            i = idx[: view.shape[0]]
+            a, b = eng.balance(view, i, grad_scale=1.0), eng.balance(view.clone(), i, grad_scale=1.0)
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    one = rand(3, 1, 50)
+    a, b = eng.balance(one.expand(40, 50), idx, grad_scale=1.0), eng.balance(one.repeat(40, 1), idx, grad_scale=1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    t = rand(4, 50, 40).t()
+    a, b = eng.balance(t, idx, grad_scale=1.0), eng.balance(t.contiguous(), idx, grad_scale=1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    cube = rand(5, 4, 10, 50)
+    a = eng.balance(cube, idx.reshape(4, 10), mask=torch.ones(4, 10, dtype=torch.bool, device=DEV), grad_scale=1.0)
+    b = eng.balance(cube.reshape(40, 50), idx[:, None], grad_scale=1.0)
+    assert a[3].shape == cube.shape and torch.equal(a[3].reshape(40, 50), b[3]) and torch.equal(a[0], b[0])
+    empty = eng.balance(torch.empty(0, 50, device=DEV), torch.empty(0, 2, dtype=torch.int64, device=DEV), grad_scale=1.0)
+    assert float(empty[0]) == 0 and not bool(empty[1].any()) and tuple(empty[3].shape) == (0, 50)
+
+
+# ------------------------------------------------------------------------------------------------- distillation
+def teacher_of(logits, k, seed, noise=1.0):
+    top = (logits.float() + noise * rand(seed, *logits.shape)).topk(k, dim=-1)
+    return top.values.to(logits.dtype), top.indices
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,k", [(1, 1, 1), (1, 8, 4), (512, 8, 4), (3, 2, 2), (65, 7, 7), (130, 64, 1), (33, 100, 16), (50, 511, 16), (257, 512, 64),
+                                   (17, 1000, 128), (20, 1025, 5), (9, 2048, 2), (10, 2049, 64), (5, 8191, 300), (3, 30011, 64), (2, 50007, 1024), (1, 131072, 128),
+                                   (12, 131072, 64), (300, 8200, 8), (2, 200003, 16)])
+def test_distill(eng, n, v, k, dtype):
+    logits = rand(n + v, n, v, scale=2.0, dtype=dtype)
+    t_logits, t_idx = teacher_of(logits, k, v)
+    mask = randint(n + 1, 0, 4, n) > 0
+    check_distill(eng.distill(logits, t_logits, t_idx), logits, t_logits, t_idx, None, 1.0, None)
+    check_distill(eng.distill(logits, t_logits, t_idx, grad_scale=float(n)), logits, t_logits, t_idx, None, 1.0, float(n))
+    check_distill(eng.distill(logits, t_logits.float(), t_idx, mask=mask, temperature=2.5, grad_scale=float(n)), logits, t_logits, t_idx, mask, 2.5, float(n))
+
+
+@pytest.mark.parametrize("v", [8, 100, 700, 5000, 40000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distill_masks(eng, v, dtype):
+    n, k = 40, 6
+    logits = rand(v, n, v, dtype=dtype)
+    t_logits, t_idx = teacher_of(logits, k, 3)
+    logits[0] = -math.inf                                     # nothing to teach: loss 0, gradient 0
+    lowest = torch.finfo(dtype).min
+    logits[2] = lowest                                        # every logit the type's lowest value: even
+    t_idx[3] = -1                                             # no entry
+    t_idx[4, 2:] = -1                                         # two entries
+    t_idx[5, 0], t_idx[5, 1] = v, 2 ** 40                     # out of range
+    t_logits[6, 1:] = -math.inf                               # one entry with all the weight
+    t_logits[7] = -math.inf                                   # entries without weight
+    t_idx[8, 1:] = t_idx[8, 0]                                # one column named by every entry
+    t_idx[9, 3] = t_idx[9, 1]
+    t_idx[9, 5] = t_idx[9, 1]
+    t_logits[10] = 1.0
+    for t in (1.0, 0.5):
+        check_distill(eng.distill(logits, t_logits, t_idx, temperature=t, grad_scale=1.0 * n), logits, t_logits, t_idx, None, t, 1.0 * n)
+    out32 = eng.distill(logits, t_logits, t_idx.clamp(-1, v).int(), grad_scale=1.0)
+    assert all(torch.equal(a, b) for a, b in zip(out32, eng.distill(logits, t_logits, t_idx, grad_scale=1.0)))
+    mask = torch.ones(n, dtype=torch.bool, device=DEV)
+    mask[11:15] = False
+    dirty, dirty_t, clean = logits.clone(), t_logits.clone(), logits.clone()
+    dirty[11], dirty[12], dirty[13], dirty_t[14] = math.nan, math.inf, -math.inf, math.nan
+    clean[11:14] = 0
+    a = eng.distill(dirty, dirty_t, t_idx, mask=mask, grad_scale=1.0)
+    b = eng.distill(clean, t_logits, t_idx, mask=mask, grad_scale=1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and not bool(a[2][11:15].any()) and not bool(a[1][11:15].any())
+    check_distill(a, clean, t_logits, t_idx, mask, 1.0, 1.0)
+    none = eng.distill(dirty, dirty_t, t_idx, mask=torch.zeros_like(mask), grad_scale=1.0)
+    assert not any(bool(t.any()) for t in none)
+
+
+@pytest.mark.parametrize("v", [20, 3000, 70000])
+def test_distill_propagates(eng, v):
+    logits = rand(1, 10, v)
+    t_logits, t_idx = teacher_of(logits, 4, 2)
+    logits[2, 5] = math.nan
+    logits[3, 6] = math.inf
+    logits[4, t_idx[4, 1]] = -math.inf  # the teacher gives weight to a column that the student cannot reach
+    t_logits[5, 0] = math.nan
+    logits[6] = math.nan
+    loss, row, grad = eng.distill(logits, t_logits, t_idx, grad_scale=1.0)
+    assert [bool(r.isnan()) for r in row] == [i in (2, 3, 5, 6) for i in range(10)]
+    assert float(row[4]) == math.inf and bool(grad[4].isfinite().all()) and bool(loss.isnan())
+    clean = [0, 1, 7, 8, 9]
+    want = distill64(logits[clean], t_logits[clean], t_idx[clean], None, 1.0, 0.5)
+    assert_within(row[clean], want[1], want[4] + store_error(want[1], torch.float32))
+    assert_within(grad[clean], want[2], want[5] + store_error(want[2], torch.float32))
+
+
+def test_distill_strides_and_shapes(eng):
+    for dtype in DTYPES:
+        for v in (50, 2100):
+            wide = rand(1, 40, v + 27, dtype=dtype)
+            for view in (wide[:, 3:v + 3], wide[:, :v], wide[::2, 1:v + 1]):
+                t_logits, t_idx = teacher_of(view, 5, 2)
+                a, b = eng.distill(view, t_logits, t_idx, grad_scale=9.0), eng.distill(view.clone(), t_logits, t_idx, grad_scale=9.0)
+                assert all(torch.equal(p, q) for p, q in zip(a, b))
+    one = rand(3, 1, 50)
+    t_logits, t_idx = teacher_of(rand(4, 40, 50), 5, 2)
+    a, b = eng.distill(one.expand(40, 50), t_logits, t_idx, grad_scale=1.0), eng.distill(one.repeat(40, 1), t_logits, t_idx, grad_scale=1.0)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    cube = rand(5, 4, 10, 50)
+    a = eng.distill(cube, t_logits.reshape(4, 10, 5), t_idx.reshape(4, 10, 5), grad_scale=1.0)
+    b = eng.distill(cube.reshape(40, 50), t_logits, t_idx, grad_scale=1.0)
+    assert a[1].shape == (4, 10) and a[2].shape == cube.shape and torch.equal(a[2].reshape(40, 50), b[2]) and torch.equal(a[0], b[0])
+    a = eng.distill(one.reshape(50), t_logits[0], t_idx[0], grad_scale=1.0)  # one row without a batch
+    assert a[1].shape == () and a[2].shape == (50,)
+    empty = eng.distill(torch.empty(0, 50, device=DEV), torch.empty(0, 3, device=DEV), torch.empty(0, 3, dtype=torch.int64, device=DEV), grad_scale=1.0)
+    assert float(empty[0]) == 0 and empty[1].numel() == 0 and tuple(empty[2].shape) == (0, 50)
+
+
+def test_offsets_beyond_32_bits(eng):
+    """33,000 rows of 131,072 logits are 4.3e9 elements: the last rows come out as in a small call."""
+    n, v, k = 33000, 131072, 4
+    logits = torch.zeros(n, v, dtype=torch.bfloat16, device=DEV)
+    t_idx = torch.zeros(n, k, dtype=torch.int64, device=DEV) + torch.arange(k, device=DEV) * 1000
+    t_logits = torch.ones(n, k, device=DEV)
+    tail = rand(1, 3, v, dtype=torch.bfloat16)
+    logits[-3:] = tail
+    _, row, grad = eng.distill(logits, t_logits, t_idx, grad_scale=float(n))
+    small = eng.distill(tail, t_logits[:3], t_idx[:3], grad_scale=3.0)
+    assert torch.equal(row[-3:], small[1])
+    # both gradients are (temperature = 1) times rows / rows, the one factor's rounding apart
+    assert bool(((grad[-3:].float() - small[2].float()).abs() <= small[2].float().abs() * 2 ** -7 + 2.0 ** -133).all())
+    del grad
+    e = 16384
+    view = logits.reshape(-1, e)  # 264,000 rows of 16,384
+    idx = torch.zeros(view.shape[0], dtype=torch.int64, device=DEV)
+    _, counts, mean_prob, grad = eng.balance(view, idx, grad_scale=float(view.shape[0]))
+    assert int(counts[0]) == view.shape[0] and abs(float(mean_prob.double().sum()) - 1) < 1e-3
+    p = torch.softmax(tail.reshape(-1, e).double(), dim=1)
+    f = torch.zeros(e, dtype=torch.float64, device=DEV)
+    f[0] = 1
+    want = e * p * (f - p[:, :1])
+    got = grad[-p.shape[0]:].double()
+    assert bool(((got - want).abs() <= want.abs() * 2 ** -7 + 2.0 ** -133).all())
+
+
+# ------------------------------------------------------------------------------------------------ run to run
+def test_results_repeat_bit_for_bit(eng):
+    x, code = rand(1, 5000, 64), rand(2, 512, 64)
+    idx = eng.vq_nearest(x, code)[0]
+
+    def once():
+        s = eng.code_logits(x, code, temperature=20.0)
+        b = eng.balance(s, idx, grad_scale=1.0)
+        top = s.flip(0).topk(16, dim=1)
+        d = eng.distill(s, top.values, top.indices, grad_scale=1.0)
+        return [s, *b, *d, *eng.code_logits_grad(b[3] + d[2], x, code, temperature=20.0)]
+
+    first = once()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, once()))
+
+
+def test_on_another_stream(eng):
+    logits = rand(1, 3000, 300)
+    t_logits, t_idx = teacher_of(logits, 8, 2)
+    want = eng.distill(logits, t_logits, t_idx, grad_scale=1.0), eng.balance(logits, t_idx, grad_scale=1.0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = eng.distill(logits, t_logits, t_idx, grad_scale=1.0), eng.balance(logits, t_idx, grad_scale=1.0)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_captured_steps_replay(eng):
+    """Two graphs of a whole training step, replayed in turn with new inputs and eager work between: every replay equals the
+    eager result on the same inputs."""
+    def step(x, code, idx, t_logits, t_idx, mask):
+        s = eng.code_logits(x, code, temperature=30.0)
+        b = eng.balance(s, idx, mask=mask, grad_scale=0.1)
+        d = eng.distill(s, t_logits, t_idx, mask=mask, grad_scale=1.0)
+        return [s, *b, *d, *eng.code_logits_grad(b[3] + d[2], x, code, temperature=30.0)]
+
+    def inputs(seed, n):
+        x, code = rand(seed, n, 64), rand(seed + 1, 512, 64)
+        s = rand(seed + 2, n, 512)
+        top = s.topk(12, dim=1)
+        return [x, code, randint(seed + 3, 0, 512, n), top.values, top.indices, randint(seed + 4, 0, 5, n) > 0]
+
+    graphs = []
+    for n in (700, 2311):
+        static = inputs(n, n)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((n, static, graph, out))
+    for turn in range(3):
+        for n, static, graph, out in graphs:
+            fresh = inputs(1000 * turn + n, n)
+            for a, b in zip(static, fresh):
+                a.copy_(b)
+            graph.replay()
+            want = step(*fresh)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), (turn, n)
+
+
+# ---------------------------------------------------------------------------------------------------- autograd
+def test_autograd_forms(eng, fn):
+    for dtype in DTYPES:
+        x, code = rand(1, 90, 48, dtype=dtype).requires_grad_(), rand(2, 70, 48, dtype=dtype).requires_grad_()
+        s = fn.code_logits(x, code, 9.0)
+        g = rand(3, 90, 70)
+        got = torch.autograd.grad(s, (x, code), g)
+        assert all(torch.equal(a, b) for a, b in zip(got, eng.code_logits_grad(g, x, code, 9.0)))
+        logits = rand(4, 90, 70, dtype=dtype).requires_grad_()
+        idx, mask = randint(5, 0, 70, 90, 2), randint(6, 0, 3, 90) > 0
+        loss, counts, mean_prob = fn.balance(logits, idx, mask)
+        ref = eng.balance(logits, idx, mask=mask, grad_scale=4.0)
+        assert torch.equal(loss, ref[0]) and torch.equal(counts, ref[1]) and torch.equal(mean_prob, ref[2])
+        assert not counts.requires_grad and not mean_prob.requires_grad
+        (4.0 * loss).backward(retain_graph=True)
+        assert torch.equal(logits.grad, ref[3])
+        logits.grad = None
+        (4.0 * loss).backward()  # the saved tensors serve a second pass
+        assert torch.equal(logits.grad, ref[3])
+        logits.grad = None
+        t_logits, t_idx = teacher_of(logits.detach(), 6, 7)
+        loss = fn.distill(logits, t_logits, t_idx, mask, 2.0)
+        ref = eng.distill(logits, t_logits, t_idx, mask=mask, temperature=2.0, grad_scale=8.0)
+        assert torch.equal(loss, ref[0])
+        (8.0 * loss).backward()
+        assert torch.equal(logits.grad, ref[2])
+
+
+def test_gradients_against_differences(eng):
+    """Central differences of the definitions in 64 bits."""
+    n, e = 6, 9
+    logits, idx = rand(1, n, e), randint(2, 0, e, n, 2)
+    t_logits, t_idx = teacher_of(rand(3, n, e), 4, 4)
+    grads = eng.balance(logits, idx, grad_scale=1.0)[3], eng.distill(logits, t_logits, t_idx, temperature=1.5, grad_scale=1.0)[2]
+    h = 1e-5
+    for which, grad in enumerate(grads):
+        for i in range(n):
+            for c in range(e):
+                vals = []
+                for sign in (1, -1):
+                    x = logits.double().cpu()
+                    x[i, c] += sign * h
+                    vals.append(float(balance64(x, idx)[0] if which == 0 else distill64(x, t_logits, t_idx, None, 1.5)[0]))
+                diff = (vals[0] - vals[1]) / (2 * h)
+                # differences are good to h^2 and 2^-53 / h, the fp32 gradient to 1e-5 of values below 9
+                assert abs(diff - float(grad[i, c])) < 1e-6
+
+
+def test_training_step_through_the_codebook(model):
+    """VQEmbedding: latents and codebook receive the gradients of both losses over their soft assignment, as in the definitions
+    differentiated in 64 bits."""
+    b, d, h, w, k = 6, 32, 4, 3, 48
+    emb = model.VQEmbedding(k, d, None).to(DEV)
+    emb.embedding.weight.data.copy_(rand(1, k, d))
+    z = rand(2, b, d, h, w).requires_grad_()
+    teacher = emb.code_logits(rand(3, b, d, h, w)).detach().topk(5, dim=-1)
+    mask = randint(4, 0, 4, b, h, w) > 0
+    even, counts, mean_prob = emb.balance(z, temperature=16.0, mask=mask)
+    kd = emb.distill(z, teacher.values, teacher.indices, temperature=16.0, mask=mask)
+    (even + 0.5 * kd).backward()
+    assert int(counts.sum()) == int(mask.sum())
+    z64 = z.detach().double().cpu().requires_grad_()
+    c64 = emb.embedding.weight.detach().double().cpu().requires_grad_()
+    x = z64.permute(0, 2, 3, 1).reshape(-1, d)
+    s = 2 * x @ c64.t() - (c64 * c64).sum(dim=1)
+    keep = mask.cpu().reshape(-1)
+    idx = emb(z).cpu().reshape(-1)
+    p = torch.softmax(s / 16.0, dim=1)[keep]
+    f = torch.bincount(idx[keep], minlength=k).double() / int(keep.sum())
+    want_even = k * (f * p.mean(dim=0)).sum()
+    log_q = torch.log_softmax(teacher.values.double().cpu().reshape(-1, 5) / 16.0, dim=1)
+    log_p = torch.log_softmax(s / 16.0, dim=1).gather(1, teacher.indices.cpu().reshape(-1, 5))
+    want_kd = 256.0 * ((log_q.exp() * (log_q - log_p)).sum(dim=1)[keep]).mean()
+    (want_even + 0.5 * want_kd).backward()
+    assert torch.equal(counts.cpu(), torch.bincount(idx[keep], minlength=k))
+    # logits of magnitude 100 carry 100 * 36 u into p; both losses and their gradients stay within 1e-3 of their own size
+    assert abs(even.item() - want_even.item()) < 1e-3 and abs(kd.item() - want_kd.item()) < 1e-3 * want_kd.item()
+    for got, want in ((z.grad, z64.grad), (emb.embedding.weight.grad, c64.grad)):
+        assert float((got.cpu().double() - want).norm()) < 1e-3 * float(want.norm())
+
+
+def test_float64_codebook_of_a_seeded_embedding(model):
+    emb = model.VQEmbedding(16, 8, torch.randn(16, 8, dtype=torch.float64).numpy()).to(DEV)
+    assert emb.code_logits(rand(1, 2, 8, 1, 1)).shape == (2, 1, 1, 16)
+
+
+# -------------------------------------------------------------------------------------------------- no CPU fallback
+def test_no_cpu_fallback(eng):
+    err = importlib.import_module("gan-discovery-pso_amd._lib").GdpsoError
+    with pytest.raises(err):
+        eng.code_logits(torch.zeros(2, 4), torch.zeros(3, 4))
+    with pytest.raises(err):
+        eng.balance(torch.zeros(2, 4), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(err):
+        eng.distill(torch.zeros(2, 4), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        eng.balance(torch.zeros(2, 4, device=DEV), torch.zeros(2, dtype=torch.int64))
