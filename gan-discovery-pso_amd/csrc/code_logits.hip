@@ -6,6 +6,13 @@
 //   d code_c  = (2 / t) (sum_i g[i,c] x_i - code_c sum_i g[i,c])
 //
 // Three products; the logits and their gradient are fp32 whatever the type of latents and codes, and so is every sum.
+//
+// The products run on the 16-bit matrix instructions, sixteen times the rate of the fp32 ones, without giving up
+// fp32 accuracy: a value is cut into bf16 parts, each the rounded rest of the one before, so that an fp32 value is three
+// parts (3 x 8 bits), an fp16 value two, a bf16 value itself, and the product of two values is the sum of the products of
+// their parts.  Those of order 2^-24 and below are left out (two middle parts of order 2^-16 are kept): six matrix
+// instructions for fp32 x fp32, five for fp32 x fp16, three for fp32 x bf16.  Parts multiply exactly and add up in fp32.  The
+// forward product of two 16-bit operands needs no cutting.
 #include "common.h"
 
 #include <math.h>
@@ -13,89 +20,359 @@
 namespace gdpso {
 namespace {
 
-constexpr int T = 16;  // output tile of a workgroup of T x T threads
 constexpr int CL_MAX_D = 4096;
+constexpr int CL_THREADS = 256;  // four waves, two by two over the output tile
+constexpr int KT = 32;           // K elements a stage: one 16x16x32 matrix instruction deep
+// LDS elements from one row of a stage to the next: 80 bytes put the sixteen rows of a fragment read on disjoint banks
+constexpr int LROW = KT + 8;
 
+using bf16x8 = __attribute__((ext_vector_type(8))) bf16_t;
+using f16x8 = __attribute__((ext_vector_type(8))) f16_t;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+
+// Vectors at element alignment: rows of any length and offset (global memory takes unaligned vector accesses).
+template <typename E, int N>
+struct VecAt {
+    typedef E type __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+};
 template <typename E>
-__global__ __launch_bounds__(T *T) void code_logits_kernel(int n, int d, int k, const E *__restrict__ x, const E *__restrict__ cb, float inv_t,
-                                                           float *__restrict__ out) {
-    __shared__ float s_x[T][T + 1], s_c[T][T + 1];
-    const int tx = threadIdx.x % T, ty = threadIdx.x / T;
-    const long i0 = (long)blockIdx.x * T;
-    const int c0 = blockIdx.y * T;
-    float acc = 0.f, sq = 0.f;
-    for (int j0 = 0; j0 < d; j0 += T) {
-        s_x[ty][tx] = i0 + ty < n && j0 + tx < d ? (float)x[(i0 + ty) * d + j0 + tx] : 0.f;
-        s_c[ty][tx] = c0 + ty < k && j0 + tx < d ? (float)cb[(size_t)(c0 + ty) * d + j0 + tx] : 0.f;
+struct VecAt<E, 1> {
+    typedef E type;
+};
+
+enum Product { LOGITS, GRAD_X, GRAD_CODE };
+
+// One operand of the product: BR rows of the output's side by KT of the summed side per stage, carried from global
+// memory through registers (so that the loads of a stage are under way while the one before multiplies) into P planes of
+// 16-bit parts in LDS, [P][BR][LROW].  ROW: the summed side is the contiguous one; else the output's side is, and the
+// eight values of a fragment are gathered from eight rows of memory in the registers of one thread.
+template <typename E, bool ROW, int BR, int P, typename M>
+struct Operand {
+    static constexpr int CW = ROW ? 1 : (BR * 4 > CL_THREADS ? BR * 4 / CL_THREADS : 1);  // columns a unit
+    static constexpr int UNITS = BR * 4 / CW;
+    static constexpr int NU = (UNITS + CL_THREADS - 1) / CL_THREADS;
+    E v[NU][CW][8];
+
+    __device__ __forceinline__ static bool unit(int i, int &row, int &kc) {
+        const int u = threadIdx.x + i * CL_THREADS;
+        if constexpr (ROW) {
+            row = u >> 2;
+            kc = u & 3;
+        } else {
+            row = u % (BR / CW) * CW;
+            kc = u / (BR / CW);
+        }
+        return UNITS % CL_THREADS == 0 || u < UNITS;
+    }
+    // rows [row0, rows) and summed indices [k0, kend) of p, rows beyond and indices beyond read as 0
+    __device__ __forceinline__ void load(const E *__restrict__ p, long ld, long row0, long rows, long k0, long kend) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            int r, kc;
+            if (!unit(i, r, kc)) continue;
+            const long row = row0 + r, k = k0 + kc * 8;
+            if constexpr (ROW) {
+                const E *q = p + row * ld + k;
+                if (row < rows && k + 8 <= kend) {
+                    constexpr int W = 16 / sizeof(E);
+#pragma unroll
+                    for (int w = 0; w < 8 / W; ++w) {
+                        const auto x = *(const typename VecAt<E, W>::type *)(q + w * W);
+#pragma unroll
+                        for (int e = 0; e < W; ++e) v[i][0][w * W + e] = x[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][0][e] = row < rows && k + e < kend ? q[e] : (E)0.f;
+                }
+            } else {
+                const E *q = p + k * ld + row;
+                if (row + CW <= rows && k + 8 <= kend) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const auto x = *(const typename VecAt<E, CW>::type *)(q + e * ld);
+                        if constexpr (CW == 1) v[i][0][e] = x;
+                        else
+#pragma unroll
+                            for (int c = 0; c < CW; ++c) v[i][c][e] = x[c];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+#pragma unroll
+                        for (int c = 0; c < CW; ++c) v[i][c][e] = row + c < rows && k + e < kend ? q[e * ld + c] : (E)0.f;
+                }
+            }
+        }
+    }
+    // sums[i][c]: running sums of the values (SQUARE: of their squares)
+    template <bool SQUARE>
+    __device__ __forceinline__ void add_up(float (&sums)[NU][CW]) const {
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int c = 0; c < CW; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = (float)v[i][c][e];
+                    sums[i][c] = SQUARE ? fmaf(x, x, sums[i][c]) : sums[i][c] + x;
+                }
+    }
+    __device__ __forceinline__ void store(M *lds) const {
+        using V = __attribute__((ext_vector_type(8))) M;
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            int r, kc;
+            if (!unit(i, r, kc)) continue;
+#pragma unroll
+            for (int c = 0; c < CW; ++c) {
+                M *dst = lds + (r + c) * LROW + kc * 8;
+                if constexpr (sizeof(E) == 2 && P == 1) {
+                    V x;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = v[i][c][e];
+                    *(V *)dst = x;
+                } else {
+                    float rest[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) rest[e] = (float)v[i][c][e];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        V x;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = (M)rest[e];
+                        *(V *)(dst + p * BR * LROW) = x;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float hi = (float)x[e];
+                            rest[e] = __builtin_isinf(hi) ? 0.f : rest[e] - hi;  // inf has no rest (inf - inf would make it NaN)
+                        }
+                    }
+                }
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+struct ProductArgs {
+    const void *m, *n;  // operands: output rows' side and output columns' side
+    void *out;          // LOGITS, GRAD_X: result; GRAD_CODE: partial sums [split][rows * cols + rows]
+    long rows, cols, sum;
+    long ld_m, ld_n;
+    int tiles_m, tiles_n, splits;
+    long sum_per_split;  // a multiple of KT
+    float scale;
+};
+
+template <Product OP, typename EM, typename EN, int PM, int PN, typename M, int BM, int BN, typename EO>
+__global__ __launch_bounds__(CL_THREADS) void product_kernel(ProductArgs a) {
+    constexpr bool ROW_M = OP != GRAD_CODE, ROW_N = OP == LOGITS;
+    constexpr int MT = BM / 32, NT = BN / 32;  // 16 x 16 tiles of a wave
+    using V = __attribute__((ext_vector_type(8))) M;
+    __shared__ __attribute__((aligned(16))) M s_m[PM][BM][LROW];
+    __shared__ __attribute__((aligned(16))) M s_n[PN][BN][LROW];
+    __shared__ float s_sum[OP == LOGITS ? BN : (OP == GRAD_CODE ? 4 * BM : 1)];
+    // Workgroups b and b + 8 run on one XCD: the tiles that share rows (GRAD_CODE: a split) go to the same one, whose L2
+    // then serves the shared operand once.
+    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    int tm, tn, split;
+    if constexpr (OP == GRAD_CODE) {
+        const int per = a.tiles_m * a.tiles_n;
+        split = slot / per * 8 + xcd;
+        tm = slot % per % a.tiles_m;
+        tn = slot % per / a.tiles_m;
+        if (split >= a.splits) return;
+    } else {
+        split = 0;
+        tm = slot / a.tiles_n * 8 + xcd;
+        tn = slot % a.tiles_n;
+        if (tm >= a.tiles_m) return;
+    }
+    const long m0 = (long)tm * BM, n0 = (long)tn * BN;
+    const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = (wave & 1) * (BM / 2), wn = (wave >> 1) * (BN / 2);
+    const int fr = lane & 15, fk = (lane >> 4) * 8;  // this lane's row and first K element of a fragment
+
+    using OpM = Operand<EM, ROW_M, BM, PM, M>;
+    using OpN = Operand<EN, ROW_N, BN, PN, M>;
+    OpM om;
+    OpN on;
+    float sums[OP == LOGITS ? OpN::NU : OpM::NU][OP == LOGITS ? OpN::CW : OpM::CW] = {};
+    f32x4 acc[MT][NT] = {};
+    om.load((const EM *)a.m, a.ld_m, m0, a.rows, k0, kend);
+    on.load((const EN *)a.n, a.ld_n, n0, a.cols, k0, kend);
+    for (long k = k0; k < kend; k += KT) {
+        if (k != k0) __syncthreads();  // the fragments of the stage before have been read
+        om.store(&s_m[0][0][0]);
+        on.store(&s_n[0][0][0]);
+        if constexpr (OP == LOGITS) on.template add_up<true>(sums);
+        if constexpr (OP == GRAD_CODE) om.template add_up<false>(sums);
         __syncthreads();
-        for (int j = 0; j < T; ++j) {
-            acc = fmaf(s_x[ty][j], s_c[tx][j], acc);
-            sq = fmaf(s_c[tx][j], s_c[tx][j], sq);
+        if (k + KT < kend) {
+            om.load((const EM *)a.m, a.ld_m, m0, a.rows, k + KT, kend);
+            on.load((const EN *)a.n, a.ld_n, n0, a.cols, k + KT, kend);
+        }
+        V fm[PM][MT], fn[PN][NT];
+#pragma unroll
+        for (int p = 0; p < PM; ++p)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fm[p][i] = *(const V *)&s_m[p][wm + i * 16 + fr][fk];
+#pragma unroll
+        for (int p = 0; p < PN; ++p)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fn[p][j] = *(const V *)&s_n[p][wn + j * 16 + fr][fk];
+        // the small products first
+#pragma unroll
+        for (int order = 2; order >= 0; --order)
+#pragma unroll
+            for (int p = 0; p < PM; ++p) {
+                const int q = order - p;
+                if (q < 0 || q >= PN) continue;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma(fn[q][j], fm[p][i], acc[i][j]);
+            }
+    }
+
+    if constexpr (OP == LOGITS) {  // |code|^2: four neighbouring threads hold a row's chunks
+#pragma unroll
+        for (int i = 0; i < OpN::NU; ++i) {
+            int r, kc;
+            if (!OpN::unit(i, r, kc)) continue;
+            float s = sums[i][0];
+            s += __shfl_xor(s, 1, 64);
+            s += __shfl_xor(s, 2, 64);
+            if (kc == 0) s_sum[r] = s;
         }
         __syncthreads();
     }
-    if (i0 + ty < n && c0 + tx < k) out[(i0 + ty) * k + c0 + tx] = fmaf(2.f, acc, -sq) * inv_t;
-}
-
-template <typename E>
-__global__ __launch_bounds__(T *T) void code_dx_kernel(int n, int d, int k, const float *__restrict__ g, const E *__restrict__ cb, float scale,
-                                                       E *__restrict__ dx) {
-    __shared__ float s_g[T][T + 1], s_c[T][T + 1];
-    const int tx = threadIdx.x % T, ty = threadIdx.x / T;
-    const long i0 = (long)blockIdx.x * T;
-    const int j0 = blockIdx.y * T;
-    float acc = 0.f;
-    for (int c0 = 0; c0 < k; c0 += T) {
-        s_g[ty][tx] = i0 + ty < n && c0 + tx < k ? g[(i0 + ty) * k + c0 + tx] : 0.f;
-        s_c[ty][tx] = c0 + ty < k && j0 + tx < d ? (float)cb[(size_t)(c0 + ty) * d + j0 + tx] : 0.f;
-        __syncthreads();
-        for (int c = 0; c < T; ++c) acc = fmaf(s_g[ty][c], s_c[c][tx], acc);
-        __syncthreads();
-    }
-    if (i0 + ty < n && j0 + tx < d) dx[(i0 + ty) * d + j0 + tx] = (E)(scale * acc);
-}
-
-// part[split][c][j] = sum of g[i,c] x[i,j] over the split's rows, part[split][k * d + c] = sum of g[i,c]
-template <typename E>
-__global__ __launch_bounds__(T *T) void code_dcode_kernel(int n, int d, int k, const float *__restrict__ g, const E *__restrict__ x, int rows_per_split,
-                                                          float *__restrict__ part) {
-    __shared__ float s_g[T][T + 1], s_x[T][T + 1];
-    const int tx = threadIdx.x % T, ty = threadIdx.x / T;
-    const int c0 = blockIdx.x * T, j0 = blockIdx.y * T;
-    const long lo = (long)blockIdx.z * rows_per_split, hi = lo + rows_per_split < n ? lo + rows_per_split : n;
-    float acc = 0.f, sum = 0.f;
-    for (long i0 = lo; i0 < hi; i0 += T) {
-        s_g[ty][tx] = i0 + ty < hi && c0 + tx < k ? g[(i0 + ty) * k + c0 + tx] : 0.f;
-        s_x[ty][tx] = i0 + ty < hi && j0 + tx < d ? (float)x[(i0 + ty) * d + j0 + tx] : 0.f;
-        __syncthreads();
-        for (int i = 0; i < T; ++i) {
-            acc = fmaf(s_g[i][ty], s_x[i][tx], acc);
-            sum += s_g[i][ty];
+    if constexpr (OP == GRAD_CODE) {
+        if (tn == 0) {
+#pragma unroll
+            for (int i = 0; i < OpM::NU; ++i) {
+                int r, kc;
+                if (!OpM::unit(i, r, kc)) continue;
+#pragma unroll
+                for (int c = 0; c < OpM::CW; ++c) s_sum[kc * BM + r + c] = sums[i][c];
+            }
+            __syncthreads();
+            float *p = (float *)a.out + split * (a.rows * a.cols + a.rows) + a.rows * a.cols;
+            for (int r = threadIdx.x; r < BM; r += CL_THREADS)
+                if (m0 + r < a.rows) p[m0 + r] = (s_sum[r] + s_sum[BM + r]) + (s_sum[2 * BM + r] + s_sum[3 * BM + r]);
         }
-        __syncthreads();
     }
-    float *p = part + (size_t)blockIdx.z * k * (d + 1);
-    if (c0 + ty < k && j0 + tx < d) p[(size_t)(c0 + ty) * d + j0 + tx] = acc;
-    if (c0 + ty < k && j0 + tx == 0) p[(size_t)k * d + c0 + ty] = sum;
+    // A lane holds four consecutive columns of one row of each 16 x 16 tile.
+    EO *out = (EO *)a.out + (OP == GRAD_CODE ? split * (a.rows * a.cols + a.rows) : 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const long m = m0 + wm + i * 16 + fr;
+        if (m >= a.rows) continue;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int nl = wn + j * 16 + (lane >> 4) * 4;
+            const long n = n0 + nl;
+            EO *dst = out + m * a.cols + n;
+            typename VecAt<EO, 4>::type r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = acc[i][j][e];
+                if constexpr (OP == LOGITS) x = fmaf(2.f, x, -s_sum[nl + e]) * a.scale;
+                if constexpr (OP == GRAD_X) x *= a.scale;
+                r[e] = (EO)x;
+            }
+            if (n + 4 <= a.cols) *(typename VecAt<EO, 4>::type *)dst = r;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.cols) dst[e] = r[e];
+        }
+    }
+}
+
+// Joins the splits' partial sums in a fixed order: 64 neighbouring elements a workgroup, the splits dealt to its waves.
+constexpr int JOIN_WAVES = 8;
+template <typename E>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void code_join_kernel(int d, int k, int splits, const float *__restrict__ part, const E *__restrict__ cb,
+                                                                    float scale, E *__restrict__ dcode) {
+    __shared__ float s_acc[JOIN_WAVES][64], s_sum[JOIN_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long size = (long)k * d, e = (long)blockIdx.x * 64 + lane;
+    float acc = 0.f, sum = 0.f;
+    if (e < size) {
+        const float *p = part + e, *ps = part + size + e / d;
+#pragma unroll 4
+        for (int s = wave; s < splits; s += JOIN_WAVES) {
+            acc += p[s * (size + k)];
+            sum += ps[s * (size + k)];
+        }
+    }
+    s_acc[wave][lane] = acc;
+    s_sum[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && e < size) {
+        for (int w = 1; w < JOIN_WAVES; ++w) {
+            acc += s_acc[w][lane];
+            sum += s_sum[w][lane];
+        }
+        dcode[e] = (E)(scale * fmaf(-sum, (float)cb[e], acc));
+    }
+}
+
+// Output tile: the largest that still gives every CU a workgroup; a side of at most 64 takes 64.
+constexpr int CL_WANT = 256;
+struct Tile {
+    int m, n;
+};
+inline Tile pick_tile(long rows, long cols, long splits) {
+    const Tile tiles[] = {{128, 128}, {128, 64}, {64, 64}};
+    for (const Tile &t : tiles) {
+        if (t.n == 128 && cols <= 64) continue;
+        if ((long)ceil_div(rows, t.m) * ceil_div(cols, t.n) * splits >= CL_WANT) return t;
+    }
+    return {32, 32};
+}
+
+// Splits of the summed rows of the codebook's gradient: about two workgroups of 128 x 128 or 128 x 64 per CU, at least
+// 128 rows a split (the partial sums a split writes and the join reads have to stay small beside its rows).
+inline int code_splits(int n, int d, int k) {
+    if (n <= 0) return 0;
+    const long tiles = (long)ceil_div(k, 128) * ceil_div(d, d <= 64 ? 64 : 128);
+    const long want = ceil_div(512, tiles), most = ceil_div(n, 128);
+    return (int)(want < most ? want : most);
+}
+
+template <Product OP, typename EM, typename EN, int PM, int PN, typename M, typename EO>
+int launch_product(hipStream_t stream, ProductArgs a) {
+    const Tile t = pick_tile(a.rows, a.cols, a.splits);
+    a.tiles_m = ceil_div(a.rows, t.m);
+    a.tiles_n = ceil_div(a.cols, t.n);
+    const long grid = OP == GRAD_CODE ? (long)ceil_div(a.splits, 8) * 8 * a.tiles_m * a.tiles_n : (long)ceil_div(a.tiles_m, 8) * 8 * a.tiles_n;
+    GDPSO_REQUIRE(grid < (1l << 31), "code_logits: too many rows for one call");
+#define CL_LAUNCH(TM, TN) hipLaunchKernelGGL((product_kernel<OP, EM, EN, PM, PN, M, TM, TN, EO>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a)
+    if (t.m == 128 && t.n == 128) CL_LAUNCH(128, 128);
+    else if (t.m == 128) CL_LAUNCH(128, 64);
+    else if (t.m == 64) CL_LAUNCH(64, 64);
+    else CL_LAUNCH(32, 32);
+#undef CL_LAUNCH
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
 }
 
 template <typename E>
-__global__ __launch_bounds__(256) void code_dcode_finish_kernel(int d, int k, int splits, const float *__restrict__ part, const E *__restrict__ cb,
-                                                                float scale, E *__restrict__ dcode) {
-    const long e = (long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= (long)k * d) return;
-    const int c = (int)(e / d);
-    float acc = 0.f, sum = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float *p = part + (size_t)s * k * (d + 1);
-        acc += p[e];
-        sum += p[(size_t)k * d + c];
-    }
-    dcode[e] = (E)(scale * fmaf(-sum, (float)cb[e], acc));
+constexpr int grad_parts() {
+    return is_f32<E>() ? 3 : (__is_same(E, f16_t) ? 2 : 1);
 }
 
-constexpr int CL_SPLIT_ROWS = 1024;
-inline int code_splits(int n) { return n > 0 ? ceil_div(n, CL_SPLIT_ROWS) : 0; }
+template <typename E>
+int logits_product(hipStream_t stream, const ProductArgs &a) {
+    if constexpr (is_f32<E>()) return launch_product<LOGITS, float, float, 3, 3, bf16_t, float>(stream, a);
+    else return launch_product<LOGITS, E, E, 1, 1, E, float>(stream, a);
+}
 
 int code_check(const char *what, int n, int d, int k, int dtype, float temperature) {
     const std::string w(what);
@@ -118,15 +395,14 @@ extern "C" int gdpso_code_logits(void *stream_, int n, int d, int k, const void 
     if (rc) return rc;
     GDPSO_REQUIRE(n == 0 || (inputs && codebook && logits), "code_logits: null argument");
     if (n == 0) return GDPSO_OK;
-    GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_logits_kernel<E>), dim3(ceil_div(n, T), ceil_div(k, T)), dim3(T * T), 0, (hipStream_t)stream_, n, d, k,
-                                               (const E *)inputs, (const E *)codebook, 1.f / temperature, logits));
-    GDPSO_HIP(hipGetLastError());
-    return GDPSO_OK;
+    ProductArgs a = {inputs, codebook, logits, n, k, d, d, d, 0, 0, 1, ceil_div(d, KT) * (long)KT, 1.f / temperature};
+    GDPSO_WITH_DTYPE(dtype, rc = logits_product<E>((hipStream_t)stream_, a));
+    return rc;
 }
 
 extern "C" size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k) {
     if (n <= 0 || d <= 0 || k <= 0) return 0;
-    return (size_t)code_splits(n) * k * (d + 1) * sizeof(float);
+    return (size_t)code_splits(n, d, k) * k * (d + 1) * sizeof(float);
 }
 
 extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const float *grad_logits, const void *inputs, const void *codebook, int dtype,
@@ -140,17 +416,22 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
         return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     const float scale = 2.f / temperature;
-    if (grad_inputs && n > 0)
-        GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_dx_kernel<E>), dim3(ceil_div(n, T), ceil_div(d, T)), dim3(T * T), 0, stream, n, d, k, grad_logits,
-                                                   (const E *)codebook, scale, (E *)grad_inputs));
-    if (grad_codebook) {
-        const int splits = code_splits(n);
-        if (splits)
-            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_dcode_kernel<E>), dim3(ceil_div(k, T), ceil_div(d, T), splits), dim3(T * T), 0, stream, n, d, k,
-                                                       grad_logits, (const E *)inputs, CL_SPLIT_ROWS, (float *)workspace));
-        GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_dcode_finish_kernel<E>), dim3(ceil_div((long)k * d, 256)), dim3(256), 0, stream, d, k, splits,
-                                                   (const float *)workspace, (const E *)codebook, scale, (E *)grad_codebook));
+    if (grad_inputs && n > 0) {
+        const ProductArgs a = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale};
+        GDPSO_WITH_DTYPE(dtype, rc = (launch_product<GRAD_X, float, E, 3, grad_parts<E>(), bf16_t, E>(stream, a)));
+        if (rc) return rc;
     }
-    GDPSO_HIP(hipGetLastError());
+    if (grad_codebook) {
+        const int splits = code_splits(n, d, k);
+        if (splits) {
+            const long per = ceil_div(ceil_div(n, splits), KT) * (long)KT;
+            const ProductArgs a = {grad_logits, inputs, workspace, k, d, n, k, d, 0, 0, splits, per, 1.f};
+            GDPSO_WITH_DTYPE(dtype, rc = (launch_product<GRAD_CODE, float, E, 3, grad_parts<E>(), bf16_t, float>(stream, a)));
+            if (rc) return rc;
+        }
+        GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E>), dim3(ceil_div((long)k * d, 64)), dim3(64 * JOIN_WAVES), 0, stream, d, k, splits,
+                                                   (const float *)workspace, (const E *)codebook, scale, (E *)grad_codebook));
+        GDPSO_HIP(hipGetLastError());
+    }
     return GDPSO_OK;
 }
