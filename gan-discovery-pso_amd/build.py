@@ -8,7 +8,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libgdpso.so")
-SOURCES = ["pack.cpp", "conv_gemm.hip", "nets.hip", "stage_resident.hip", "pso.hip", "vq.hip", "code_logits.hip", "losses.hip"]
+SOURCES = ["pack.cpp", "conv_gemm.hip", "nets.hip", "stage_resident.hip", "pso.hip", "vq.hip", "code_logits.hip", "balance.hip", "distill.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
          # no packed fp32 instructions (-O3 makes them of plain float code): some of their forms have given wrong results
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -32,7 +32,7 @@ def _flags_changed(stamp: str, key: str) -> bool:
 
 def build(force: bool = False, verbose: bool = True) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(HERE, "..", "include", "gdpso.h")]
+    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "loss_rows.h"), os.path.join(HERE, "..", "include", "gdpso.h")]
     objs = []
     procs = []
     os.makedirs(os.path.join(CSRC, "build"), exist_ok=True)

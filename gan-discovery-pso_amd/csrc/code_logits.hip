@@ -13,9 +13,7 @@
 // their parts.  Those of order 2^-24 and below are left out (two middle parts of order 2^-16 are kept): six matrix
 // instructions for fp32 x fp32, five for fp32 x fp16, three for fp32 x bf16.  Parts multiply exactly and add up in fp32.  The
 // forward product of two 16-bit operands needs no cutting.
-#include "common.h"
-
-#include <math.h>
+#include "loss_rows.h"
 
 namespace gdpso {
 namespace {
@@ -28,17 +26,6 @@ constexpr int LROW = KT + 8;
 
 using bf16x8 = __attribute__((ext_vector_type(8))) bf16_t;
 using f16x8 = __attribute__((ext_vector_type(8))) f16_t;
-using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
-
-// Vectors at element alignment: rows of any length and offset (global memory takes unaligned vector accesses).
-template <typename E, int N>
-struct VecAt {
-    typedef E type __attribute__((ext_vector_type(N), aligned(sizeof(E))));
-};
-template <typename E>
-struct VecAt<E, 1> {
-    typedef E type;
-};
 
 enum Product { LOGITS, GRAD_X, GRAD_CODE };
 
@@ -91,10 +78,8 @@ struct Operand {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const auto x = *(const typename VecAt<E, CW>::type *)(q + e * ld);
-                        if constexpr (CW == 1) v[i][0][e] = x;
-                        else
 #pragma unroll
-                            for (int c = 0; c < CW; ++c) v[i][c][e] = x[c];
+                        for (int c = 0; c < CW; ++c) v[i][c][e] = x[c];
                     }
                 } else {
 #pragma unroll

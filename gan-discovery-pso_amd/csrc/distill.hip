@@ -1,0 +1,636 @@
+// Distillation from a teacher's k highest logits (t the temperature, idx their columns):
+//
+//   q_i = softmax(teacher's logits / t), p_i = softmax(row i / t), loss = t^2 mean_i sum_j q_ij (log q_ij - log p_i[idx_ij])
+//   d loss / d s[i,c] = (t / rows) (p[i,c] - sum of q_ij with idx_ij = c)
+//
+// The work is one softmax over a long row and k corrections, bound by reading the logits and writing the gradient once
+// each.  Rows are therefore held in registers between the two: by 1 ... 64 lanes up to 2048 columns (dist_team_kernel), by a
+// workgroup of 256 or 1024 threads up to 131072 columns of 16-bit logits or 65536 of fp32 (dist_row_kernel).  Longer rows,
+// and few long rows (whose workgroups would leave most CUs idle), are cut into segments: one launch leaves every
+// segment's maximum and sum, a second joins them and writes (dist_part_kernel, dist_apply_kernel).
+//
+// The columns that a teacher names are stored a second time, behind the row's plain p; where a row names a column
+// twice (a bit per column in LDS finds out, columns folded to 65536 bits), the first of its entries adds the others' weight in
+// order and stores for all.  So nothing depends on the order of atomics, and the same call gives the same bits.
+//
+// Softmax statistics, terms and gradients are fp32, the mean over the rows fp64; the gradient is rounded once, to the logits'
+// type, when it is stored.
+#include "loss_rows.h"
+
+#include <algorithm>
+
+namespace gdpso {
+namespace {
+
+constexpr int DIST_MAX_K = GDPSO_DISTILL_MAX_K;
+constexpr int TEAM_THREADS = 256;
+constexpr int TEAM_MAX_V = 2048;
+constexpr int SEG_THREADS = 256, SEG_NCH = 8;  // a segment: at most 8192 fp32 or 16384 16-bit columns
+constexpr int BITS = 1 << 16;
+constexpr float LN2 = 0.69314718f;
+
+struct DistArgs {
+    int n, v, k;
+    const void *logits;
+    long long row_stride;
+    const void *t_logits;
+    int t_dtype;
+    const void *t_idx;
+    int index_bytes;
+    const unsigned char *mask;
+    float temperature, c;  // c = log2(e) / temperature
+    float grad_scale;
+    const float *upstream;
+    float *stats;            // maximum and sum of every row, written with VALUE, read without
+    const float *inv_rows;   // 1 / rows kept, or null: inv_all
+    float inv_all;
+    float *row_loss;
+    void *grad;
+    double *loss_part;       // sums of row losses, one a workgroup (segments: one a row)
+    int seg, segs;           // columns a segment, segments a row
+    float2 *parts;           // [n][segs] maximum and sum of a segment; null: stats are read
+};
+
+__device__ __forceinline__ float grad_factor(const DistArgs &a) {
+    return (a.upstream ? *a.upstream : a.grad_scale) * a.temperature * (a.inv_rows ? *a.inv_rows : a.inv_all);
+}
+// Entry j of row i: its column (-1: absent) and logit (-inf where absent).
+__device__ __forceinline__ void entry(const DistArgs &a, long long i, int j, int &c, float &t) {
+    const long long col = load_index(a.t_idx, a.index_bytes, i * a.k + j);
+    const bool in = col >= 0 && col < a.v;
+    c = in ? (int)col : -1;
+    t = in ? load_typed(a.t_logits, a.t_dtype, i * a.k + j) : -INFINITY;
+}
+// q (log2 q - log2 p) short of the two sums' logarithms
+__device__ __forceinline__ float entry_term(float q, float t_arg, float s_arg) { return q == 0.f ? 0.f : q * (t_arg - s_arg); }
+__device__ __forceinline__ float row_loss_of(const DistArgs &a, float terms, float l, float tl) {
+    return l == 0.f || tl == 0.f ? 0.f : a.temperature * a.temperature * LN2 * (terms + (log2f(l) - log2f(tl)));
+}
+
+// 1 / rows that the mask keeps
+__global__ __launch_bounds__(1024) void dist_kept_kernel(int n, const unsigned char *__restrict__ mask, float *__restrict__ inv_rows) {
+    const long long kept = count_kept<1024>(mask, n);
+    if (threadIdx.x == 0) *inv_rows = kept > 0 ? (float)(1. / (double)kept) : 0.f;
+}
+
+// ------------------------------------------------------------------------------------- rows of up to 2048 columns
+template <typename E, int TEAM, int NCH, bool VALUE, bool GRAD>
+__global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
+    constexpr int VEC = vec_of<E>(), TEAMS = TEAM_THREADS / TEAM, WORDS = (TEAM * NCH * VEC + 31) / 32;
+    __shared__ unsigned s_bits[GRAD ? TEAMS : 1][GRAD ? WORDS : 1];
+    __shared__ double s_loss[VALUE ? TEAMS : 1];
+    const int lane = threadIdx.x & 63, pos = threadIdx.x & (TEAM - 1), team = threadIdx.x / TEAM;
+    float factor = 0.f;
+    if constexpr (GRAD) {
+        factor = grad_factor(a);
+        for (int w = pos; w < WORDS; w += TEAM) s_bits[team][w] = 0;
+    }
+    double sum = 0.;
+    for (long long i = (long long)blockIdx.x * TEAMS + team; i < a.n; i += (long long)gridDim.x * TEAMS) {
+        const E *row = (const E *)a.logits + i * a.row_stride;
+        E *grow = (E *)a.grad + i * a.v;
+        if (a.mask && !a.mask[i]) {
+            if (VALUE && pos == 0) {
+                a.row_loss[i] = 0.f;
+                a.stats[2 * i] = 0.f;
+                a.stats[2 * i + 1] = 0.f;
+            }
+            if constexpr (GRAD) RowRegs<E, TEAM, NCH>::store(grow, a.v, pos, [](int, int) { return 0.f; });
+            continue;
+        }
+        RowRegs<E, TEAM, NCH> r;
+        r.load(row, a.v, pos);
+        // the lane's first entry stays in registers; rows with more entries than lanes read theirs again where needed
+        int c0 = -1;
+        float t0 = -INFINITY, s0 = 0.f;
+        if (pos < a.k) entry(a, i, pos, c0, t0);
+        if (c0 >= 0) s0 = (float)row[c0];
+        const auto each = [&](auto f) {  // f(j, column, teacher's logit, student's logit) for this lane's entries
+            if (pos < a.k) f(pos, c0, t0, s0);
+            for (int j = pos + TEAM; j < a.k; j += TEAM) {
+                int c;
+                float t;
+                entry(a, i, j, c, t);
+                f(j, c, t, c >= 0 ? (float)row[c] : 0.f);
+            }
+        };
+        float m, l;
+        if constexpr (VALUE) m = team_max<TEAM>(r.max());
+        else {
+            m = a.stats[2 * i];
+            l = a.stats[2 * i + 1];
+        }
+        const Shift s(a.c, m);
+        float ex[NCH][VEC];
+        float mine = 0.f;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                ex[j][v] = s.exp(r.at(j, v));
+                mine += ex[j][v];
+            }
+        if constexpr (VALUE) l = team_sum<TEAM>(mine);
+        float tm = -INFINITY;
+        each([&](int, int, float t, float) { tm = fmaxf(tm, t); });
+        const Shift ts(a.c, team_max<TEAM>(tm));
+        float tl = 0.f;
+        each([&](int, int, float t, float) { tl += ts.exp(t); });
+        tl = team_sum<TEAM>(tl);
+        const bool empty = l == 0.f || tl == 0.f;
+        const float inv_l = empty ? 0.f : 1.f / l, inv_tl = empty ? 0.f : 1.f / tl;
+        if constexpr (VALUE) {
+            float terms = 0.f;
+            each([&](int, int, float t, float x) {
+                const float arg = ts.arg(t);
+                terms += entry_term(__builtin_amdgcn_exp2f(arg) * inv_tl, arg, s.arg(x));
+            });
+            terms = team_sum<TEAM>(terms);
+            if (pos == 0) {
+                const float loss = row_loss_of(a, terms, l, tl);
+                a.row_loss[i] = loss;
+                a.stats[2 * i] = m;
+                a.stats[2 * i + 1] = l;
+                sum += loss;
+            }
+        }
+        if constexpr (GRAD) {
+            RowRegs<E, TEAM, NCH>::store(grow, a.v, pos, [&](int j, int v) { return empty ? 0.f : factor * (ex[j][v] * inv_l); });
+            if (empty) continue;
+            bool twice = false;
+            each([&](int, int c, float, float) {
+                if (c >= 0) twice |= (atomicOr(&s_bits[team][c >> 5], 1u << (c & 31)) >> (c & 31)) & 1;
+            });
+            __builtin_amdgcn_wave_barrier();
+            each([&](int, int c, float, float) {
+                if (c >= 0) s_bits[team][c >> 5] = 0;
+            });
+            __builtin_amdgcn_wave_barrier();
+            const unsigned long long team_lanes = (TEAM == 64 ? ~0ull : (1ull << (TEAM & 63)) - 1) << (lane & ~(TEAM - 1));
+            const bool repeats = (__ballot(twice) & team_lanes) != 0;
+            each([&](int j, int c, float t, float x) {
+                if (c < 0) return;
+                float q = ts.exp(t) * inv_tl;
+                if (repeats) {
+                    for (int h = 0; h < a.k; ++h) {
+                        if (h == j) continue;
+                        int ch;
+                        float th;
+                        entry(a, i, h, ch, th);
+                        if (ch != c) continue;
+                        if (h < j) return;  // an entry before this one stores for both
+                        q += ts.exp(th) * inv_tl;
+                    }
+                }
+                grow[c] = (E)(factor * (s.exp(x) * inv_l - q));
+            });
+        }
+    }
+    if constexpr (VALUE) {
+        if (pos == 0) s_loss[team] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < TEAMS; ++w) sum += s_loss[w];
+            a.loss_part[blockIdx.x] = sum;
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------- a workgroup a row or segment
+// Two values reduced over the workgroup with one barrier; `slot` has to be free (two barriers ago or never used).
+template <int THREADS>
+struct PairRed {
+    float a[THREADS / 64], b[THREADS / 64];
+};
+template <int THREADS>
+__device__ __forceinline__ void wide_max2(PairRed<THREADS> &slot, float &x, float &y) {
+    x = team_max<64>(x);
+    y = team_max<64>(y);
+    if ((threadIdx.x & 63) == 0) {
+        slot.a[threadIdx.x >> 6] = x;
+        slot.b[threadIdx.x >> 6] = y;
+    }
+    __syncthreads();
+    x = slot.a[0];
+    y = slot.b[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) {
+        x = fmaxf(x, slot.a[w]);
+        y = fmaxf(y, slot.b[w]);
+    }
+}
+template <int THREADS>
+__device__ __forceinline__ void wide_sum2(PairRed<THREADS> &slot, float &x, float &y) {
+    x = team_sum<64>(x);
+    y = team_sum<64>(y);
+    if ((threadIdx.x & 63) == 0) {
+        slot.a[threadIdx.x >> 6] = x;
+        slot.b[threadIdx.x >> 6] = y;
+    }
+    __syncthreads();
+    x = slot.a[0];
+    y = slot.b[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) {
+        x += slot.a[w];
+        y += slot.b[w];
+    }
+}
+
+// The teacher's entries of one row in LDS, and the columns they name.
+struct Entries {
+    int c[DIST_MAX_K];
+    float t[DIST_MAX_K];
+};
+
+template <typename E, int THREADS, int NCH, bool GRAD>
+__global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
+    __shared__ PairRed<THREADS> s_max, s_sum;
+    __shared__ Entries s_e[2];  // by turns: a wave may still read the last row's while the next row's are stored
+    __shared__ float s_terms[THREADS / 64];
+    __shared__ unsigned s_bits[GRAD ? BITS / 32 : 1];
+    __shared__ int s_repeats;
+    const int tid = threadIdx.x;
+    float factor = 0.f;
+    if constexpr (GRAD) {
+        factor = grad_factor(a);
+        for (int w = tid; w < BITS / 32; w += THREADS) s_bits[w] = 0;
+    }
+    double sum = 0.;
+    int turn = 0;
+    for (long long i = blockIdx.x; i < a.n; i += gridDim.x) {
+        const E *row = (const E *)a.logits + i * a.row_stride;
+        E *grow = (E *)a.grad + i * a.v;
+        if (a.mask && !a.mask[i]) {
+            if (tid == 0) {
+                a.row_loss[i] = 0.f;
+                a.stats[2 * i] = 0.f;
+                a.stats[2 * i + 1] = 0.f;
+            }
+            if constexpr (GRAD) RowRegs<E, THREADS, NCH>::store(grow, a.v, tid, [](int, int) { return 0.f; });
+            continue;
+        }
+        RowRegs<E, THREADS, NCH> r;
+        r.load(row, a.v, tid);
+        Entries &ent = s_e[turn];
+        turn ^= 1;  // only rows that pass the barriers below take turns
+        float tm = -INFINITY;
+        for (int j = tid; j < a.k; j += THREADS) {
+            int c;
+            float t;
+            entry(a, i, j, c, t);
+            ent.c[j] = c;
+            ent.t[j] = t;
+            tm = fmaxf(tm, t);
+        }
+        float m = r.max();
+        wide_max2<THREADS>(s_max, m, tm);
+        if (tid == 0) s_repeats = 0;  // read by all before that barrier, set by any behind the next
+        const Shift s(a.c, m), ts(a.c, tm);
+        float l = r.sum_exp(s), tl = 0.f;
+        for (int j = tid; j < a.k; j += THREADS) tl += ts.exp(ent.t[j]);
+        wide_sum2<THREADS>(s_sum, l, tl);
+        const bool empty = l == 0.f || tl == 0.f;
+        const float inv_l = empty ? 0.f : 1.f / l, inv_tl = empty ? 0.f : 1.f / tl;
+        float terms = 0.f;
+        for (int j = tid; j < a.k; j += THREADS) {
+            const int c = ent.c[j];
+            const float arg = ts.arg(ent.t[j]);
+            if (c >= 0) terms += entry_term(__builtin_amdgcn_exp2f(arg) * inv_tl, arg, s.arg((float)row[c]));
+            if (GRAD && c >= 0) {
+                const unsigned bit = 1u << (c & 31);
+                if (atomicOr(&s_bits[(c & (BITS - 1)) >> 5], bit) & bit) s_repeats = 1;
+            }
+        }
+        if constexpr (GRAD) RowRegs<E, THREADS, NCH>::store(grow, a.v, tid, [&](int j, int v) { return empty ? 0.f : factor * (s.exp(r.at(j, v)) * inv_l); });
+        if (tid < (a.k + 63) / 64 * 64 || tid < 64) {
+            terms = team_sum<64>(terms);
+            if ((tid & 63) == 0) s_terms[tid >> 6] = terms;
+        }
+        __syncthreads();  // the row's plain gradient, the bits and the terms are there
+        if (tid == 0) {
+            const int waves = std::min(THREADS / 64, (a.k + 63) / 64);
+            for (int w = 1; w < waves; ++w) terms += s_terms[w];
+            const float loss = row_loss_of(a, terms, l, tl);
+            a.row_loss[i] = loss;
+            a.stats[2 * i] = m;
+            a.stats[2 * i + 1] = l;
+            sum += loss;
+        }
+        if constexpr (GRAD) {
+            const bool repeats = s_repeats != 0;
+            for (int j = tid; j < a.k; j += THREADS) {
+                const int c = ent.c[j];
+                if (c < 0) continue;
+                s_bits[(c & (BITS - 1)) >> 5] = 0;
+                if (empty) continue;
+                float q = ts.exp(ent.t[j]) * inv_tl;
+                bool first = true;
+                if (repeats)
+                    for (int h = 0; h < a.k; ++h) {
+                        if (ent.c[h] != c || h == j) continue;
+                        if (h < j) {
+                            first = false;  // an entry before this one stores for both
+                            break;
+                        }
+                        q += ts.exp(ent.t[h]) * inv_tl;
+                    }
+                if (first) grow[c] = (E)(factor * (s.exp((float)row[c]) * inv_l - q));
+            }
+        }
+    }
+    if (tid == 0) a.loss_part[blockIdx.x] = sum;
+}
+
+// Maximum and sum of a segment.
+template <typename E>
+__global__ __launch_bounds__(SEG_THREADS) void dist_part_kernel(DistArgs a) {
+    __shared__ PairRed<SEG_THREADS> s_max, s_sum;
+    const long long i = blockIdx.x / a.segs;
+    const int seg = (int)(blockIdx.x - i * a.segs), lo = seg * a.seg, len = std::min(a.seg, a.v - lo);
+    if (a.mask && !a.mask[i]) return;
+    RowRegs<E, SEG_THREADS, SEG_NCH> r;
+    r.load((const E *)a.logits + i * a.row_stride + lo, len, threadIdx.x);
+    float m = r.max(), none = 0.f;
+    wide_max2<SEG_THREADS>(s_max, m, none);
+    float l = r.sum_exp(Shift(a.c, m));
+    wide_sum2<SEG_THREADS>(s_sum, l, none);
+    if (threadIdx.x == 0) a.parts[blockIdx.x] = make_float2(m, l);
+}
+
+// Joins a row's segments (or reads its stats), and writes its loss (the first segment's workgroup) and one segment of its gradient.
+template <typename E, bool VALUE, bool GRAD>
+__global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
+    __shared__ PairRed<SEG_THREADS> s_max, s_sum;
+    __shared__ Entries ent;
+    __shared__ float s_terms[SEG_THREADS / 64];
+    __shared__ unsigned s_bits[GRAD ? BITS / 32 : 1];
+    __shared__ int s_repeats;
+    const int tid = threadIdx.x;
+    const long long i = GRAD ? blockIdx.x / a.segs : blockIdx.x;
+    const int seg = GRAD ? (int)(blockIdx.x - i * a.segs) : 0, lo = seg * a.seg, len = std::min(a.seg, a.v - lo);
+    const E *row = (const E *)a.logits + i * a.row_stride;
+    E *grow = (E *)a.grad + i * a.v;
+    if (a.mask && !a.mask[i]) {
+        if (VALUE && seg == 0 && tid == 0) {
+            a.row_loss[i] = 0.f;
+            a.stats[2 * i] = 0.f;
+            a.stats[2 * i + 1] = 0.f;
+            a.loss_part[i] = 0.;
+        }
+        if constexpr (GRAD) RowRegs<E, SEG_THREADS, SEG_NCH>::store(grow + lo, len, tid, [](int, int) { return 0.f; });
+        return;
+    }
+    RowRegs<E, SEG_THREADS, SEG_NCH> r;
+    if constexpr (GRAD) r.load(row + lo, len, tid);
+    float tm = -INFINITY, m = -INFINITY;
+    for (int j = tid; j < a.k; j += SEG_THREADS) {
+        int c;
+        float t;
+        entry(a, i, j, c, t);
+        ent.c[j] = c;
+        ent.t[j] = t;
+        tm = fmaxf(tm, t);
+    }
+    if constexpr (VALUE)
+        for (int p = tid; p < a.segs; p += SEG_THREADS) m = fmaxf(m, a.parts[i * a.segs + p].x);
+    else m = a.stats[2 * i];
+    if constexpr (GRAD) {
+        for (int w = tid; w < BITS / 32; w += SEG_THREADS) s_bits[w] = 0;
+        if (tid == 0) s_repeats = 0;
+    }
+    wide_max2<SEG_THREADS>(s_max, m, tm);
+    const Shift s(a.c, m), ts(a.c, tm);
+    float tl = 0.f, l = 0.f;
+    if constexpr (VALUE)
+        for (int p = tid; p < a.segs; p += SEG_THREADS) {
+            const float2 part = a.parts[i * a.segs + p];
+            // a segment's sum is relative to its own shift: to the row's by the quotient of the two
+            const Shift own(a.c, part.x);
+            l += part.y == 0.f ? 0.f : part.y * __builtin_amdgcn_exp2f(s.arg(part.x) - own.arg(part.x));
+        }
+    for (int j = tid; j < a.k; j += SEG_THREADS) tl += ts.exp(ent.t[j]);
+    wide_sum2<SEG_THREADS>(s_sum, l, tl);
+    if constexpr (!VALUE) l = a.stats[2 * i + 1];
+    const bool empty = l == 0.f || tl == 0.f;
+    const float inv_l = empty ? 0.f : 1.f / l, inv_tl = empty ? 0.f : 1.f / tl;
+    float terms = 0.f;
+    for (int j = tid; j < a.k; j += SEG_THREADS) {
+        const int c = ent.c[j];
+        if (c < 0) continue;
+        if (VALUE && seg == 0) {
+            const float arg = ts.arg(ent.t[j]);
+            terms += entry_term(__builtin_amdgcn_exp2f(arg) * inv_tl, arg, s.arg((float)row[c]));
+        }
+        if (GRAD && c >= lo && c < lo + len) {
+            const unsigned bit = 1u << (c & 31);
+            if (atomicOr(&s_bits[(c & (BITS - 1)) >> 5], bit) & bit) s_repeats = 1;
+        }
+    }
+    if constexpr (GRAD) {
+        const float factor = grad_factor(a);
+        RowRegs<E, SEG_THREADS, SEG_NCH>::store(grow + lo, len, tid, [&](int j, int v) { return empty ? 0.f : factor * (s.exp(r.at(j, v)) * inv_l); });
+    }
+    if (VALUE && seg == 0) {
+        terms = team_sum<64>(terms);
+        if ((tid & 63) == 0) s_terms[tid >> 6] = terms;
+    }
+    __syncthreads();  // the segment's plain gradient, the bits and the terms are there
+    if (VALUE && seg == 0 && tid == 0) {
+        for (int w = 1; w < SEG_THREADS / 64; ++w) terms += s_terms[w];
+        const float loss = row_loss_of(a, terms, l, tl);
+        a.row_loss[i] = loss;
+        a.stats[2 * i] = m;
+        a.stats[2 * i + 1] = l;
+        a.loss_part[i] = loss;
+    }
+    if constexpr (GRAD) {
+        if (empty) return;
+        const float factor = grad_factor(a);
+        for (int j = tid; j < a.k; j += SEG_THREADS) {
+            const int c = ent.c[j];
+            if (c < lo || c >= lo + len) continue;
+            float q = ts.exp(ent.t[j]) * inv_tl;
+            bool first = true;
+            if (s_repeats)
+                for (int h = 0; h < a.k; ++h) {
+                    if (ent.c[h] != c || h == j) continue;
+                    if (h < j) {
+                        first = false;
+                        break;
+                    }
+                    q += ts.exp(ent.t[h]) * inv_tl;
+                }
+            if (first) grow[c] = (E)(factor * (s.exp((float)row[c]) * inv_l - q));
+        }
+    }
+}
+
+// loss = sum of the parts / rows kept, and 1 / rows kept for a later gradient.  kept: already there (a mask and a gradient).
+__global__ __launch_bounds__(1024) void dist_finish_kernel(int n, const unsigned char *__restrict__ mask, bool kept, int parts, const double *__restrict__ part,
+                                                           float *inv_rows, float *__restrict__ loss) {
+    __shared__ double s_sum[16];
+    double s = 0.;
+    for (int i = threadIdx.x; i < parts; i += 1024) s += part[i];
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = s;
+    long long rows = n;
+    if (mask && !kept) rows = count_kept<1024>(mask, n);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float inv = kept ? *inv_rows : (rows > 0 ? (float)(1. / (double)rows) : 0.f);
+        if (!kept) *inv_rows = inv;
+        for (int w = 1; w < 16; ++w) s += s_sum[w];
+        *loss = (float)(s * (double)inv);
+    }
+}
+
+int distill_check(const char *what, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits, int t_dtype,
+                  const void *t_idx, int index_bytes, float temperature) {
+    const std::string w(what);
+    GDPSO_REQUIRE(n >= 0 && v > 0 && k > 0, w + ": n >= 0, v > 0 and k > 0 are required");
+    GDPSO_REQUIRE(k <= DIST_MAX_K, w + ": more than 1024 teacher logits a row");
+    GDPSO_REQUIRE(dtype_ok(dtype) && dtype_ok(t_dtype), w + ": unknown element type");
+    GDPSO_REQUIRE(index_bytes == 4 || index_bytes == 8, w + ": indices are 4 or 8 bytes");
+    GDPSO_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, w + ": temperature must lie in [1e-6, 1e6]");
+    GDPSO_REQUIRE(n == 0 || (logits && t_logits && t_idx), w + ": null argument");
+    GDPSO_REQUIRE(row_stride >= 0, w + ": negative row stride");
+    return GDPSO_OK;
+}
+
+// How rows of v columns are held.
+enum Way { BY_TEAM, BY_ROW, BY_SEGMENT };
+struct Plan {
+    Way way;
+    int team, chunks;  // BY_TEAM: lanes a row, chunks a lane
+    int threads;       // BY_ROW: threads a row (chunks a thread in `chunks`)
+    int seg, segs;
+};
+inline Plan plan_rows(int n, int v, int vec) {
+    Plan p = {BY_TEAM, 0, 0, 0, 0, 0};
+    const int chunks = ceil_div(v, vec);
+    if (v <= TEAM_MAX_V) {
+        p.team = 1;
+        while (p.team < chunks && p.team < 64) p.team <<= 1;
+        p.chunks = 1;
+        while (p.team * p.chunks < chunks) p.chunks <<= 1;
+        return p;
+    }
+    p.way = BY_ROW;
+    if (chunks <= 256 * 8) p.threads = 256, p.chunks = 8;
+    else if (chunks <= 1024 * 8) p.threads = 1024, p.chunks = 8;
+    else if (chunks <= 1024 * 16) p.threads = 1024, p.chunks = 16;
+    else p.way = BY_SEGMENT;
+    // few rows of many columns: as workgroups of a row they would occupy one CU each
+    if (n < 128 && v >= 16384) p.way = BY_SEGMENT;
+    const int most = SEG_THREADS * SEG_NCH * vec, least = SEG_THREADS * vec;
+    // about two workgroups a CU, segments of whole rounds of the workgroup's loads
+    long seg = ceil_div((long)v * n, 512 * (long)least) * (long)least;
+    p.seg = (int)std::min<long>(std::max<long>(seg, least), most);
+    p.segs = ceil_div(v, p.seg);
+    return p;
+}
+
+constexpr int DIST_BLOCKS = 2048;
+inline int dist_blocks(const Plan &p, int n) {
+    const long rows = p.way == BY_TEAM ? TEAM_THREADS / p.team : 1;
+    const long want = ((long)n + rows - 1) / rows;
+    return (int)(want < 1 ? 1 : std::min<long>(want, DIST_BLOCKS));
+}
+inline size_t parts_bytes(const Plan &p, int n) { return p.way == BY_SEGMENT ? (size_t)n * p.segs * sizeof(float2) : 0; }
+inline size_t loss_bytes(const Plan &p, int n) { return (size_t)(p.way == BY_SEGMENT ? (n > 0 ? n : 1) : dist_blocks(p, n)) * sizeof(double); }
+
+template <typename E, bool VALUE, bool GRAD>
+int launch_team(hipStream_t stream, const DistArgs &a, const Plan &p) {
+    const dim3 grid(dist_blocks(p, a.n));
+#define DIST_TEAM(T, C) hipLaunchKernelGGL((dist_team_kernel<E, T, C, VALUE, GRAD>), grid, dim3(TEAM_THREADS), 0, stream, a)
+    switch (p.team * 16 + p.chunks) {
+        case 1 * 16 + 1: DIST_TEAM(1, 1); break;
+        case 2 * 16 + 1: DIST_TEAM(2, 1); break;
+        case 4 * 16 + 1: DIST_TEAM(4, 1); break;
+        case 8 * 16 + 1: DIST_TEAM(8, 1); break;
+        case 16 * 16 + 1: DIST_TEAM(16, 1); break;
+        case 32 * 16 + 1: DIST_TEAM(32, 1); break;
+        case 64 * 16 + 1: DIST_TEAM(64, 1); break;
+        case 64 * 16 + 2: DIST_TEAM(64, 2); break;
+        case 64 * 16 + 4: DIST_TEAM(64, 4); break;
+        default:
+            if constexpr (is_f32<E>()) DIST_TEAM(64, 8);
+            break;
+    }
+#undef DIST_TEAM
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
+}
+
+template <typename E, bool VALUE, bool GRAD>
+int launch_distill(hipStream_t stream, const DistArgs &a, const Plan &p) {
+    if (p.way == BY_TEAM) return launch_team<E, VALUE, GRAD>(stream, a, p);
+    if (VALUE && p.way == BY_ROW) {
+        const dim3 grid(dist_blocks(p, a.n));
+        if (p.threads == 256) hipLaunchKernelGGL((dist_row_kernel<E, 256, 8, GRAD>), grid, dim3(256), 0, stream, a);
+        else if (p.chunks == 8) hipLaunchKernelGGL((dist_row_kernel<E, 1024, 8, GRAD>), grid, dim3(1024), 0, stream, a);
+        else hipLaunchKernelGGL((dist_row_kernel<E, 1024, 16, GRAD>), grid, dim3(1024), 0, stream, a);
+    } else {
+        const long blocks = (long)a.n * a.segs;
+        GDPSO_REQUIRE(blocks < (1l << 31), "distill: too many rows for one call");
+        if (VALUE) hipLaunchKernelGGL((dist_part_kernel<E>), dim3((unsigned)blocks), dim3(SEG_THREADS), 0, stream, a);
+        hipLaunchKernelGGL((dist_apply_kernel<E, VALUE, GRAD>), dim3((unsigned)(GRAD ? blocks : a.n)), dim3(SEG_THREADS), 0, stream, a);
+    }
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
+}
+
+}  // namespace
+}  // namespace gdpso
+
+using namespace gdpso;
+
+extern "C" size_t gdpso_distill_workspace_bytes(int n, int v, int k) {
+    if (n < 0 || v <= 0 || k <= 0) return 0;
+    const Plan a = plan_rows(n, v, 4), b = plan_rows(n, v, 8);
+    return std::max(parts_bytes(a, n) + loss_bytes(a, n), parts_bytes(b, n) + loss_bytes(b, n));
+}
+
+extern "C" int gdpso_distill(void *stream_, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits, int t_dtype,
+                             const void *t_indices, int index_bytes, const unsigned char *mask, float temperature, float grad_scale, float *loss,
+                             float *row_loss, float *row_stats, void *grad, void *workspace, size_t workspace_bytes) {
+    int rc = distill_check("distill", n, v, k, logits, row_stride, dtype, t_logits, t_dtype, t_indices, index_bytes, temperature);
+    if (rc) return rc;
+    GDPSO_REQUIRE(loss && row_stats && workspace && (n == 0 || row_loss), "distill: null argument");
+    if (workspace_bytes < gdpso_distill_workspace_bytes(n, v, k)) return fail(GDPSO_ERR_WORKSPACE, "distill: workspace too small");
+    hipStream_t stream = (hipStream_t)stream_;
+    float *inv_rows = row_stats + 2 * (size_t)n;
+    const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype));
+    double *loss_part = (double *)workspace;
+    float2 *parts = (float2 *)((char *)workspace + loss_bytes(p, n));
+    const bool kept = mask && grad && n > 0;
+    DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), grad_scale, nullptr,
+                  row_stats, kept ? inv_rows : nullptr, n > 0 ? (float)(1. / n) : 0.f, row_loss, grad, loss_part, p.seg, p.segs, parts};
+    if (kept) hipLaunchKernelGGL(dist_kept_kernel, dim3(1), dim3(1024), 0, stream, n, mask, inv_rows);
+    if (n > 0) {
+        if (grad)
+            GDPSO_WITH_DTYPE(dtype, rc = (launch_distill<E, true, true>(stream, a, p)));
+        else
+            GDPSO_WITH_DTYPE(dtype, rc = (launch_distill<E, true, false>(stream, a, p)));
+        if (rc) return rc;
+    }
+    const int count = n == 0 ? 0 : (p.way == BY_SEGMENT ? n : dist_blocks(p, n));
+    hipLaunchKernelGGL(dist_finish_kernel, dim3(1), dim3(1024), 0, stream, n, mask, kept, count, loss_part, inv_rows, loss);
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
+}
+
+extern "C" int gdpso_distill_grad(void *stream_, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits,
+                                  int t_dtype, const void *t_indices, int index_bytes, const unsigned char *mask, float temperature,
+                                  const float *row_stats, const float *upstream, void *grad) {
+    int rc = distill_check("distill_grad", n, v, k, logits, row_stride, dtype, t_logits, t_dtype, t_indices, index_bytes, temperature);
+    if (rc) return rc;
+    GDPSO_REQUIRE(n == 0 || (row_stats && upstream && grad), "distill_grad: null argument");
+    if (n == 0) return GDPSO_OK;
+    const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype));
+    const DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), 0.f, upstream,
+                        (float *)row_stats, row_stats + 2 * (size_t)n, 0.f, nullptr, grad, nullptr, p.seg, p.segs, nullptr};
+    GDPSO_WITH_DTYPE(dtype, rc = (launch_distill<E, false, true>((hipStream_t)stream_, a, p)));
+    return rc;
+}
