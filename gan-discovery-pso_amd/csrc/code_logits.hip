@@ -19,48 +19,128 @@ namespace gdpso {
 namespace {
 
 constexpr int CL_MAX_D = 4096;
-constexpr int CL_THREADS = 256;  // four waves, two by two over the output tile
-constexpr int KT = 32;           // K elements a stage: one 16x16x32 matrix instruction deep
+constexpr int CL_THREADS = 256;  // four waves, one below the other over the output tile's rows
+constexpr int KT = 32;           // summed elements a stage: one 16x16x32 matrix instruction deep
 // LDS elements from one row of a stage to the next: 80 bytes put the sixteen rows of a fragment read on disjoint banks
 constexpr int LROW = KT + 8;
 
 using bf16x8 = __attribute__((ext_vector_type(8))) bf16_t;
 using f16x8 = __attribute__((ext_vector_type(8))) f16_t;
+template <typename M>
+using Frag = __attribute__((ext_vector_type(8))) M;
+
+// Cuts eight values into P parts of type M: parts[p] is the rounded rest of what the parts before it leave.
+template <int P, typename M, typename E>
+__device__ __forceinline__ void cut(const E (&v)[8], Frag<M> (&parts)[P]) {
+    if constexpr (__is_same(E, M) && P == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) parts[0][e] = v[e];
+    } else {
+        float rest[8], most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            rest[e] = (float)v[e];
+            most = fmaxf(most, fabsf(rest[e]));
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) parts[p][e] = (M)rest[e];
+            if (p + 1 < P)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rest[e] -= (float)parts[p][e];
+        }
+        if (P > 1 && most > 3.3895e38f) {  // an infinite first part (inf, or rounded up to it) has no rest: inf - inf made it NaN
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (__builtin_isinf((float)parts[0][e]))
+#pragma unroll
+                    for (int p = 1; p < P; ++p) parts[p][e] = (M)0.f;
+        }
+    }
+}
 
 enum Product { LOGITS, GRAD_X, GRAD_CODE };
 
-// One operand of the product: BR rows of the output's side by KT of the summed side per stage, carried from global
-// memory through registers (so that the loads of a stage are under way while the one before multiplies) into P planes of
-// 16-bit parts in LDS, [P][BR][LROW].  ROW: the summed side is the contiguous one; else the output's side is, and the
-// eight values of a fragment are gathered from eight rows of memory in the registers of one thread.
-template <typename E, bool ROW, int BR, int P, typename M>
-struct Operand {
-    static constexpr int CW = ROW ? 1 : (BR * 4 > CL_THREADS ? BR * 4 / CL_THREADS : 1);  // columns a unit
-    static constexpr int UNITS = BR * 4 / CW;
+// The operand on the output rows' side.  Every wave has rows of its own, so its fragments come straight from global
+// memory into registers, a stage ahead, and no value passes through LDS.  KC: the summed side is contiguous, a lane reads
+// its eight values of a row in one piece; else the rows' side is, and a lane reads MT neighbouring rows at eight summed
+// indices (tile t of the wave then holds rows t, MT + t, 2 MT + t ...).
+template <typename E, bool KC, int MT, int P, typename M>
+struct RowsOperand {
+    E v[MT][8];
+
+    __device__ __forceinline__ static long row(long wave_row0, int i, int fr) { return KC ? wave_row0 + i * 16 + fr : wave_row0 + fr * MT + i; }
+    // values [k, kend) of this lane's rows; indices beyond read as 0, rows beyond as the last one (KC) or 0: nothing uses them
+    __device__ __forceinline__ void load(const E *__restrict__ p, long ld, long wave_row0, long rows, int fr, long k, long kend) {
+        if constexpr (KC) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const E *q = p + min(row(wave_row0, i, fr), rows - 1) * ld + k;
+                if (k + 8 <= kend) {
+                    constexpr int W = 16 / sizeof(E);
+#pragma unroll
+                    for (int w = 0; w < 8 / W; ++w) {
+                        const auto x = *(const typename VecAt<E, W>::type *)(q + w * W);
+#pragma unroll
+                        for (int e = 0; e < W; ++e) v[i][w * W + e] = x[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] = k + e < kend ? q[e] : (E)0.f;
+                }
+            }
+        } else {
+            const long r = row(wave_row0, 0, fr);
+            const E *q = p + k * ld + r;
+            if (r + MT <= rows && k + 8 <= kend) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const auto x = *(const typename VecAt<E, MT>::type *)(q + e * ld);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) v[i][e] = x[i];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) v[i][e] = r + i < rows && k + e < kend ? q[e * ld + i] : (E)0.f;
+            }
+        }
+    }
+};
+
+// The operand on the output columns' side, shared by the waves: BN columns by KT of the summed side per stage, through
+// registers (a stage ahead) into P planes of parts in LDS, [P][BN][LROW].  KC: the summed side is contiguous in
+// memory; else the columns' side is, and the eight values of a fragment are gathered from eight rows by one thread.
+template <typename E, bool KC, int BN, int P, typename M>
+struct ColsOperand {
+    static constexpr int CW = KC ? 1 : (BN * 4 > CL_THREADS ? BN * 4 / CL_THREADS : 1);  // columns a unit
+    static constexpr int UNITS = BN * 4 / CW;
     static constexpr int NU = (UNITS + CL_THREADS - 1) / CL_THREADS;
     E v[NU][CW][8];
 
-    __device__ __forceinline__ static bool unit(int i, int &row, int &kc) {
+    __device__ __forceinline__ static bool unit(int i, int &col, int &kc) {
         const int u = threadIdx.x + i * CL_THREADS;
-        if constexpr (ROW) {
-            row = u >> 2;
+        if constexpr (KC) {
+            col = u >> 2;
             kc = u & 3;
         } else {
-            row = u % (BR / CW) * CW;
-            kc = u / (BR / CW);
+            col = u % (BN / CW) * CW;
+            kc = u / (BN / CW);
         }
         return UNITS % CL_THREADS == 0 || u < UNITS;
     }
-    // rows [row0, rows) and summed indices [k0, kend) of p, rows beyond and indices beyond read as 0
-    __device__ __forceinline__ void load(const E *__restrict__ p, long ld, long row0, long rows, long k0, long kend) {
+    // columns [col0, cols) and summed indices [k0, kend) of p, what lies beyond reads as 0
+    __device__ __forceinline__ void load(const E *__restrict__ p, long ld, long col0, long cols, long k0, long kend) {
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            int r, kc;
-            if (!unit(i, r, kc)) continue;
-            const long row = row0 + r, k = k0 + kc * 8;
-            if constexpr (ROW) {
-                const E *q = p + row * ld + k;
-                if (row < rows && k + 8 <= kend) {
+            int c0, kc;
+            if (!unit(i, c0, kc)) continue;
+            const long col = col0 + c0, k = k0 + kc * 8;
+            if constexpr (KC) {
+                const E *q = p + col * ld + k;
+                if (col < cols && k + 8 <= kend) {
                     constexpr int W = 16 / sizeof(E);
 #pragma unroll
                     for (int w = 0; w < 8 / W; ++w) {
@@ -70,11 +150,11 @@ struct Operand {
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][0][e] = row < rows && k + e < kend ? q[e] : (E)0.f;
+                    for (int e = 0; e < 8; ++e) v[i][0][e] = col < cols && k + e < kend ? q[e] : (E)0.f;
                 }
             } else {
-                const E *q = p + k * ld + row;
-                if (row + CW <= rows && k + 8 <= kend) {
+                const E *q = p + k * ld + col;
+                if (col + CW <= cols && k + 8 <= kend) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const auto x = *(const typename VecAt<E, CW>::type *)(q + e * ld);
@@ -85,55 +165,28 @@ struct Operand {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
 #pragma unroll
-                        for (int c = 0; c < CW; ++c) v[i][c][e] = row + c < rows && k + e < kend ? q[e * ld + c] : (E)0.f;
+                        for (int c = 0; c < CW; ++c) v[i][c][e] = col + c < cols && k + e < kend ? q[e * ld + c] : (E)0.f;
                 }
             }
         }
     }
-    // sums[i][c]: running sums of the values (SQUARE: of their squares)
-    template <bool SQUARE>
-    __device__ __forceinline__ void add_up(float (&sums)[NU][CW]) const {
+    __device__ __forceinline__ void add_squares(float (&sums)[NU]) const {
 #pragma unroll
         for (int i = 0; i < NU; ++i)
 #pragma unroll
-            for (int c = 0; c < CW; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = (float)v[i][c][e];
-                    sums[i][c] = SQUARE ? fmaf(x, x, sums[i][c]) : sums[i][c] + x;
-                }
+            for (int e = 0; e < 8; ++e) sums[i] = fmaf((float)v[i][0][e], (float)v[i][0][e], sums[i]);
     }
     __device__ __forceinline__ void store(M *lds) const {
-        using V = __attribute__((ext_vector_type(8))) M;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            int r, kc;
-            if (!unit(i, r, kc)) continue;
+            int c0, kc;
+            if (!unit(i, c0, kc)) continue;
 #pragma unroll
             for (int c = 0; c < CW; ++c) {
-                M *dst = lds + (r + c) * LROW + kc * 8;
-                if constexpr (sizeof(E) == 2 && P == 1) {
-                    V x;
+                Frag<M> parts[P];
+                cut<P, M>(v[i][c], parts);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = v[i][c][e];
-                    *(V *)dst = x;
-                } else {
-                    float rest[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) rest[e] = (float)v[i][c][e];
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        V x;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = (M)rest[e];
-                        *(V *)(dst + p * BR * LROW) = x;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float hi = (float)x[e];
-                            rest[e] = __builtin_isinf(hi) ? 0.f : rest[e] - hi;  // inf has no rest (inf - inf would make it NaN)
-                        }
-                    }
-                }
+                for (int p = 0; p < P; ++p) *(Frag<M> *)(lds + (p * BN + c0 + c) * LROW + kc * 8) = parts[p];
             }
         }
     }
@@ -152,14 +205,15 @@ struct ProductArgs {
     float scale;
 };
 
-template <Product OP, typename EM, typename EN, int PM, int PN, typename M, int BM, int BN, typename EO>
+// An output tile of 64 MT x 16 NT a workgroup: each wave 16 MT rows of it and all its columns.
+template <Product OP, typename EM, typename EN, int PM, int PN, typename M, int MT, int NT, typename EO>
 __global__ __launch_bounds__(CL_THREADS) void product_kernel(ProductArgs a) {
-    constexpr bool ROW_M = OP != GRAD_CODE, ROW_N = OP == LOGITS;
-    constexpr int MT = BM / 32, NT = BN / 32;  // 16 x 16 tiles of a wave
-    using V = __attribute__((ext_vector_type(8))) M;
-    __shared__ __attribute__((aligned(16))) M s_m[PM][BM][LROW];
-    __shared__ __attribute__((aligned(16))) M s_n[PN][BN][LROW];
-    __shared__ float s_sum[OP == LOGITS ? BN : (OP == GRAD_CODE ? 4 * BM : 1)];
+    constexpr bool KC_M = OP != GRAD_CODE, KC_N = OP == LOGITS;
+    constexpr int BN = NT * 16;
+    using OpM = RowsOperand<EM, KC_M, MT, PM, M>;
+    using OpN = ColsOperand<EN, KC_N, BN, PN, M>;
+    __shared__ __attribute__((aligned(16))) M s_n[2][PN][BN][LROW];
+    __shared__ float s_norm[OP == LOGITS ? BN : 1];
     // Workgroups b and b + 8 run on one XCD: the tiles that share rows (GRAD_CODE: a split) go to the same one, whose L2
     // then serves the shared operand once.
     const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
@@ -176,97 +230,99 @@ __global__ __launch_bounds__(CL_THREADS) void product_kernel(ProductArgs a) {
         tn = slot % a.tiles_n;
         if (tm >= a.tiles_m) return;
     }
-    const long m0 = (long)tm * BM, n0 = (long)tn * BN;
-    const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave & 1) * (BM / 2), wn = (wave >> 1) * (BN / 2);
-    const int fr = lane & 15, fk = (lane >> 4) * 8;  // this lane's row and first K element of a fragment
+    const long m0 = ((long)tm * 4 + wave) * (MT * 16), n0 = (long)tn * BN;
+    const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
+    const int fr = lane & 15, fk = (lane >> 4) * 8;  // this lane's row and first summed element of a fragment
 
-    using OpM = Operand<EM, ROW_M, BM, PM, M>;
-    using OpN = Operand<EN, ROW_N, BN, PN, M>;
     OpM om;
     OpN on;
-    float sums[OP == LOGITS ? OpN::NU : OpM::NU][OP == LOGITS ? OpN::CW : OpM::CW] = {};
+    float sq[OpN::NU] = {}, sum_m[MT] = {};
     f32x4 acc[MT][NT] = {};
-    om.load((const EM *)a.m, a.ld_m, m0, a.rows, k0, kend);
+    om.load((const EM *)a.m, a.ld_m, m0, a.rows, fr, k0 + fk, kend);
     on.load((const EN *)a.n, a.ld_n, n0, a.cols, k0, kend);
-    for (long k = k0; k < kend; k += KT) {
-        if (k != k0) __syncthreads();  // the fragments of the stage before have been read
-        om.store(&s_m[0][0][0]);
-        on.store(&s_n[0][0][0]);
-        if constexpr (OP == LOGITS) on.template add_up<true>(sums);
-        if constexpr (OP == GRAD_CODE) om.template add_up<false>(sums);
-        __syncthreads();
-        if (k + KT < kend) {
-            om.load((const EM *)a.m, a.ld_m, m0, a.rows, k + KT, kend);
+    on.store(&s_n[0][0][0][0]);
+    if constexpr (OP == LOGITS) on.add_squares(sq);
+    int buf = 0;
+    for (long k = k0; k < kend; k += KT, buf ^= 1) {
+        Frag<M> fm[MT][PM];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (OP == GRAD_CODE)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum_m[i] += (float)om.v[i][e];
+            cut<PM, M>(om.v[i], fm[i]);
+        }
+        const bool more = k + KT < kend;
+        if (more) {
+            om.load((const EM *)a.m, a.ld_m, m0, a.rows, fr, k + KT + fk, kend);
             on.load((const EN *)a.n, a.ld_n, n0, a.cols, k + KT, kend);
         }
-        V fm[PM][MT], fn[PN][NT];
+        // The barrier orders this stage's plane after its stores and the other plane's next stores after its last reads.
+        __syncthreads();
 #pragma unroll
-        for (int p = 0; p < PM; ++p)
+        for (int j = 0; j < NT; ++j) {
+            Frag<M> fn[PN];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) fm[p][i] = *(const V *)&s_m[p][wm + i * 16 + fr][fk];
+            for (int p = 0; p < PN; ++p) fn[p] = *(const Frag<M> *)&s_n[buf][p][j * 16 + fr][fk];
+            // the small products first
 #pragma unroll
-        for (int p = 0; p < PN; ++p)
+            for (int order = 2; order >= 0; --order)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) fn[p][j] = *(const V *)&s_n[p][wn + j * 16 + fr][fk];
-        // the small products first
+                for (int p = 0; p < PM; ++p) {
+                    const int q = order - p;
+                    if (q < 0 || q >= PN) continue;
 #pragma unroll
-        for (int order = 2; order >= 0; --order)
-#pragma unroll
-            for (int p = 0; p < PM; ++p) {
-                const int q = order - p;
-                if (q < 0 || q >= PN) continue;
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma(fn[q][j], fm[p][i], acc[i][j]);
-            }
+                    for (int i = 0; i < MT; ++i) acc[i][j] = mfma(fn[q], fm[i][p], acc[i][j]);
+                }
+        }
+        if (more) {
+            on.store(&s_n[buf ^ 1][0][0][0]);
+            if constexpr (OP == LOGITS) on.add_squares(sq);
+        }
     }
 
     if constexpr (OP == LOGITS) {  // |code|^2: four neighbouring threads hold a row's chunks
 #pragma unroll
         for (int i = 0; i < OpN::NU; ++i) {
-            int r, kc;
-            if (!OpN::unit(i, r, kc)) continue;
-            float s = sums[i][0];
+            int c, kc;
+            if (!OpN::unit(i, c, kc)) continue;
+            float s = sq[i];
             s += __shfl_xor(s, 1, 64);
             s += __shfl_xor(s, 2, 64);
-            if (kc == 0) s_sum[r] = s;
+            if (kc == 0) s_norm[c] = s;
         }
         __syncthreads();
     }
     if constexpr (OP == GRAD_CODE) {
         if (tn == 0) {
-#pragma unroll
-            for (int i = 0; i < OpM::NU; ++i) {
-                int r, kc;
-                if (!OpM::unit(i, r, kc)) continue;
-#pragma unroll
-                for (int c = 0; c < OpM::CW; ++c) s_sum[kc * BM + r + c] = sums[i][c];
-            }
-            __syncthreads();
             float *p = (float *)a.out + split * (a.rows * a.cols + a.rows) + a.rows * a.cols;
-            for (int r = threadIdx.x; r < BM; r += CL_THREADS)
-                if (m0 + r < a.rows) p[m0 + r] = (s_sum[r] + s_sum[BM + r]) + (s_sum[2 * BM + r] + s_sum[3 * BM + r]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float s = sum_m[i];
+                s += __shfl_xor(s, 16, 64);
+                s += __shfl_xor(s, 32, 64);
+                const long m = OpM::row(m0, i, fr);
+                if (lane < 16 && m < a.rows) p[m] = s;
+            }
         }
     }
     // A lane holds four consecutive columns of one row of each 16 x 16 tile.
     EO *out = (EO *)a.out + (OP == GRAD_CODE ? split * (a.rows * a.cols + a.rows) : 0);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const long m = m0 + wm + i * 16 + fr;
+        const long m = OpM::row(m0, i, fr);
         if (m >= a.rows) continue;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int nl = wn + j * 16 + (lane >> 4) * 4;
+            const int nl = j * 16 + (lane >> 4) * 4;
             const long n = n0 + nl;
             EO *dst = out + m * a.cols + n;
             typename VecAt<EO, 4>::type r;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float x = acc[i][j][e];
-                if constexpr (OP == LOGITS) x = fmaf(2.f, x, -s_sum[nl + e]) * a.scale;
+                if constexpr (OP == LOGITS) x = fmaf(2.f, x, -s_norm[nl + e]) * a.scale;
                 if constexpr (OP == GRAD_X) x *= a.scale;
                 r[e] = (EO)x;
             }
@@ -319,7 +375,7 @@ inline Tile pick_tile(long rows, long cols, long splits) {
         if (t.n == 128 && cols <= 64) continue;
         if ((long)ceil_div(rows, t.m) * ceil_div(cols, t.n) * splits >= CL_WANT) return t;
     }
-    return {32, 32};
+    return {64, 32};
 }
 
 // Splits of the summed rows of the codebook's gradient: about two workgroups of 128 x 128 or 128 x 64 per CU, at least
@@ -338,11 +394,11 @@ int launch_product(hipStream_t stream, ProductArgs a) {
     a.tiles_n = ceil_div(a.cols, t.n);
     const long grid = OP == GRAD_CODE ? (long)ceil_div(a.splits, 8) * 8 * a.tiles_m * a.tiles_n : (long)ceil_div(a.tiles_m, 8) * 8 * a.tiles_n;
     GDPSO_REQUIRE(grid < (1l << 31), "code_logits: too many rows for one call");
-#define CL_LAUNCH(TM, TN) hipLaunchKernelGGL((product_kernel<OP, EM, EN, PM, PN, M, TM, TN, EO>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a)
-    if (t.m == 128 && t.n == 128) CL_LAUNCH(128, 128);
-    else if (t.m == 128) CL_LAUNCH(128, 64);
-    else if (t.m == 64) CL_LAUNCH(64, 64);
-    else CL_LAUNCH(32, 32);
+#define CL_LAUNCH(MT, NT) hipLaunchKernelGGL((product_kernel<OP, EM, EN, PM, PN, M, MT, NT, EO>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a)
+    if (t.n == 128) CL_LAUNCH(2, 8);
+    else if (t.m == 128) CL_LAUNCH(2, 4);
+    else if (t.n == 64) CL_LAUNCH(1, 4);
+    else CL_LAUNCH(1, 2);
 #undef CL_LAUNCH
     GDPSO_HIP(hipGetLastError());
     return GDPSO_OK;
