@@ -88,9 +88,9 @@ _PROTOTYPES = {
     "gdpso_code_logits_grad_workspace_bytes": (c_size_t, [c_int] * 3),
     "gdpso_code_logits_grad": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p] * 3 + [c_int, c_float] + [c_void_p] * 3 + [c_size_t]),
     "gdpso_balance_workspace_bytes": (c_size_t, [c_int, c_int]),
-    "gdpso_balance": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, C.c_longlong, c_int, c_void_p, c_int, c_void_p, c_float] + [c_void_p] * 5
+    "gdpso_balance": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, C.c_longlong, c_int, c_void_p, c_int, c_void_p, c_float] + [c_void_p] * 6
                       + [c_size_t]),
-    "gdpso_balance_grad": (c_int, [c_void_p, c_int, c_int, c_void_p, C.c_longlong, c_int] + [c_void_p] * 4),
+    "gdpso_balance_grad": (c_int, [c_void_p, c_int, c_int, c_void_p, C.c_longlong, c_int] + [c_void_p] * 5),
     "gdpso_distill_workspace_bytes": (c_size_t, [c_int] * 3),
     "gdpso_distill": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, C.c_longlong, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_float, c_float]
                       + [c_void_p] * 5 + [c_size_t]),
@@ -177,6 +177,23 @@ def host_float_pointers(arrays):
 def stream_handle(device=None) -> int:
     """Raw hipStream_t of torch's current stream on ``device``."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def run(device, fn, *args) -> None:
+    """``fn(stream, *args)`` of the library on the current stream of ``device`` (with an index), made the current device for the call.
+    The switch and the stream object cost as much as a launch, so the first is left out where it changes nothing and the handle is
+    read directly."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(_raw_stream(index), *args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(_raw_stream(index), *args)
+    if rc:
+        check(rc)
 
 
 def ptr(t) -> int:

@@ -24,6 +24,7 @@ constexpr int WIDE_THREADS = 512; // rows of up to 16384 columns: 32 values a th
 constexpr int HIST_THREADS = 1024;
 constexpr int JOIN_COLS = 16, JOIN_GROUPS = 64;
 constexpr int HIST_MAX = 64;
+constexpr int OWN_CHOICES = 4096;  // choices that every workgroup of the gradient counts for itself (16 a thread)
 
 // Counting workgroups: sixteen choices a thread keep the loads of a thread in flight together; the partial counts are
 // read again by every workgroup of the gradient, so there are at most 64 of them.
@@ -40,16 +41,18 @@ struct Choices {
     int blocks;
     unsigned *part;  // [blocks][e + 2]: choices of every code, rows kept, choices counted
 };
+inline __host__ __device__ int hist_copies(int e) { return e <= 256 ? 8 : 1; }
 
-// Counts of this block's share of the choices.  LDS copies by lane keep the lanes of a wave off each other's counters
-// where there are few codes.
-__device__ void count_choices(const Choices &a, int block, unsigned *s_hist, int threads) {
-    const int copies = a.e <= 256 ? 8 : 1;
+// Counts of one of `blocks` shares of the choices into s_hist[0, e) and s_total (rows kept, choices counted).  Copies by
+// lane keep the lanes of a wave off each other's counters where there are few codes.
+__device__ void count_choices(const Choices &a, int block, int blocks, unsigned *s_hist, unsigned *s_total, int threads) {
+    const int copies = hist_copies(a.e);
     for (int c = threadIdx.x; c < copies * a.e; c += threads) s_hist[c] = 0;
+    if (threadIdx.x < 2) s_total[threadIdx.x] = 0;
     __syncthreads();
     unsigned *mine = s_hist + (copies > 1 ? (threadIdx.x & 7) * a.e : 0);
     unsigned rows = 0, counted = 0;
-    const long long step = (long long)a.blocks * threads, first = (long long)block * threads + threadIdx.x;
+    const long long step = (long long)blocks * threads, first = (long long)block * threads + threadIdx.x;
     if (a.mask) {
         for (long long i = first; i < a.n; i += step) {
             if (!a.mask[i]) continue;
@@ -74,31 +77,35 @@ __device__ void count_choices(const Choices &a, int block, unsigned *s_hist, int
         }
         if (block == 0 && threadIdx.x == 0) rows = a.n;
     }
-    __syncthreads();
-    unsigned *out = a.part + (size_t)block * (a.e + 2);
-    for (int c = threadIdx.x; c < a.e; c += threads) {
-        unsigned s = s_hist[c];
-        for (int r = 1; r < copies; ++r) s += s_hist[r * a.e + c];
-        out[c] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) s_hist[threadIdx.x] = 0;
-    __syncthreads();
     for (int o = 32; o > 0; o >>= 1) {
         rows += __shfl_xor(rows, o, 64);
         counted += __shfl_xor(counted, o, 64);
     }
     if ((threadIdx.x & 63) == 0) {
-        atomicAdd(&s_hist[0], rows);
-        atomicAdd(&s_hist[1], counted);
+        atomicAdd(&s_total[0], rows);
+        atomicAdd(&s_total[1], counted);
     }
     __syncthreads();
-    if (threadIdx.x < 2) out[a.e + threadIdx.x] = s_hist[threadIdx.x];
+    if (copies > 1) {
+        for (int c = threadIdx.x; c < a.e; c += threads) {
+            unsigned s = s_hist[c];
+            for (int r = 1; r < copies; ++r) s += s_hist[r * a.e + c];
+            s_hist[c] = s;
+        }
+        __syncthreads();
+    }
+}
+__device__ __forceinline__ void write_counts(const Choices &a, int block, const unsigned *s_hist, const unsigned *s_total, int threads) {
+    unsigned *out = a.part + (size_t)block * (a.e + 2);
+    for (int c = threadIdx.x; c < a.e; c += threads) out[c] = s_hist[c];
+    if (threadIdx.x < 2) out[a.e + threadIdx.x] = s_total[threadIdx.x];
 }
 
 __global__ __launch_bounds__(HIST_THREADS) void bal_count_kernel(Choices a) {
     extern __shared__ unsigned s_hist[];
-    count_choices(a, blockIdx.x, s_hist, HIST_THREADS);
+    __shared__ unsigned s_total[2];
+    count_choices(a, blockIdx.x, a.blocks, s_hist, s_total, HIST_THREADS);
+    write_counts(a, blockIdx.x, s_hist, s_total, HIST_THREADS);
 }
 
 struct BalArgs {
@@ -110,19 +117,20 @@ struct BalArgs {
     float *col_part;            // [row_blocks][e] column sums of p
     const unsigned *count_part; // [count_blocks][e + 2]
     int count_blocks;
-    const long long *counts;    // or the finished counts [e + 2]
+    const long long *counts, *totals;  // or the finished counts [e] and totals [2]
     float grad_scale;
     const float *upstream;
     void *grad;
     unsigned *ticket;           // cleared here for the join
+    bool own_counts;
 };
 
 // f into LDS and the gradient's factor grad_scale * e / rows (0 when no row is kept).
 __device__ __forceinline__ float shares(const BalArgs &a, float *s_f, int threads) {
     long long rows = 0, counted = 0;
     if (a.counts) {
-        rows = a.counts[a.e];
-        counted = a.counts[a.e + 1];
+        rows = a.totals[0];
+        counted = a.totals[1];
     } else {
         for (int h = 0; h < a.count_blocks; ++h) {
             rows += a.count_part[(size_t)h * (a.e + 2) + a.e];
@@ -147,15 +155,27 @@ template <typename E, int TEAM, int NCH, bool SUMS, bool GRAD>
 __global__ __launch_bounds__(TEAM_THREADS) void bal_team_kernel(BalArgs a, Choices ch) {
     constexpr int VEC = vec_of<E>(), TEAMS = TEAM_THREADS / TEAM;
     extern __shared__ float s_mem[];
+    __shared__ unsigned s_total[SUMS ? 2 : 1];
     if (SUMS && !GRAD && (int)blockIdx.x >= a.row_blocks) {  // without a gradient nothing waits for the counts: they ride along
-        count_choices(ch, blockIdx.x - a.row_blocks, (unsigned *)s_mem, TEAM_THREADS);
+        count_choices(ch, blockIdx.x - a.row_blocks, ch.blocks, (unsigned *)s_mem, s_total, TEAM_THREADS);
+        write_counts(ch, blockIdx.x - a.row_blocks, (unsigned *)s_mem, s_total, TEAM_THREADS);
         return;
     }
     const int pos = threadIdx.x & (TEAM - 1), team = threadIdx.x / TEAM;
     float f[NCH][VEC], acc[NCH][VEC];
     float factor = 0.f;
     if constexpr (GRAD) {
-        factor = shares(a, s_mem, TEAM_THREADS);
+        if (SUMS && a.own_counts) {  // few choices: every workgroup counts them all, which costs less than a launch ahead of this one
+            unsigned *s_hist = (unsigned *)s_mem;
+            count_choices(ch, 0, 1, s_hist, s_total, TEAM_THREADS);
+            if (blockIdx.x == 0) write_counts(ch, 0, s_hist, s_total, TEAM_THREADS);
+            const float inv = s_total[1] > 0 ? (float)(1. / (double)s_total[1]) : 0.f;
+            for (int c = threadIdx.x; c < a.e; c += TEAM_THREADS) s_mem[c] = (float)s_hist[c] * inv;
+            factor = s_total[0] > 0 ? a.grad_scale * (float)a.e / (float)s_total[0] : 0.f;
+            __syncthreads();
+        } else {
+            factor = shares(a, s_mem, TEAM_THREADS);
+        }
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
@@ -310,7 +330,8 @@ __global__ __launch_bounds__(WIDE_THREADS) void bal_wide_kernel(BalArgs a) {
 // workgroup to finish adds the workgroups' shares of the loss up in order.
 __global__ __launch_bounds__(JOIN_COLS *JOIN_GROUPS) void bal_join_kernel(int e, int row_blocks, const float *__restrict__ col_part, int count_blocks,
                                                                          const unsigned *__restrict__ count_part, float *__restrict__ mean_prob,
-                                                                         long long *__restrict__ counts, double *dots, unsigned *ticket,
+                                                                         long long *__restrict__ counts, long long *__restrict__ totals, double *dots,
+                                                                         unsigned *ticket,
                                                                          float *__restrict__ loss) {
     __shared__ double s_col[JOIN_GROUPS][JOIN_COLS];
     __shared__ unsigned s_cnt[JOIN_GROUPS][JOIN_COLS];
@@ -360,8 +381,8 @@ __global__ __launch_bounds__(JOIN_COLS *JOIN_GROUPS) void bal_join_kernel(int e,
     }
     if (threadIdx.x == 0) {
         if (blockIdx.x == 0) {
-            counts[e] = s_total[0];
-            counts[e + 1] = s_total[1];
+            totals[0] = s_total[0];
+            totals[1] = s_total[1];
         }
         if (gridDim.x == 1) {
             *loss = (float)(dot * e);
@@ -428,12 +449,12 @@ inline BalSpace balance_space(void *ws, int e) {
 }
 
 int balance_check(const char *what, int n, int e, const void *logits, long long row_stride, int dtype) {
-    const std::string w(what);
-    GDPSO_REQUIRE(n >= 0 && e > 0, w + ": n >= 0 and e > 0 are required");
-    GDPSO_REQUIRE(e <= BAL_MAX_E, w + ": more than 16384 experts");
-    GDPSO_REQUIRE(dtype_ok(dtype), w + ": unknown element type");
-    GDPSO_REQUIRE(n == 0 || logits, w + ": null argument");
-    GDPSO_REQUIRE(row_stride >= 0, w + ": negative row stride");
+    using w = std::string;
+    GDPSO_REQUIRE(n >= 0 && e > 0, w(what) + ": n >= 0 and e > 0 are required");
+    GDPSO_REQUIRE(e <= BAL_MAX_E, w(what) + ": more than 16384 experts");
+    GDPSO_REQUIRE(dtype_ok(dtype), w(what) + ": unknown element type");
+    GDPSO_REQUIRE(n == 0 || logits, w(what) + ": null argument");
+    GDPSO_REQUIRE(row_stride >= 0, w(what) + ": negative row stride");
     return GDPSO_OK;
 }
 
@@ -443,8 +464,8 @@ int launch_rows(hipStream_t stream, const BalArgs &a, const Choices &ch) {
     const bool ride = SUMS && !GRAD && h.team;
     const dim3 grid(a.row_blocks + (ride ? ch.blocks : 0));
     // f, or the column sums of a workgroup, or the counters of one that counts
-    const size_t lds = std::max((size_t)a.e, ride ? (size_t)a.e * (a.e <= 256 ? 8 : 1) : 0) * sizeof(float);
-#define BAL_TEAM(T, C) hipLaunchKernelGGL((bal_team_kernel<E, T, C, SUMS, GRAD>), grid, dim3(TEAM_THREADS), std::max(lds, (size_t)8), stream, a, ch)
+    const size_t lds = std::max((size_t)a.e, ride || a.own_counts ? (size_t)a.e * hist_copies(a.e) : 0) * sizeof(float);
+#define BAL_TEAM(T, C) hipLaunchKernelGGL((bal_team_kernel<E, T, C, SUMS, GRAD>), grid, dim3(TEAM_THREADS), lds, stream, a, ch)
     switch (h.team * 16 + h.chunks) {
         case 1 * 16 + 1: BAL_TEAM(1, 1); break;
         case 2 * 16 + 1: BAL_TEAM(2, 1); break;
@@ -477,24 +498,25 @@ extern "C" size_t gdpso_balance_workspace_bytes(int n, int e) {
 }
 
 extern "C" int gdpso_balance(void *stream_, int n, int e, int k, const void *logits, long long row_stride, int dtype, const void *indices,
-                             int index_bytes, const unsigned char *mask, float grad_scale, float *loss, long long *counts, float *mean_prob,
-                             void *grad, void *workspace, size_t workspace_bytes) {
+                             int index_bytes, const unsigned char *mask, float grad_scale, float *loss, long long *counts, long long *totals,
+                             float *mean_prob, void *grad, void *workspace, size_t workspace_bytes) {
     int rc = balance_check("balance", n, e, logits, row_stride, dtype);
     if (rc) return rc;
     GDPSO_REQUIRE(k > 0, "balance: k > 0 is required");
     GDPSO_REQUIRE((long long)n * k < (1ll << 37), "balance: too many choices for one call");
     GDPSO_REQUIRE(index_bytes == 4 || index_bytes == 8, "balance: indices are 4 or 8 bytes");
-    GDPSO_REQUIRE((n == 0 || indices) && loss && counts && mean_prob && workspace, "balance: null argument");
+    GDPSO_REQUIRE((n == 0 || indices) && loss && counts && totals && mean_prob && workspace, "balance: null argument");
     if (workspace_bytes < gdpso_balance_workspace_bytes(n, e)) return fail(GDPSO_ERR_WORKSPACE, "balance: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     const BalSpace ws = balance_space(workspace, e);
-    const bool apart = grad || e > TEAM_MAX_E;  // the counting as a launch of its own
-    const int hb = hist_blocks((long long)n * k, apart ? HIST_THREADS : TEAM_THREADS);
+    const bool own = grad && e <= TEAM_MAX_E && (long long)n * k <= OWN_CHOICES;
+    const bool apart = !own && (grad || e > TEAM_MAX_E);  // the counting as a launch of its own
+    const int hb = own ? 1 : hist_blocks((long long)n * k, apart ? HIST_THREADS : TEAM_THREADS);
     const Choices ch = {indices, index_bytes, mask, n, k, e, hb, ws.count_part};
-    BalArgs a = {n, e, logits, row_stride, mask, row_blocks(n, e, dtype), ws.col_part, ws.count_part, hb, nullptr, grad_scale, nullptr, grad, ws.ticket};
-    const size_t hist_lds = (size_t)e * (e <= 256 ? 8 : 1) * sizeof(unsigned);
+    BalArgs a = {n, e, logits, row_stride, mask, row_blocks(n, e, dtype), ws.col_part, ws.count_part, hb, nullptr, nullptr, grad_scale, nullptr,
+                 grad, ws.ticket, own};
     if (apart) {
-        hipLaunchKernelGGL(bal_count_kernel, dim3(hb), dim3(HIST_THREADS), std::max(hist_lds, (size_t)8), stream, ch);
+        hipLaunchKernelGGL(bal_count_kernel, dim3(hb), dim3(HIST_THREADS), (size_t)e * hist_copies(e) * sizeof(unsigned), stream, ch);
         GDPSO_HIP(hipGetLastError());
     }
     if (grad)
@@ -503,18 +525,19 @@ extern "C" int gdpso_balance(void *stream_, int n, int e, int k, const void *log
         GDPSO_WITH_DTYPE(dtype, rc = (launch_rows<E, true, false>(stream, a, ch)));
     if (rc) return rc;
     hipLaunchKernelGGL(bal_join_kernel, dim3(ceil_div(e, JOIN_COLS)), dim3(JOIN_COLS * JOIN_GROUPS), 0, stream, e, a.row_blocks, ws.col_part, hb,
-                       ws.count_part, mean_prob, counts, ws.dots, ws.ticket, loss);
+                       ws.count_part, mean_prob, counts, totals, ws.dots, ws.ticket, loss);
     GDPSO_HIP(hipGetLastError());
     return GDPSO_OK;
 }
 
 extern "C" int gdpso_balance_grad(void *stream_, int n, int e, const void *logits, long long row_stride, int dtype, const unsigned char *mask,
-                                  const long long *counts, const float *upstream, void *grad) {
+                                  const long long *counts, const long long *totals, const float *upstream, void *grad) {
     int rc = balance_check("balance_grad", n, e, logits, row_stride, dtype);
     if (rc) return rc;
-    GDPSO_REQUIRE(n == 0 || (counts && upstream && grad), "balance_grad: null argument");
+    GDPSO_REQUIRE(n == 0 || (counts && totals && upstream && grad), "balance_grad: null argument");
     if (n == 0) return GDPSO_OK;
-    const BalArgs a = {n, e, logits, row_stride, mask, row_blocks(n, e, dtype), nullptr, nullptr, 0, counts, 0.f, upstream, grad, nullptr};
+    const BalArgs a = {n, e, logits, row_stride, mask, row_blocks(n, e, dtype), nullptr, nullptr, 0, counts, totals, 0.f, upstream,
+                       grad, nullptr, false};
     GDPSO_WITH_DTYPE(dtype, rc = (launch_rows<E, false, true>((hipStream_t)stream_, a, Choices{})));
     return rc;
 }

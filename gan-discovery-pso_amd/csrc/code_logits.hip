@@ -15,6 +15,9 @@
 // forward product of two 16-bit operands needs no cutting.
 #include "loss_rows.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace gdpso {
 namespace {
 
@@ -29,6 +32,12 @@ using f16x8 = __attribute__((ext_vector_type(8))) f16_t;
 template <typename M>
 using Frag = __attribute__((ext_vector_type(8))) M;
 
+// p[off] for a pointer that is the same in the whole wave and a lane's offset in bytes: a scalar base and one register.
+template <typename V, typename E>
+__device__ __forceinline__ V at_bytes(const E *p, unsigned off) {
+    return *(const V *)((const char *)p + off);
+}
+
 // Cuts eight values into P parts of type M: parts[p] is the rounded rest of what the parts before it leave.
 template <int P, typename M, typename E>
 __device__ __forceinline__ void cut(const E (&v)[8], Frag<M> (&parts)[P]) {
@@ -36,27 +45,35 @@ __device__ __forceinline__ void cut(const E (&v)[8], Frag<M> (&parts)[P]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) parts[0][e] = v[e];
     } else {
-        float rest[8], most = 0.f;
+        static_assert(__is_same(M, bf16_t), "parts are bf16");
+        using f32x2 = __attribute__((ext_vector_type(2))) float;
+        using bf16x2 = __attribute__((ext_vector_type(2))) bf16_t;
+        using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+        u32x4 words[P];
+        float most = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            rest[e] = (float)v[e];
-            most = fmaxf(most, fabsf(rest[e]));
-        }
+        for (int w = 0; w < 4; ++w) {  // two values at a time: one conversion instruction packs both
+            f32x2 rest = {(float)v[2 * w], (float)v[2 * w + 1]};
+            if (P > 1) most = fmaxf(most, fmaxf(fabsf(rest[0]), fabsf(rest[1])));
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) parts[p][e] = (M)rest[e];
-            if (p + 1 < P)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) rest[e] -= (float)parts[p][e];
+            for (int p = 0; p < P; ++p) {
+                const unsigned bits = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, bf16x2));
+                words[p][w] = bits;
+                rest[0] -= __builtin_bit_cast(float, bits << 16);
+                rest[1] -= __builtin_bit_cast(float, bits & 0xffff0000u);
+            }
         }
         if (P > 1 && most > 3.3895e38f) {  // an infinite first part (inf, or rounded up to it) has no rest: inf - inf made it NaN
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (__builtin_isinf((float)parts[0][e]))
+            for (int w = 0; w < 4; ++w) {
+                const unsigned low = (words[0][w] & 0x7fffu) == 0x7f80u ? 0u : 0xffffu;
+                const unsigned high = (words[0][w] & 0x7fff0000u) == 0x7f800000u ? 0u : 0xffff0000u;
 #pragma unroll
-                    for (int p = 1; p < P; ++p) parts[p][e] = (M)0.f;
+                for (int p = 1; p < P; ++p) words[p][w] &= low | high;
+            }
         }
+#pragma unroll
+        for (int p = 0; p < P; ++p) parts[p] = __builtin_bit_cast(Frag<M>, words[p]);
     }
 }
 
@@ -71,40 +88,55 @@ struct RowsOperand {
     E v[MT][8];
 
     __device__ __forceinline__ static long row(long wave_row0, int i, int fr) { return KC ? wave_row0 + i * 16 + fr : wave_row0 + fr * MT + i; }
-    // values [k, kend) of this lane's rows; indices beyond read as 0, rows beyond as the last one (KC) or 0: nothing uses them
-    __device__ __forceinline__ void load(const E *__restrict__ p, long ld, long wave_row0, long rows, int fr, long k, long kend) {
+    // The wave's first row and, from there, the byte offsets of this lane's piece of a stage.  Rows beyond the last one are
+    // clamped into the matrix (nothing uses their results); a vector over MT neighbouring rows (`pairs`) is clamped as a
+    // whole, so that it ends with the matrix's last row.  Whole stages load without a branch, so that the compiler can
+    // leave later stages' loads on the way while it waits for this one's.
+    __device__ __forceinline__ static long first_row(long wave_row0, long rows, bool pairs) { return min(wave_row0, rows - (!KC && pairs ? MT : 1)); }
+    __device__ __forceinline__ static void offsets(long ld, long wave_row0, long rows, int fr, int fk, bool pairs, unsigned (&off)[MT]) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const long last = !KC && pairs ? rows - MT + i : rows - 1;
+            const long r = min(row(wave_row0, i, fr), last) - first_row(wave_row0, rows, pairs);
+            off[i] = (unsigned)((KC ? r * ld + fk : fk * ld + r) * (long)sizeof(E));
+        }
+    }
+    // stage: the wave's first row at the stage's first summed element; pairs: a lane's MT rows are neighbours after clamping
+    __device__ __forceinline__ void load_whole(const E *__restrict__ stage, long ld, const unsigned (&off)[MT], bool pairs) {
         if constexpr (KC) {
+            constexpr int W = 16 / sizeof(E);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const E *q = p + min(row(wave_row0, i, fr), rows - 1) * ld + k;
-                if (k + 8 <= kend) {
-                    constexpr int W = 16 / sizeof(E);
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int w = 0; w < 8 / W; ++w) {
-                        const auto x = *(const typename VecAt<E, W>::type *)(q + w * W);
+                for (int w = 0; w < 8 / W; ++w) {
+                    const auto x = at_bytes<typename VecAt<E, W>::type>(stage + w * W, off[i]);
 #pragma unroll
-                        for (int e = 0; e < W; ++e) v[i][w * W + e] = x[e];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][e] = k + e < kend ? q[e] : (E)0.f;
+                    for (int e = 0; e < W; ++e) v[i][w * W + e] = x[e];
                 }
+        } else if (pairs) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const auto x = at_bytes<typename VecAt<E, MT>::type>(stage + e * ld, off[0]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) v[i][e] = x[i];
             }
         } else {
-            const long r = row(wave_row0, 0, fr);
-            const E *q = p + k * ld + r;
-            if (r + MT <= rows && k + 8 <= kend) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const auto x = *(const typename VecAt<E, MT>::type *)(q + e * ld);
+            for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) v[i][e] = x[i];
-                }
-            } else {
+                for (int i = 0; i < MT; ++i) v[i][e] = at_bytes<E>(stage + e * ld, off[i]);
+        }
+    }
+    // The stage that the sum's end cuts: `left` elements of it are there, the others read as 0.
+    __device__ __forceinline__ void load_part(const E *__restrict__ stage, long ld, const unsigned (&off)[MT], int fk, int left) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 8; ++e) {
+            const int back = max(0, fk + e - (left - 1));  // elements beyond the last one that is there
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) v[i][e] = r + i < rows && k + e < kend ? q[e * ld + i] : (E)0.f;
+            for (int i = 0; i < MT; ++i) {
+                const long step = ((long)e - back) * (KC ? 1 : ld) * (long)sizeof(E);
+                const E x = at_bytes<E>(stage, (unsigned)(off[i] + step));
+                v[i][e] = back == 0 ? x : (E)0.f;
             }
         }
     }
@@ -131,41 +163,59 @@ struct ColsOperand {
         }
         return UNITS % CL_THREADS == 0 || u < UNITS;
     }
-    // columns [col0, cols) and summed indices [k0, kend) of p, what lies beyond reads as 0
-    __device__ __forceinline__ void load(const E *__restrict__ p, long ld, long col0, long cols, long k0, long kend) {
+    // As RowsOperand::offsets and load_whole, from the tile's first column; threads without a unit repeat another's.
+    __device__ __forceinline__ static void offsets(long ld, long col0, long cols, bool pairs, unsigned (&off)[NU][CW]) {
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             int c0, kc;
-            if (!unit(i, c0, kc)) continue;
-            const long col = col0 + c0, k = k0 + kc * 8;
+            unit(i, c0, kc);
+            kc &= 3;
+#pragma unroll
+            for (int c = 0; c < CW; ++c) {
+                const long col = min(col0 + c0 + c, !KC && pairs ? cols - CW + c : cols - 1) - col0;
+                off[i][c] = (unsigned)((KC ? col * ld + kc * 8 : kc * 8 * ld + col) * (long)sizeof(E));
+            }
+        }
+    }
+    __device__ __forceinline__ void load_whole(const E *__restrict__ stage, long ld, const unsigned (&off)[NU][CW], bool pairs) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
             if constexpr (KC) {
-                const E *q = p + col * ld + k;
-                if (col < cols && k + 8 <= kend) {
-                    constexpr int W = 16 / sizeof(E);
+                constexpr int W = 16 / sizeof(E);
 #pragma unroll
-                    for (int w = 0; w < 8 / W; ++w) {
-                        const auto x = *(const typename VecAt<E, W>::type *)(q + w * W);
+                for (int w = 0; w < 8 / W; ++w) {
+                    const auto x = at_bytes<typename VecAt<E, W>::type>(stage + w * W, off[i][0]);
 #pragma unroll
-                        for (int e = 0; e < W; ++e) v[i][0][w * W + e] = x[e];
-                    }
-                } else {
+                    for (int e = 0; e < W; ++e) v[i][0][w * W + e] = x[e];
+                }
+            } else if (pairs) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][0][e] = col < cols && k + e < kend ? q[e] : (E)0.f;
+                for (int e = 0; e < 8; ++e) {
+                    const auto x = at_bytes<typename VecAt<E, CW>::type>(stage + e * ld, off[i][0]);
+#pragma unroll
+                    for (int c = 0; c < CW; ++c) v[i][c][e] = x[c];
                 }
             } else {
-                const E *q = p + k * ld + col;
-                if (col + CW <= cols && k + 8 <= kend) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const auto x = *(const typename VecAt<E, CW>::type *)(q + e * ld);
+                for (int e = 0; e < 8; ++e)
 #pragma unroll
-                        for (int c = 0; c < CW; ++c) v[i][c][e] = x[c];
-                    }
-                } else {
+                    for (int c = 0; c < CW; ++c) v[i][c][e] = at_bytes<E>(stage + e * ld, off[i][c]);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_part(const E *__restrict__ stage, long ld, const unsigned (&off)[NU][CW], int left) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+        for (int i = 0; i < NU; ++i) {
+            int c0, kc;
+            unit(i, c0, kc);
 #pragma unroll
-                        for (int c = 0; c < CW; ++c) v[i][c][e] = col + c < cols && k + e < kend ? q[e * ld + c] : (E)0.f;
+            for (int e = 0; e < 8; ++e) {
+                const int back = max(0, (kc & 3) * 8 + e - (left - 1));
+#pragma unroll
+                for (int c = 0; c < CW; ++c) {
+                    const long step = ((long)e - back) * (KC ? 1 : ld) * (long)sizeof(E);
+                    const E x = at_bytes<E>(stage, (unsigned)(off[i][c] + step));
+                    v[i][c][e] = back == 0 ? x : (E)0.f;
                 }
             }
         }
@@ -192,31 +242,70 @@ struct ColsOperand {
     }
 };
 
+// Squared norms of the codes of a tile: four neighbouring threads hold a code's chunks.
+template <typename OpN>
+__device__ __forceinline__ void norms(const float (&sq)[OpN::NU], float *s_norm) {
+#pragma unroll
+    for (int i = 0; i < OpN::NU; ++i) {
+        int c, kc;
+        if (!OpN::unit(i, c, kc)) continue;
+        float s = sq[i];
+        s += __shfl_xor(s, 1, 64);
+        s += __shfl_xor(s, 2, 64);
+        if (kc == 0) s_norm[c] = s;
+    }
+}
+
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 struct ProductArgs {
     const void *m, *n;  // operands: output rows' side and output columns' side
-    void *out;          // LOGITS, GRAD_X: result; GRAD_CODE: partial sums [split][rows * cols + rows]
+    void *out;          // result; GRAD_CODE with several splits: partial sums, float [split][rows * cols + rows]
     long rows, cols, sum;
     long ld_m, ld_n;
     int tiles_m, tiles_n, splits;
     long sum_per_split;  // a multiple of KT
     float scale;
+    const void *code;    // GRAD_CODE with one split: the codebook
 };
+// LDS of a tile: two stages of the columns' operand, and the norms of its codes.
+template <Product OP, int PN, int NT>
+constexpr int tile_lds() {
+    return 2 * PN * NT * 16 * LROW * 2 + (OP == LOGITS ? NT * 16 * 4 : 0);
+}
 
-// An output tile of 64 MT x 16 NT a workgroup: each wave 16 MT rows of it and all its columns.
+// Four consecutive columns of a row.
+template <typename EO>
+__device__ __forceinline__ void put4(EO *row, long n, long cols, const float (&x)[4]) {
+    typename VecAt<EO, 4>::type r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (EO)x[e];
+    if (n + 4 <= cols) *(typename VecAt<EO, 4>::type *)(row + n) = r;
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < cols) row[n + e] = r[e];
+}
+
+// One workgroup's tile of 64 MT x 16 NT outputs: each wave 16 MT rows of it and all its columns.  depth() stages of both
+// operands are on the way while one multiplies: a stage's matrix instructions take less time than memory to answer, the
+// more so in the small tiles that small products take.
+template <int NT>
+constexpr int depth() {
+    return NT == 2 ? 4 : 2;
+}
 template <Product OP, typename EM, typename EN, int PM, int PN, typename M, int MT, int NT, typename EO>
-__global__ __launch_bounds__(CL_THREADS) void product_kernel(ProductArgs a) {
+__device__ __forceinline__ void product_tile(const ProductArgs &a, const int block, char *lds) {
     constexpr bool KC_M = OP != GRAD_CODE, KC_N = OP == LOGITS;
     constexpr int BN = NT * 16;
     using OpM = RowsOperand<EM, KC_M, MT, PM, M>;
     using OpN = ColsOperand<EN, KC_N, BN, PN, M>;
-    __shared__ __attribute__((aligned(16))) M s_n[2][PN][BN][LROW];
-    __shared__ float s_norm[OP == LOGITS ? BN : 1];
+    M(*s_n)[PN][BN][LROW] = (M(*)[PN][BN][LROW])lds;
+    float *s_norm = (float *)(lds + 2 * PN * BN * LROW * sizeof(M));
     // Workgroups b and b + 8 run on one XCD: the tiles that share rows (GRAD_CODE: a split) go to the same one, whose L2
     // then serves the shared operand once.
-    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int xcd = block & 7, slot = block >> 3;
     int tm, tn, split;
     if constexpr (OP == GRAD_CODE) {
         const int per = a.tiles_m * a.tiles_n;
@@ -230,36 +319,37 @@ __global__ __launch_bounds__(CL_THREADS) void product_kernel(ProductArgs a) {
         tn = slot % a.tiles_n;
         if (tm >= a.tiles_m) return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long m0 = ((long)tm * 4 + wave) * (MT * 16), n0 = (long)tn * BN;
     const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
     const int fr = lane & 15, fk = (lane >> 4) * 8;  // this lane's row and first summed element of a fragment
 
-    OpM om;
-    OpN on;
+    constexpr int DEPTH = depth<NT>();
+    OpM om[DEPTH];
+    OpN on[DEPTH];
     float sq[OpN::NU] = {}, sum_m[MT] = {};
     f32x4 acc[MT][NT] = {};
-    om.load((const EM *)a.m, a.ld_m, m0, a.rows, fr, k0 + fk, kend);
-    on.load((const EN *)a.n, a.ld_n, n0, a.cols, k0, kend);
-    on.store(&s_n[0][0][0][0]);
-    if constexpr (OP == LOGITS) on.add_squares(sq);
-    int buf = 0;
-    for (long k = k0; k < kend; k += KT, buf ^= 1) {
-        Frag<M> fm[MT][PM];
+    // a lane's MT rows (a unit's CW columns) are all there or none where their number divides evenly
+    const bool pairs_m = a.rows % MT == 0, pairs_n = a.cols % OpN::CW == 0;
+    unsigned off_m[MT], off_n[OpN::NU][OpN::CW];
+    OpM::offsets(a.ld_m, m0, a.rows, fr, fk, pairs_m, off_m);
+    OpN::offsets(a.ld_n, n0, a.cols, pairs_n, off_n);
+    const EM *const pm = (const EM *)a.m + OpM::first_row(m0, a.rows, pairs_m) * (KC_M ? a.ld_m : 1);
+    const EN *const pn = (const EN *)a.n + (KC_N ? n0 * a.ld_n : n0);
+    const auto stage = [&](OpN &n, int buf, bool there) {
+        n.store(&s_n[buf][0][0][0]);
+        if (OP == LOGITS && there) n.add_squares(sq);
+    };
+    const auto rows_fragments = [&](const OpM &m, Frag<M> (&fm)[MT][PM]) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if constexpr (OP == GRAD_CODE)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum_m[i] += (float)om.v[i][e];
-            cut<PM, M>(om.v[i], fm[i]);
+                for (int e = 0; e < 8; ++e) sum_m[i] += (float)m.v[i][e];
+            cut<PM, M>(m.v[i], fm[i]);
         }
-        const bool more = k + KT < kend;
-        if (more) {
-            om.load((const EM *)a.m, a.ld_m, m0, a.rows, fr, k + KT + fk, kend);
-            on.load((const EN *)a.n, a.ld_n, n0, a.cols, k + KT, kend);
-        }
-        // The barrier orders this stage's plane after its stores and the other plane's next stores after its last reads.
-        __syncthreads();
+    };
+    const auto multiply = [&](const Frag<M> (&fm)[MT][PM], int buf) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             Frag<M> fn[PN];
@@ -276,63 +366,204 @@ __global__ __launch_bounds__(CL_THREADS) void product_kernel(ProductArgs a) {
                     for (int i = 0; i < MT; ++i) acc[i][j] = mfma(fn[q], fm[i][p], acc[i][j]);
                 }
         }
-        if (more) {
-            on.store(&s_n[buf ^ 1][0][0][0]);
-            if constexpr (OP == LOGITS) on.add_squares(sq);
-        }
-    }
-
-    if constexpr (OP == LOGITS) {  // |code|^2: four neighbouring threads hold a row's chunks
-#pragma unroll
-        for (int i = 0; i < OpN::NU; ++i) {
-            int c, kc;
-            if (!OpN::unit(i, c, kc)) continue;
-            float s = sq[i];
-            s += __shfl_xor(s, 1, 64);
-            s += __shfl_xor(s, 2, 64);
-            if (kc == 0) s_norm[c] = s;
-        }
+    };
+    // Whole stages: the loads ahead are never skipped (past the last stage they repeat it), so that the compiler can tell how
+    // many are behind the one it waits for.
+    const int stages = (int)((kend - k0) / KT);
+    const auto load = [&](OpM &m, OpN &n, int s) {
+        const long k = k0 + (long)min(s, stages - 1) * KT;
+        m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m, pairs_m);
+        n.load_whole(pn + (KC_N ? k : k * a.ld_n), a.ld_n, off_n, pairs_n);
+    };
+    // stage s: its rows' operand is in om[CUR], its columns' in plane CUR & 1
+    const auto step = [&](auto which, int s) {
+        constexpr int CUR = decltype(which)::value, NEXT = (CUR + 1) % DEPTH;
+        Frag<M> fm[MT][PM];
+        rows_fragments(om[CUR], fm);
+        load(om[CUR], on[CUR], s + DEPTH);
+        // The barrier orders this plane's reads after its stores, and the other plane's next stores after its last reads.
         __syncthreads();
-    }
-    if constexpr (OP == GRAD_CODE) {
-        if (tn == 0) {
-            float *p = (float *)a.out + split * (a.rows * a.cols + a.rows) + a.rows * a.cols;
+        multiply(fm, CUR & 1);
+        stage(on[NEXT], NEXT & 1, s + 1 < stages);
+    };
+    if (stages > 0) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                float s = sum_m[i];
-                s += __shfl_xor(s, 16, 64);
-                s += __shfl_xor(s, 32, 64);
-                const long m = OpM::row(m0, i, fr);
-                if (lane < 16 && m < a.rows) p[m] = s;
+        for (int i = 0; i < DEPTH; ++i) load(om[i], on[i], i);
+        stage(on[0], 0, true);
+        for (int s = 0; s < stages; s += DEPTH) {
+            step(std::integral_constant<int, 0>{}, s);
+            if (s + 1 >= stages) break;
+            step(std::integral_constant<int, 1>{}, s + 1);
+            if constexpr (DEPTH == 4) {
+                if (s + 2 >= stages) break;
+                step(std::integral_constant<int, 2>{}, s + 2);
+                if (s + 3 >= stages) break;
+                step(std::integral_constant<int, 3>{}, s + 3);
             }
         }
     }
+    const long done = k0 + (long)stages * KT;
+    if (done < kend) {  // what is left of the sum
+        const int left = (int)(kend - done);
+        om[0].load_part(pm + (KC_M ? done : done * a.ld_m), a.ld_m, off_m, fk, left);
+        on[0].load_part(pn + (KC_N ? done : done * a.ld_n), a.ld_n, off_n, left);
+        Frag<M> fm[MT][PM];
+        rows_fragments(om[0], fm);
+        __syncthreads();
+        stage(on[0], 0, true);
+        __syncthreads();
+        multiply(fm, 0);
+    }
+
+    if constexpr (OP == LOGITS) {  // |code|^2: four neighbouring threads hold a row's chunks
+        norms<OpN>(sq, s_norm);
+        __syncthreads();
+    }
+    if constexpr (OP == GRAD_CODE) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            sum_m[i] += __shfl_xor(sum_m[i], 16, 64);
+            sum_m[i] += __shfl_xor(sum_m[i], 32, 64);
+        }
+    }
+    const bool part = OP == GRAD_CODE && a.splits > 1;
+    float *partial = (float *)a.out + split * (a.rows * a.cols + a.rows);
     // A lane holds four consecutive columns of one row of each 16 x 16 tile.
-    EO *out = (EO *)a.out + (OP == GRAD_CODE ? split * (a.rows * a.cols + a.rows) : 0);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const long m = OpM::row(m0, i, fr);
         if (m >= a.rows) continue;
+        if (part && tn == 0 && lane < 16) partial[a.rows * a.cols + m] = sum_m[i];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int nl = j * 16 + (lane >> 4) * 4;
             const long n = n0 + nl;
-            EO *dst = out + m * a.cols + n;
-            typename VecAt<EO, 4>::type r;
+            float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = acc[i][j][e];
-                if constexpr (OP == LOGITS) x = fmaf(2.f, x, -s_norm[nl + e]) * a.scale;
-                if constexpr (OP == GRAD_X) x *= a.scale;
-                r[e] = (EO)x;
+                x[e] = acc[i][j][e];
+                if constexpr (OP == LOGITS) x[e] = fmaf(2.f, x[e], -s_norm[nl + e]) * a.scale;
+                if constexpr (OP == GRAD_X) x[e] *= a.scale;
+                if constexpr (OP == GRAD_CODE)
+                    if (!part && n + e < a.cols) x[e] = a.scale * fmaf(-sum_m[i], (float)((const EN *)a.code)[m * a.cols + n + e], x[e]);
             }
-            if (n + 4 <= a.cols) *(typename VecAt<EO, 4>::type *)dst = r;
-            else
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < a.cols) dst[e] = r[e];
+            if (part) put4(partial + m * a.cols, n, a.cols, x);
+            else put4((EO *)a.out + m * a.cols, n, a.cols, x);
         }
     }
+}
+
+// The logits of long rows (those whose fragments logits_kernel could not keep in registers).
+template <typename E, int P, typename M, int MT, int NT>
+__global__ __launch_bounds__(CL_THREADS, 2) void logits_tile_kernel(ProductArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds<LOGITS, P, NT>()];
+    product_tile<LOGITS, E, E, P, P, M, MT, NT, float>(a, blockIdx.x, lds);
+}
+
+// The logits: a workgroup keeps the fragments of its 64 MT rows for all NS stages of the sum in registers, cut once, and
+// walks over its share of the codes, 64 at a time; their stores drain while the next codes multiply.  The output is what has
+// to move (d is small against the number of codes), so nothing else is read twice.
+template <typename E, int P, typename M, int NS, int MT>
+__global__ __launch_bounds__(CL_THREADS) void logits_kernel(ProductArgs a) {
+    constexpr int NT = 4, BN = NT * 16;
+    using OpM = RowsOperand<E, true, MT, P, M>;
+    using OpN = ColsOperand<E, true, BN, P, M>;
+    __shared__ __attribute__((aligned(16))) M s_n[NS][P][BN][LROW];
+    __shared__ float s_norm[BN];
+    // tiles_n here: workgroups that share a tile of rows
+    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int tm = slot / a.tiles_n * 8 + xcd, first = slot % a.tiles_n;
+    if (tm >= a.tiles_m) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long m0 = ((long)tm * 4 + wave) * (MT * 16);
+    const int fr = lane & 15, fk = (lane >> 4) * 8;
+    const int col_tiles = (int)((a.cols + BN - 1) / BN);
+    OpN on[NS];
+    // The workgroups start at different codes: rows of logits lie a multiple of 1 KiB apart as often as not, and side by side in
+    // the same columns all of them would write to the same few memory channels.
+    const int mine = (col_tiles - first + a.tiles_n - 1) / a.tiles_n, turn = tm % mine;
+    const auto col_tile = [&](int i) { return first + (i + turn < mine ? i + turn : i + turn - mine) * a.tiles_n; };
+    const auto load_codes = [&](int t) {
+        unsigned off[OpN::NU][OpN::CW];
+        OpN::offsets(a.ld_n, (long)t * BN, a.cols, false, off);
+        const E *p = (const E *)a.n + (long)t * BN * a.ld_n;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int left = (int)a.sum - s * KT;  // only the last stage may be cut
+            if (s + 1 < NS || left >= KT) on[s].load_whole(p + s * KT, a.ld_n, off, true);
+            else on[s].load_part(p + s * KT, a.ld_n, off, left);
+        }
+    };
+    Frag<M> fm[NS][MT][P];
+    {
+        OpM om[NS];
+        unsigned off[MT];
+        OpM::offsets(a.ld_m, m0, a.rows, fr, fk, false, off);
+        const E *p = (const E *)a.m + OpM::first_row(m0, a.rows, false) * a.ld_m;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int left = (int)a.sum - s * KT;
+            if (s + 1 < NS || left >= KT) om[s].load_whole(p + s * KT, a.ld_m, off, true);
+            else om[s].load_part(p + s * KT, a.ld_m, off, fk, left);
+        }
+        load_codes(col_tile(0));
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) cut<P, M>(om[s].v[i], fm[s][i]);
+    }
+    for (int i = 0; i < mine; ++i) {
+        const int t = col_tile(i);
+        if (i != 0) __syncthreads();  // all waves are through with the codes before
+        float sq[OpN::NU] = {};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            on[s].store(&s_n[s][0][0][0]);
+            on[s].add_squares(sq);
+        }
+        norms<OpN>(sq, s_norm);
+        __syncthreads();
+        if (i + 1 < mine) load_codes(col_tile(i + 1));
+        f32x4 acc[MT][NT] = {};
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                Frag<M> fn[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) fn[p] = *(const Frag<M> *)&s_n[s][p][j * 16 + fr][fk];
+#pragma unroll
+                for (int order = 2; order >= 0; --order)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const int q = order - p;
+                        if (q < 0 || q >= P) continue;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) acc[i][j] = mfma(fn[q], fm[s][i][p], acc[i][j]);
+                    }
+            }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const long m = OpM::row(m0, i, fr);
+            if (m >= a.rows) continue;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int nl = j * 16 + (lane >> 4) * 4;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(2.f, acc[i][j][e], -s_norm[nl + e]) * a.scale;
+                put4((float *)a.out + m * a.cols, (long)t * BN + nl, a.cols, x);
+            }
+        }
+    }
+}
+
+// Both gradients in one launch, the codebook's workgroups first (they run longer).
+template <typename E, int P, int MT, int NT>
+__global__ __launch_bounds__(CL_THREADS, 2) void grads_kernel(ProductArgs code, int code_blocks, ProductArgs x) {
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds<GRAD_X, P, NT>()];
+    if ((int)blockIdx.x < code_blocks) product_tile<GRAD_CODE, float, E, 3, P, bf16_t, MT, NT, E>(code, blockIdx.x, lds);
+    else product_tile<GRAD_X, float, E, 3, P, bf16_t, MT, NT, E>(x, blockIdx.x - code_blocks, lds);
 }
 
 // Joins the splits' partial sums in a fixed order: 64 neighbouring elements a workgroup, the splits dealt to its waves.
@@ -364,64 +595,103 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void code_join_kernel(int d, int k
     }
 }
 
-// Output tile: the largest that still gives every CU a workgroup; a side of at most 64 takes 64.
-constexpr int CL_WANT = 256;
-struct Tile {
-    int m, n;
-};
-inline Tile pick_tile(long rows, long cols, long splits) {
-    const Tile tiles[] = {{128, 128}, {128, 64}, {64, 64}};
-    for (const Tile &t : tiles) {
-        if (t.n == 128 && cols <= 64) continue;
-        if ((long)ceil_div(rows, t.m) * ceil_div(cols, t.n) * splits >= CL_WANT) return t;
-    }
-    return {64, 32};
-}
-
-// Splits of the summed rows of the codebook's gradient: about two workgroups of 128 x 128 or 128 x 64 per CU, at least
-// 128 rows a split (the partial sums a split writes and the join reads have to stay small beside its rows).
-inline int code_splits(int n, int d, int k) {
-    if (n <= 0) return 0;
-    const long tiles = (long)ceil_div(k, 128) * ceil_div(d, d <= 64 ? 64 : 128);
-    const long want = ceil_div(512, tiles), most = ceil_div(n, 128);
-    return (int)(want < most ? want : most);
-}
-
-template <Product OP, typename EM, typename EN, int PM, int PN, typename M, typename EO>
-int launch_product(hipStream_t stream, ProductArgs a) {
-    const Tile t = pick_tile(a.rows, a.cols, a.splits);
-    a.tiles_m = ceil_div(a.rows, t.m);
-    a.tiles_n = ceil_div(a.cols, t.n);
-    const long grid = OP == GRAD_CODE ? (long)ceil_div(a.splits, 8) * 8 * a.tiles_m * a.tiles_n : (long)ceil_div(a.tiles_m, 8) * 8 * a.tiles_n;
-    GDPSO_REQUIRE(grid < (1l << 31), "code_logits: too many rows for one call");
-#define CL_LAUNCH(MT, NT) hipLaunchKernelGGL((product_kernel<OP, EM, EN, PM, PN, M, MT, NT, EO>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a)
-    if (t.n == 128) CL_LAUNCH(2, 8);
-    else if (t.m == 128) CL_LAUNCH(2, 4);
-    else if (t.n == 64) CL_LAUNCH(1, 4);
-    else CL_LAUNCH(1, 2);
-#undef CL_LAUNCH
-    GDPSO_HIP(hipGetLastError());
-    return GDPSO_OK;
-}
-
 template <typename E>
 constexpr int grad_parts() {
     return is_f32<E>() ? 3 : (__is_same(E, f16_t) ? 2 : 1);
 }
 
+// Gradient tiles of 64 MT rows by 16 NT columns.  All d columns in one tile up to 256 (the rows' operand, the large one, is
+// then read and cut once); with few rows tiles of 32 columns, so that more CUs share them.
+struct Tile {
+    int mt, nt;
+};
+inline Tile grad_tile(int n, int d) {
+    if (n <= 4096) return {1, 2};
+    const int nt = d <= 32 ? 2 : (d <= 64 ? 4 : (d <= 128 ? 8 : 16));
+    // 128 rows a workgroup once they fill the chip; 256 columns leave registers for 64
+    return {nt < 16 && n >= 32768 ? 2 : 1, nt};
+}
+// Splits of the summed rows of the codebook's gradient: about two workgroups a CU, at least 128 rows each (the partial
+// sums that a split writes and the join reads have to stay small beside its rows).  Up to 512 rows one split does without
+// the join's launch.
+inline int code_splits(int n, int d, int k) {
+    if (n <= 512) return n > 0 ? 1 : 0;
+    const Tile t = grad_tile(n, d);
+    const long tiles = (long)ceil_div(k, 64 * t.mt) * ceil_div(d, 16 * t.nt);
+    const long want = ceil_div(512, tiles), most = ceil_div(n, 128);
+    return (int)(want < most ? want : most);
+}
+
 template <typename E>
-int logits_product(hipStream_t stream, const ProductArgs &a) {
-    if constexpr (is_f32<E>()) return launch_product<LOGITS, float, float, 3, 3, bf16_t, float>(stream, a);
-    else return launch_product<LOGITS, E, E, 1, 1, E, float>(stream, a);
+int launch_logits(hipStream_t stream, ProductArgs a) {
+    constexpr int P = is_f32<E>() ? 3 : 1;
+    using M = std::conditional_t<is_f32<E>(), bf16_t, E>;
+    const int stages = ceil_div(a.sum, KT);
+    const bool held = stages <= (is_f32<E>() ? 4 : 8);
+    // 128 rows a workgroup once they fill the chip, else 64, and then several workgroups share a tile's codes
+    const int mt = a.rows >= 32768 ? 2 : 1, bn = held ? 64 : 128;
+    a.tiles_m = ceil_div(a.rows, 64 * mt);
+    const int col_tiles = ceil_div(a.cols, bn);
+    a.tiles_n = held ? std::min(col_tiles, std::max(1, ceil_div(512, a.tiles_m))) : col_tiles;
+    const long grid = (long)ceil_div(a.tiles_m, 8) * 8 * a.tiles_n;
+    GDPSO_REQUIRE(grid < (1l << 31), "code_logits: too many rows for one call");
+#define CL_LOGITS(NS)                                                                                                                        \
+    do {                                                                                                                                     \
+        if (mt == 2) hipLaunchKernelGGL((logits_kernel<E, P, M, NS, 2>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a);              \
+        else hipLaunchKernelGGL((logits_kernel<E, P, M, NS, 1>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a);                      \
+    } while (0)
+    if (stages == 1) CL_LOGITS(1);
+    else if (stages == 2) CL_LOGITS(2);
+    else if (stages == 3) CL_LOGITS(3);
+    else if (stages == 4) CL_LOGITS(4);
+    else if (held) {
+        if constexpr (!is_f32<E>()) {
+            if (stages == 5) CL_LOGITS(5);
+            else if (stages == 6) CL_LOGITS(6);
+            else if (stages == 7) CL_LOGITS(7);
+            else CL_LOGITS(8);
+        }
+    } else if (mt == 2) hipLaunchKernelGGL((logits_tile_kernel<E, P, M, 2, 8>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a);
+    else hipLaunchKernelGGL((logits_tile_kernel<E, P, M, 1, 8>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a);
+#undef CL_LOGITS
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
+}
+
+// code.out or x.out null: that gradient is not wanted
+template <typename E>
+int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
+    constexpr int P = grad_parts<E>();
+    code.tiles_m = ceil_div(code.rows, 64 * t.mt);
+    code.tiles_n = ceil_div(code.cols, 16 * t.nt);
+    x.tiles_m = ceil_div(x.rows, 64 * t.mt);
+    x.tiles_n = code.tiles_n;
+    const long code_blocks = code.out ? (long)ceil_div(code.splits, 8) * 8 * code.tiles_m * code.tiles_n : 0;
+    const long grid = code_blocks + (x.out ? (long)ceil_div(x.tiles_m, 8) * 8 * x.tiles_n : 0);
+    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
+#define CL_GRADS(MT, NT) hipLaunchKernelGGL((grads_kernel<E, P, MT, NT>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x)
+    if (t.mt == 2) {
+        if (t.nt == 2) CL_GRADS(2, 2);
+        else if (t.nt == 4) CL_GRADS(2, 4);
+        else CL_GRADS(2, 8);
+    } else {
+        if (t.nt == 2) CL_GRADS(1, 2);
+        else if (t.nt == 4) CL_GRADS(1, 4);
+        else if (t.nt == 8) CL_GRADS(1, 8);
+        else CL_GRADS(1, 16);
+    }
+#undef CL_GRADS
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
 }
 
 int code_check(const char *what, int n, int d, int k, int dtype, float temperature) {
-    const std::string w(what);
-    GDPSO_REQUIRE(n >= 0 && k > 0 && d > 0, w + ": n >= 0, k > 0 and d > 0 are required");
-    GDPSO_REQUIRE(d <= CL_MAX_D, w + ": embedding size above 4096");
-    GDPSO_REQUIRE(k <= (1 << 20), w + ": more than 2^20 codes");
-    GDPSO_REQUIRE(dtype_ok(dtype), w + ": unknown element type");
-    GDPSO_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, w + ": temperature must lie in [1e-6, 1e6]");
+    using w = std::string;
+    GDPSO_REQUIRE(n >= 0 && k > 0 && d > 0, w(what) + ": n >= 0, k > 0 and d > 0 are required");
+    GDPSO_REQUIRE(d <= CL_MAX_D, w(what) + ": embedding size above 4096");
+    GDPSO_REQUIRE(k <= (1 << 20), w(what) + ": more than 2^20 codes");
+    GDPSO_REQUIRE(dtype_ok(dtype), w(what) + ": unknown element type");
+    GDPSO_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, w(what) + ": temperature must lie in [1e-6, 1e6]");
     return GDPSO_OK;
 }
 
@@ -436,14 +706,15 @@ extern "C" int gdpso_code_logits(void *stream_, int n, int d, int k, const void 
     if (rc) return rc;
     GDPSO_REQUIRE(n == 0 || (inputs && codebook && logits), "code_logits: null argument");
     if (n == 0) return GDPSO_OK;
-    ProductArgs a = {inputs, codebook, logits, n, k, d, d, d, 0, 0, 1, ceil_div(d, KT) * (long)KT, 1.f / temperature};
-    GDPSO_WITH_DTYPE(dtype, rc = logits_product<E>((hipStream_t)stream_, a));
+    const ProductArgs a = {inputs, codebook, logits, n, k, d, d, d, 0, 0, 1, ceil_div(d, KT) * (long)KT, 1.f / temperature, nullptr};
+    GDPSO_WITH_DTYPE(dtype, rc = launch_logits<E>((hipStream_t)stream_, a));
     return rc;
 }
 
 extern "C" size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k) {
     if (n <= 0 || d <= 0 || k <= 0) return 0;
-    return (size_t)code_splits(n, d, k) * k * (d + 1) * sizeof(float);
+    const int splits = code_splits(n, d, k);
+    return splits > 1 ? (size_t)splits * k * (d + 1) * sizeof(float) : 0;
 }
 
 extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const float *grad_logits, const void *inputs, const void *codebook, int dtype,
@@ -452,24 +723,21 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
     if (rc) return rc;
     GDPSO_REQUIRE(n == 0 || (grad_logits && inputs), "code_logits_grad: null argument");
     GDPSO_REQUIRE(codebook, "code_logits_grad: null argument");
-    GDPSO_REQUIRE(!grad_codebook || n == 0 || workspace, "code_logits_grad: null workspace");
-    if (grad_codebook && workspace_bytes < gdpso_code_logits_grad_workspace_bytes(n, d, k))
+    const size_t need = grad_codebook ? gdpso_code_logits_grad_workspace_bytes(n, d, k) : 0;
+    GDPSO_REQUIRE(need == 0 || workspace, "code_logits_grad: null workspace");
+    if (workspace_bytes < need)
         return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     const float scale = 2.f / temperature;
-    if (grad_inputs && n > 0) {
-        const ProductArgs a = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale};
-        GDPSO_WITH_DTYPE(dtype, rc = (launch_product<GRAD_X, float, E, 3, grad_parts<E>(), bf16_t, E>(stream, a)));
+    const int splits = code_splits(n, d, k);
+    if (n > 0 && (grad_inputs || grad_codebook)) {
+        const long per = ceil_div(ceil_div(n, splits), KT) * (long)KT;
+        const ProductArgs code = {grad_logits, inputs, splits > 1 && grad_codebook ? workspace : grad_codebook, k, d, n, k, d, 0, 0, splits, per, scale, codebook};
+        const ProductArgs x = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale, nullptr};
+        GDPSO_WITH_DTYPE(dtype, rc = launch_grads<E>(stream, code, x, grad_tile(n, d)));
         if (rc) return rc;
     }
-    if (grad_codebook) {
-        const int splits = code_splits(n, d, k);
-        if (splits) {
-            const long per = ceil_div(ceil_div(n, splits), KT) * (long)KT;
-            const ProductArgs a = {grad_logits, inputs, workspace, k, d, n, k, d, 0, 0, splits, per, 1.f};
-            GDPSO_WITH_DTYPE(dtype, rc = (launch_product<GRAD_CODE, float, E, 3, grad_parts<E>(), bf16_t, float>(stream, a)));
-            if (rc) return rc;
-        }
+    if (grad_codebook && splits != 1) {  // no rows: zeros
         GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E>), dim3(ceil_div((long)k * d, 64)), dim3(64 * JOIN_WAVES), 0, stream, d, k, splits,
                                                    (const float *)workspace, (const E *)codebook, scale, (E *)grad_codebook));
         GDPSO_HIP(hipGetLastError());

@@ -29,6 +29,10 @@ constexpr int SEG_THREADS = 256, SEG_NCH = 8;  // a segment: at most 8192 fp32 o
 constexpr int BITS = 1 << 16;
 constexpr float LN2 = 0.69314718f;
 
+// Where 1 / rows kept comes from: there is no mask, the stats hold it, or every workgroup counts the mask itself.
+enum Kept { KEPT_ALL, KEPT_READ, KEPT_COUNT };
+constexpr int COUNT_ROWS = 16384;  // rows up to which counting is cheaper than a launch for it: 64 mask bytes a thread
+
 struct DistArgs {
     int n, v, k;
     const void *logits;
@@ -42,8 +46,11 @@ struct DistArgs {
     float grad_scale;
     const float *upstream;
     float *stats;            // maximum and sum of every row, written with VALUE, read without
-    const float *inv_rows;   // 1 / rows kept, or null: inv_all
-    float inv_all;
+    float *inv_rows;         // 1 / rows kept, last of the stats: written by the kernel that finishes, or ahead of this one
+    float inv_all;           // the same where no mask leaves rows out
+    Kept kept;
+    unsigned *ticket;        // segments: cleared by their first launch, the last workgroup of the second finishes; else null
+    float *loss;
     float *row_loss;
     void *grad;
     double *loss_part;       // sums of row losses, one a workgroup (segments: one a row)
@@ -51,8 +58,45 @@ struct DistArgs {
     float2 *parts;           // [n][segs] maximum and sum of a segment; null: stats are read
 };
 
-__device__ __forceinline__ float grad_factor(const DistArgs &a) {
-    return (a.upstream ? *a.upstream : a.grad_scale) * a.temperature * (a.inv_rows ? *a.inv_rows : a.inv_all);
+__device__ __forceinline__ float inverse(long long rows) { return rows > 0 ? (float)(1. / (double)rows) : 0.f; }
+template <int THREADS>
+__device__ __forceinline__ float inv_kept(const DistArgs &a) {  // called by the whole workgroup
+    if (a.kept == KEPT_COUNT) return inverse(count_kept<THREADS>(a.mask, a.n));
+    return a.kept == KEPT_READ ? *a.inv_rows : a.inv_all;
+}
+__device__ __forceinline__ float grad_factor(const DistArgs &a, float inv) { return (a.upstream ? *a.upstream : a.grad_scale) * a.temperature * inv; }
+
+// The mean over the rows: thread 0's `sum` is workgroup `block` of `blocks`.  One workgroup finishes by itself; with a ticket the last
+// one adds all sums up in order; else a launch behind this one does (a ticket's release writes the L2's dirty lines back: with
+// thousands of workgroups behind a large gradient it took 70 us, the launch 3).
+template <int THREADS>
+__device__ __forceinline__ void finish_loss(const DistArgs &a, double sum, int block, int blocks, float inv) {
+    __shared__ double s_sum[THREADS / 64];
+    __shared__ bool s_last;
+    if (threadIdx.x == 0) {
+        s_last = false;
+        if (blocks == 1) {
+            *a.loss = (float)(sum * (double)inv);
+            if (a.kept != KEPT_READ) *a.inv_rows = inv;
+        } else if (a.ticket) {
+            __hip_atomic_store(&a.loss_part[block], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s_last = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)blocks - 1;
+        } else {
+            a.loss_part[block] = sum;
+        }
+    }
+    __syncthreads();
+    if (!s_last) return;
+    double s = 0.;
+    for (int b = threadIdx.x; b < blocks; b += THREADS) s += __hip_atomic_load(&a.loss_part[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < THREADS / 64; ++w) s += s_sum[w];
+        *a.loss = (float)(s * (double)inv);
+        if (a.kept != KEPT_READ) *a.inv_rows = inv;
+    }
 }
 // Entry j of row i: its column (-1: absent) and logit (-inf where absent).
 __device__ __forceinline__ void entry(const DistArgs &a, long long i, int j, int &c, float &t) {
@@ -69,8 +113,8 @@ __device__ __forceinline__ float row_loss_of(const DistArgs &a, float terms, flo
 
 // 1 / rows that the mask keeps
 __global__ __launch_bounds__(1024) void dist_kept_kernel(int n, const unsigned char *__restrict__ mask, float *__restrict__ inv_rows) {
-    const long long kept = count_kept<1024>(mask, n);
-    if (threadIdx.x == 0) *inv_rows = kept > 0 ? (float)(1. / (double)kept) : 0.f;
+    const float inv = inverse(count_kept<1024>(mask, n));
+    if (threadIdx.x == 0) *inv_rows = inv;
 }
 
 // ------------------------------------------------------------------------------------- rows of up to 2048 columns
@@ -80,9 +124,10 @@ __global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
     __shared__ unsigned s_bits[GRAD ? TEAMS : 1][GRAD ? WORDS : 1];
     __shared__ double s_loss[VALUE ? TEAMS : 1];
     const int lane = threadIdx.x & 63, pos = threadIdx.x & (TEAM - 1), team = threadIdx.x / TEAM;
+    const float inv = inv_kept<TEAM_THREADS>(a);
     float factor = 0.f;
     if constexpr (GRAD) {
-        factor = grad_factor(a);
+        factor = grad_factor(a, inv);
         for (int w = pos; w < WORDS; w += TEAM) s_bits[team][w] = 0;
     }
     double sum = 0.;
@@ -189,10 +234,9 @@ __global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
     if constexpr (VALUE) {
         if (pos == 0) s_loss[team] = sum;
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0)
             for (int w = 1; w < TEAMS; ++w) sum += s_loss[w];
-            a.loss_part[blockIdx.x] = sum;
-        }
+        finish_loss<TEAM_THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
     }
 }
 
@@ -251,9 +295,10 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
     __shared__ unsigned s_bits[GRAD ? BITS / 32 : 1];
     __shared__ int s_repeats;
     const int tid = threadIdx.x;
+    const float inv = inv_kept<THREADS>(a);
     float factor = 0.f;
     if constexpr (GRAD) {
-        factor = grad_factor(a);
+        factor = grad_factor(a, inv);
         for (int w = tid; w < BITS / 32; w += THREADS) s_bits[w] = 0;
     }
     double sum = 0.;
@@ -339,15 +384,23 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
             }
         }
     }
-    if (tid == 0) a.loss_part[blockIdx.x] = sum;
+    finish_loss<THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
 }
 
-// Maximum and sum of a segment.
+// Maximum and sum of a segment; one workgroup more counts the mask.
 template <typename E>
 __global__ __launch_bounds__(SEG_THREADS) void dist_part_kernel(DistArgs a) {
     __shared__ PairRed<SEG_THREADS> s_max, s_sum;
     const long long i = blockIdx.x / a.segs;
     const int seg = (int)(blockIdx.x - i * a.segs), lo = seg * a.seg, len = std::min(a.seg, a.v - lo);
+    if (i == a.n) {
+        const float inv = inverse(a.mask ? count_kept<SEG_THREADS>(a.mask, a.n) : a.n);
+        if (threadIdx.x == 0) {
+            *a.inv_rows = inv;
+            *a.ticket = 0;
+        }
+        return;
+    }
     if (a.mask && !a.mask[i]) return;
     RowRegs<E, SEG_THREADS, SEG_NCH> r;
     r.load((const E *)a.logits + i * a.row_stride + lo, len, threadIdx.x);
@@ -372,11 +425,13 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
     const E *row = (const E *)a.logits + i * a.row_stride;
     E *grow = (E *)a.grad + i * a.v;
     if (a.mask && !a.mask[i]) {
-        if (VALUE && seg == 0 && tid == 0) {
-            a.row_loss[i] = 0.f;
-            a.stats[2 * i] = 0.f;
-            a.stats[2 * i + 1] = 0.f;
-            a.loss_part[i] = 0.;
+        if (VALUE && seg == 0) {
+            if (tid == 0) {
+                a.row_loss[i] = 0.f;
+                a.stats[2 * i] = 0.f;
+                a.stats[2 * i + 1] = 0.f;
+            }
+            finish_loss<SEG_THREADS>(a, 0., (int)i, a.n, *a.inv_rows);
         }
         if constexpr (GRAD) RowRegs<E, SEG_THREADS, SEG_NCH>::store(grow + lo, len, tid, [](int, int) { return 0.f; });
         return;
@@ -427,8 +482,8 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
             if (atomicOr(&s_bits[(c & (BITS - 1)) >> 5], bit) & bit) s_repeats = 1;
         }
     }
+    const float inv = *a.inv_rows, factor = grad_factor(a, inv);
     if constexpr (GRAD) {
-        const float factor = grad_factor(a);
         RowRegs<E, SEG_THREADS, SEG_NCH>::store(grow + lo, len, tid, [&](int j, int v) { return empty ? 0.f : factor * (s.exp(r.at(j, v)) * inv_l); });
     }
     if (VALUE && seg == 0) {
@@ -436,17 +491,19 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
         if ((tid & 63) == 0) s_terms[tid >> 6] = terms;
     }
     __syncthreads();  // the segment's plain gradient, the bits and the terms are there
-    if (VALUE && seg == 0 && tid == 0) {
-        for (int w = 1; w < SEG_THREADS / 64; ++w) terms += s_terms[w];
-        const float loss = row_loss_of(a, terms, l, tl);
-        a.row_loss[i] = loss;
-        a.stats[2 * i] = m;
-        a.stats[2 * i + 1] = l;
-        a.loss_part[i] = loss;
+    if (VALUE && seg == 0) {
+        float loss = 0.f;
+        if (tid == 0) {
+            for (int w = 1; w < SEG_THREADS / 64; ++w) terms += s_terms[w];
+            loss = row_loss_of(a, terms, l, tl);
+            a.row_loss[i] = loss;
+            a.stats[2 * i] = m;
+            a.stats[2 * i + 1] = l;
+        }
+        finish_loss<SEG_THREADS>(a, loss, (int)i, a.n, inv);
     }
     if constexpr (GRAD) {
         if (empty) return;
-        const float factor = grad_factor(a);
         for (int j = tid; j < a.k; j += SEG_THREADS) {
             const int c = ent.c[j];
             if (c < lo || c >= lo + len) continue;
@@ -466,35 +523,32 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
     }
 }
 
-// loss = sum of the parts / rows kept, and 1 / rows kept for a later gradient.  kept: already there (a mask and a gradient).
-__global__ __launch_bounds__(1024) void dist_finish_kernel(int n, const unsigned char *__restrict__ mask, bool kept, int parts, const double *__restrict__ part,
-                                                           float *inv_rows, float *__restrict__ loss) {
+// The mean where neither one workgroup nor a ticket could finish it.
+__global__ __launch_bounds__(1024) void dist_finish_kernel(DistArgs a, int parts) {
     __shared__ double s_sum[16];
     double s = 0.;
-    for (int i = threadIdx.x; i < parts; i += 1024) s += part[i];
+    for (int i = threadIdx.x; i < parts; i += 1024) s += a.loss_part[i];
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = s;
-    long long rows = n;
-    if (mask && !kept) rows = count_kept<1024>(mask, n);
+    const float inv = inverse(a.mask ? count_kept<1024>(a.mask, a.n) : a.n);
     __syncthreads();
     if (threadIdx.x == 0) {
-        float inv = kept ? *inv_rows : (rows > 0 ? (float)(1. / (double)rows) : 0.f);
-        if (!kept) *inv_rows = inv;
         for (int w = 1; w < 16; ++w) s += s_sum[w];
-        *loss = (float)(s * (double)inv);
+        *a.loss = (float)(s * (double)inv);
+        *a.inv_rows = inv;
     }
 }
 
 int distill_check(const char *what, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits, int t_dtype,
                   const void *t_idx, int index_bytes, float temperature) {
-    const std::string w(what);
-    GDPSO_REQUIRE(n >= 0 && v > 0 && k > 0, w + ": n >= 0, v > 0 and k > 0 are required");
-    GDPSO_REQUIRE(k <= DIST_MAX_K, w + ": more than 1024 teacher logits a row");
-    GDPSO_REQUIRE(dtype_ok(dtype) && dtype_ok(t_dtype), w + ": unknown element type");
-    GDPSO_REQUIRE(index_bytes == 4 || index_bytes == 8, w + ": indices are 4 or 8 bytes");
-    GDPSO_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, w + ": temperature must lie in [1e-6, 1e6]");
-    GDPSO_REQUIRE(n == 0 || (logits && t_logits && t_idx), w + ": null argument");
-    GDPSO_REQUIRE(row_stride >= 0, w + ": negative row stride");
+    using w = std::string;
+    GDPSO_REQUIRE(n >= 0 && v > 0 && k > 0, w(what) + ": n >= 0, v > 0 and k > 0 are required");
+    GDPSO_REQUIRE(k <= DIST_MAX_K, w(what) + ": more than 1024 teacher logits a row");
+    GDPSO_REQUIRE(dtype_ok(dtype) && dtype_ok(t_dtype), w(what) + ": unknown element type");
+    GDPSO_REQUIRE(index_bytes == 4 || index_bytes == 8, w(what) + ": indices are 4 or 8 bytes");
+    GDPSO_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, w(what) + ": temperature must lie in [1e-6, 1e6]");
+    GDPSO_REQUIRE(n == 0 || (logits && t_logits && t_idx), w(what) + ": null argument");
+    GDPSO_REQUIRE(row_stride >= 0, w(what) + ": negative row stride");
     return GDPSO_OK;
 }
 
@@ -533,12 +587,19 @@ inline Plan plan_rows(int n, int v, int vec) {
 
 constexpr int DIST_BLOCKS = 2048;
 inline int dist_blocks(const Plan &p, int n) {
+    if (p.way == BY_SEGMENT) return n > 0 ? n : 1;
     const long rows = p.way == BY_TEAM ? TEAM_THREADS / p.team : 1;
     const long want = ((long)n + rows - 1) / rows;
+    // up to four rounds of rows one workgroup goes alone: that is less than the launch that would join several
+    if (p.way == BY_TEAM && want <= 4) return 1;
     return (int)(want < 1 ? 1 : std::min<long>(want, DIST_BLOCKS));
 }
-inline size_t parts_bytes(const Plan &p, int n) { return p.way == BY_SEGMENT ? (size_t)n * p.segs * sizeof(float2) : 0; }
-inline size_t loss_bytes(const Plan &p, int n) { return (size_t)(p.way == BY_SEGMENT ? (n > 0 ? n : 1) : dist_blocks(p, n)) * sizeof(double); }
+// Workspace: ticket, sums of row losses, segments
+constexpr size_t TICKET_BYTES = 16;
+inline size_t loss_bytes(const Plan &p, int n) { return ((size_t)dist_blocks(p, n) * sizeof(double) + 15) / 16 * 16; }
+inline size_t space_bytes(const Plan &p, int n) {
+    return TICKET_BYTES + loss_bytes(p, n) + (p.way == BY_SEGMENT ? (size_t)n * p.segs * sizeof(float2) : 0);
+}
 
 template <typename E, bool VALUE, bool GRAD>
 int launch_team(hipStream_t stream, const DistArgs &a, const Plan &p) {
@@ -573,8 +634,8 @@ int launch_distill(hipStream_t stream, const DistArgs &a, const Plan &p) {
         else hipLaunchKernelGGL((dist_row_kernel<E, 1024, 16, GRAD>), grid, dim3(1024), 0, stream, a);
     } else {
         const long blocks = (long)a.n * a.segs;
-        GDPSO_REQUIRE(blocks < (1l << 31), "distill: too many rows for one call");
-        if (VALUE) hipLaunchKernelGGL((dist_part_kernel<E>), dim3((unsigned)blocks), dim3(SEG_THREADS), 0, stream, a);
+        GDPSO_REQUIRE(blocks < (1l << 31) - 1, "distill: too many rows for one call");
+        if (VALUE) hipLaunchKernelGGL((dist_part_kernel<E>), dim3((unsigned)blocks + 1), dim3(SEG_THREADS), 0, stream, a);
         hipLaunchKernelGGL((dist_apply_kernel<E, VALUE, GRAD>), dim3((unsigned)(GRAD ? blocks : a.n)), dim3(SEG_THREADS), 0, stream, a);
     }
     GDPSO_HIP(hipGetLastError());
@@ -588,8 +649,7 @@ using namespace gdpso;
 
 extern "C" size_t gdpso_distill_workspace_bytes(int n, int v, int k) {
     if (n < 0 || v <= 0 || k <= 0) return 0;
-    const Plan a = plan_rows(n, v, 4), b = plan_rows(n, v, 8);
-    return std::max(parts_bytes(a, n) + loss_bytes(a, n), parts_bytes(b, n) + loss_bytes(b, n));
+    return std::max(space_bytes(plan_rows(n, v, 4), n), space_bytes(plan_rows(n, v, 8), n));  // whatever the type
 }
 
 extern "C" int gdpso_distill(void *stream_, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits, int t_dtype,
@@ -602,21 +662,25 @@ extern "C" int gdpso_distill(void *stream_, int n, int v, int k, const void *log
     hipStream_t stream = (hipStream_t)stream_;
     float *inv_rows = row_stats + 2 * (size_t)n;
     const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype));
-    double *loss_part = (double *)workspace;
-    float2 *parts = (float2 *)((char *)workspace + loss_bytes(p, n));
-    const bool kept = mask && grad && n > 0;
-    DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), grad_scale, nullptr,
-                  row_stats, kept ? inv_rows : nullptr, n > 0 ? (float)(1. / n) : 0.f, row_loss, grad, loss_part, p.seg, p.segs, parts};
-    if (kept) hipLaunchKernelGGL(dist_kept_kernel, dim3(1), dim3(1024), 0, stream, n, mask, inv_rows);
+    unsigned *ticket = (unsigned *)workspace;
+    double *loss_part = (double *)((char *)workspace + TICKET_BYTES);
+    float2 *parts = (float2 *)((char *)loss_part + loss_bytes(p, n));
+    const bool one = dist_blocks(p, n) == 1;
+    // the kept rows ahead of a gradient: by the workgroups themselves, by the segments' first launch, or by a launch of its own
+    const bool ahead = mask && n > COUNT_ROWS && p.way != BY_SEGMENT && (grad || one);
+    const Kept kept = p.way == BY_SEGMENT || ahead ? KEPT_READ : (mask && (grad || one) ? KEPT_COUNT : KEPT_ALL);
+    const DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), grad_scale,
+                        nullptr, row_stats, inv_rows, n > 0 ? (float)(1. / n) : 0.f, kept, p.way == BY_SEGMENT ? ticket : nullptr, loss, row_loss,
+                        grad, loss_part, p.seg, p.segs, parts};
     if (n > 0) {
+        if (ahead) hipLaunchKernelGGL(dist_kept_kernel, dim3(1), dim3(1024), 0, stream, n, mask, inv_rows);
         if (grad)
             GDPSO_WITH_DTYPE(dtype, rc = (launch_distill<E, true, true>(stream, a, p)));
         else
             GDPSO_WITH_DTYPE(dtype, rc = (launch_distill<E, true, false>(stream, a, p)));
         if (rc) return rc;
     }
-    const int count = n == 0 ? 0 : (p.way == BY_SEGMENT ? n : dist_blocks(p, n));
-    hipLaunchKernelGGL(dist_finish_kernel, dim3(1), dim3(1024), 0, stream, n, mask, kept, count, loss_part, inv_rows, loss);
+    if (n == 0 || (!one && !a.ticket)) hipLaunchKernelGGL(dist_finish_kernel, dim3(1), dim3(1024), 0, stream, a, n > 0 ? dist_blocks(p, n) : 0);
     GDPSO_HIP(hipGetLastError());
     return GDPSO_OK;
 }
@@ -630,7 +694,8 @@ extern "C" int gdpso_distill_grad(void *stream_, int n, int v, int k, const void
     if (n == 0) return GDPSO_OK;
     const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype));
     const DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), 0.f, upstream,
-                        (float *)row_stats, row_stats + 2 * (size_t)n, 0.f, nullptr, grad, nullptr, p.seg, p.segs, nullptr};
+                        (float *)row_stats, (float *)row_stats + 2 * (size_t)n, 0.f, KEPT_READ, nullptr, nullptr, nullptr, grad, nullptr, p.seg, p.segs,
+                        nullptr};
     GDPSO_WITH_DTYPE(dtype, rc = (launch_distill<E, false, true>((hipStream_t)stream_, a, p)));
     return rc;
 }

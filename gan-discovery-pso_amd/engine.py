@@ -367,108 +367,116 @@ def vq_seed_codebook(codebook: torch.Tensor, positions: torch.Tensor, row0: int 
 
 
 # -------------------------------------------------- soft code assignment and losses over it
-_LOGIT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_LOGIT_CODES = {torch.float32: _lib.DTYPES["f32"], torch.bfloat16: _lib.DTYPES["bf16"], torch.float16: _lib.DTYPES["f16"]}
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _cuda_device(t: torch.Tensor, **others):
+    """The device of ``t``, on which all the others (None aside) have to be."""
+    device = t.device
+    if device.type != "cuda":
+        _device_guard(device)
+    for name, other in others.items():
+        if other is not None and other.device != device:
+            raise ValueError(f"{name} is on {other.device}, expected {device}")
+    return device
 
 
-def _code_args(inputs: torch.Tensor, codebook: torch.Tensor):
-    device = _device_guard(codebook.device)
-    _same_device(device, inputs=inputs)
+def _matrix(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """[..., cols] as contiguous rows; a copy only where the strides need one."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
+    return t.detach().reshape(t.numel() // cols, cols).contiguous()
+
+
+def _code_args(inputs: torch.Tensor, codebook: torch.Tensor, **others):
+    device = _cuda_device(codebook, inputs=inputs, **others)
     if codebook.dim() != 2 or codebook.shape[0] == 0 or codebook.shape[1] == 0:
         raise ValueError("codebook must be [K, D]")
-    if inputs.dim() == 0 or inputs.shape[-1] != codebook.shape[1]:
-        raise ValueError(f"inputs must be [..., {codebook.shape[1]}], got {tuple(inputs.shape)}")
-    if inputs.dtype not in _LOGIT_TYPES or codebook.dtype != inputs.dtype:
+    k, d = codebook.shape
+    if inputs.dim() == 0 or inputs.shape[-1] != d:
+        raise ValueError(f"inputs must be [..., {d}], got {tuple(inputs.shape)}")
+    dtype = _LOGIT_CODES.get(inputs.dtype)
+    if dtype is None or codebook.dtype != inputs.dtype:
         raise ValueError(f"inputs and codebook must share one of float32, bfloat16, float16 (got {inputs.dtype} and {codebook.dtype})")
-    return device, inputs.detach().reshape(-1, inputs.shape[-1]).contiguous(), codebook.detach().contiguous()
+    return device, _matrix(inputs, d), _matrix(codebook, d), k, d, dtype
 
 
 def code_logits(inputs: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
     """Logits of the soft assignment of ``inputs`` [..., D] to the rows of ``codebook`` [K, D] (gdpso_code_logits):
     (2 <x, code> - |code|^2) / temperature, float32 [..., K], whatever the type of the inputs."""
-    device, x, cb = _code_args(inputs, codebook)
-    (n, d), k = x.shape, cb.shape[0]
-    out = torch.empty(n, k, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        check(_lib.lib().gdpso_code_logits(_lib.stream_handle(device), n, d, k, ptr(x), ptr(cb), _dtype_code(x.dtype), temperature, ptr(out)))
-    return out.reshape(*inputs.shape[:-1], k)
+    device, x, cb, k, d, dtype = _code_args(inputs, codebook)
+    out = torch.empty((*inputs.shape[:-1], k), dtype=torch.float32, device=device)
+    _lib.run(device, _lib.lib().gdpso_code_logits, x.shape[0], d, k, x.data_ptr(), cb.data_ptr(), dtype, temperature, out.data_ptr())
+    return out
 
 
 def code_logits_grad(grad_logits: torch.Tensor, inputs: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.0, want_inputs=True,
                      want_codebook=True):
     """Gradients of ``code_logits`` for ``grad_logits`` float32 [..., K] (gdpso_code_logits_grad): (gradient of the inputs or
     None, gradient of the codebook or None), in their type."""
-    device, x, cb = _code_args(inputs, codebook)
-    (n, d), k = x.shape, cb.shape[0]
-    _same_device(device, grad_logits=grad_logits)
+    device, x, cb, k, d, dtype = _code_args(inputs, codebook, grad_logits=grad_logits)
+    n = x.shape[0]
     if grad_logits.dtype != torch.float32 or grad_logits.shape != (*inputs.shape[:-1], k):
         raise ValueError(f"grad_logits must be float32 {(*inputs.shape[:-1], k)}, got {grad_logits.dtype} {tuple(grad_logits.shape)}")
-    g = grad_logits.detach().reshape(n, k).contiguous()
-    dx = torch.empty_like(x) if want_inputs else None
-    dcb = torch.empty_like(cb) if want_codebook else None
+    g = _matrix(grad_logits, k)
+    dx = torch.empty(inputs.shape, dtype=x.dtype, device=device) if want_inputs else None
+    dcb = torch.empty((k, d), dtype=x.dtype, device=device) if want_codebook else None
     L = _lib.lib()
-    with torch.cuda.device(device):
-        ws = torch.empty(L.gdpso_code_logits_grad_workspace_bytes(n, d, k), dtype=torch.uint8, device=device) if want_codebook else None
-        check(L.gdpso_code_logits_grad(_lib.stream_handle(device), n, d, k, ptr(g), ptr(x), ptr(cb), _dtype_code(x.dtype), temperature, ptr(dx), ptr(dcb),
-                                       ptr(ws), 0 if ws is None else ws.numel()))
-    return None if dx is None else dx.reshape(inputs.shape), dcb
+    size = L.gdpso_code_logits_grad_workspace_bytes(n, d, k) if want_codebook else 0
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _lib.run(device, L.gdpso_code_logits_grad, n, d, k, g.data_ptr(), x.data_ptr(), cb.data_ptr(), dtype, temperature, ptr(dx), ptr(dcb), ptr(ws), size)
+    return dx, dcb
 
 
-def _loss_rows(logits: torch.Tensor, mask):
-    """Rows [n, E] of ``logits`` [..., E] with consecutive columns (a view where the strides allow it) and the mask's bytes."""
-    device = _device_guard(logits.device)
-    if logits.dtype not in _LOGIT_TYPES:
+def _loss_rows(logits: torch.Tensor, mask, **others):
+    """Rows [n, E] of ``logits`` [..., E] with consecutive columns (a view where the strides allow it), their stride and type, and
+    the mask's bytes."""
+    device = _cuda_device(logits, mask=mask, **others)
+    dtype = _LOGIT_CODES.get(logits.dtype)
+    if dtype is None:
         raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError(f"logits must be [..., E] with E > 0, got {tuple(logits.shape)}")
-    e = logits.shape[-1]
-    rows = logits.detach().reshape(logits.numel() // e, e)
+    shape = logits.shape
+    if logits.dim() == 0 or shape[-1] == 0:
+        raise ValueError(f"logits must be [..., E] with E > 0, got {tuple(shape)}")
+    e = shape[-1]
+    rows = logits if logits.dim() == 2 else logits.detach().reshape(logits.numel() // e, e)
     if rows.stride(1) != 1 and e > 1:
-        rows = rows.contiguous()
+        rows = rows.detach().contiguous()
+    n = rows.shape[0]
+    stride = rows.stride(0) if n > 1 else e
     if mask is not None:
-        _same_device(device, mask=mask)
-        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape[:-1]:
-            raise ValueError(f"mask must be bool {tuple(logits.shape[:-1])}, got {mask.dtype} {tuple(mask.shape)}")
-        mask = mask.detach().reshape(-1).contiguous()
-    return device, rows, mask
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != shape[:-1]:
+            raise ValueError(f"mask must be bool {tuple(shape[:-1])}, got {mask.dtype} {tuple(mask.shape)}")
+        mask = mask.contiguous()
+    return device, rows, n, e, stride, dtype, mask
 
 
-def _row_indices(indices: torch.Tensor, lead, device, what):
-    """indices [..., k], or [...] for one a row -> contiguous [n, k]."""
-    _same_device(device, **{what: indices})
-    if indices.dtype not in (torch.int64, torch.int32):
+def _row_indices(indices: torch.Tensor, lead, n: int, what: str):
+    """indices [..., k], or [...] for one a row -> contiguous, k, bytes of an index."""
+    size = {torch.int64: 8, torch.int32: 4}.get(indices.dtype)
+    if size is None:
         raise ValueError(f"{what} must be int64 or int32, got {indices.dtype}")
-    if indices.shape == lead:
-        indices = indices.unsqueeze(-1)
-    if indices.shape[:-1] != lead or indices.shape[-1] == 0:
-        raise ValueError(f"{what} must be {(*lead, 'k')}, got {tuple(indices.shape)}")
-    return indices.detach().reshape(lead.numel(), indices.shape[-1]).contiguous()
-
-
-def _row_stride(rows):
-    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+    shape = indices.shape
+    k = 1 if shape == lead else (shape[-1] if shape[:-1] == lead else 0)
+    if k == 0:
+        raise ValueError(f"{what} must be {(*lead, 'k')}, got {tuple(shape)}")
+    return indices.contiguous(), k, size
 
 
 def _balance(logits, indices, mask, grad_scale):
-    device, rows, mask = _loss_rows(logits, mask)
-    n, e = rows.shape
-    idx = _row_indices(indices, logits.shape[:-1], device, "indices")
+    device, rows, n, e, stride, dtype, mask = _loss_rows(logits, mask, indices=indices)
+    idx, k, index_bytes = _row_indices(indices, logits.shape[:-1], n, "indices")
     loss = torch.empty((), dtype=torch.float32, device=device)
-    counts = torch.empty(e + 2, dtype=torch.int64, device=device)
+    counts = torch.empty(e, dtype=torch.int64, device=device)
     mean_prob = torch.empty(e, dtype=torch.float32, device=device)
-    grad = None if grad_scale is None else torch.empty(n, e, dtype=rows.dtype, device=device)
+    grad = None if grad_scale is None else torch.empty(logits.shape, dtype=logits.dtype, device=device)
     L = _lib.lib()
-    with torch.cuda.device(device):
-        ws = torch.empty(L.gdpso_balance_workspace_bytes(n, e), dtype=torch.uint8, device=device)
-        check(L.gdpso_balance(_lib.stream_handle(device), n, e, idx.shape[1], ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(idx),
-                              idx.element_size(), ptr(mask), 0.0 if grad_scale is None else grad_scale, ptr(loss), ptr(counts), ptr(mean_prob),
-                              ptr(grad), ptr(ws), ws.numel()))
-    return loss, counts, mean_prob, None if grad is None else grad.reshape(logits.shape)
+    size = L.gdpso_balance_workspace_bytes(n, e)
+    ws = torch.empty((size + 7) // 8 + 2, dtype=torch.int64, device=device)  # two totals, then the call's workspace
+    base = ws.data_ptr()
+    _lib.run(device, L.gdpso_balance, n, e, k, rows.data_ptr(), stride, dtype, idx.data_ptr(), index_bytes, ptr(mask),
+             0.0 if grad_scale is None else grad_scale, loss.data_ptr(), counts.data_ptr(), base, mean_prob.data_ptr(), ptr(grad), base + 16, size)
+    return loss, counts, mean_prob, grad, ws
 
 
 def balance(logits: torch.Tensor, indices: torch.Tensor, mask=None, grad_scale=None):
@@ -476,51 +484,46 @@ def balance(logits: torch.Tensor, indices: torch.Tensor, mask=None, grad_scale=N
     E * sum_c f[c] P[c], f the share of the choices that fell on c, P the mean softmax.  ``mask`` bool [...]: rows to leave
     out are False.  An index outside [0, E) is a choice that is not counted.  Returns (loss, choices per expert int64 [E], P
     float32 [E], gradient of ``grad_scale`` * loss by the logits, or None without a ``grad_scale``)."""
-    loss, counts, mean_prob, grad = _balance(logits, indices, mask, grad_scale)
-    return loss, counts[:-2], mean_prob, grad
+    return _balance(logits, indices, mask, grad_scale)[:4]
 
 
-def balance_grad(logits: torch.Tensor, counts: torch.Tensor, upstream: torch.Tensor, mask=None) -> torch.Tensor:
+def balance_grad(logits: torch.Tensor, counts: torch.Tensor, totals: torch.Tensor, upstream: torch.Tensor, mask=None) -> torch.Tensor:
     """Gradient of ``upstream`` (a float32 scalar on the device) * balance loss by the logits (gdpso_balance_grad); ``counts``
-    int64 [E + 2] as gdpso_balance leaves them: choices per expert, rows kept, choices counted."""
-    device, rows, mask = _loss_rows(logits, mask)
-    n, e = rows.shape
-    _same_device(device, counts=counts, upstream=upstream)
-    if counts.dtype != torch.int64 or counts.shape != (e + 2,) or not counts.is_contiguous():
-        raise ValueError(f"counts must be contiguous int64 [{e + 2}]")
+    int64 [E] and ``totals`` int64 [2] (rows kept, choices counted) as gdpso_balance leaves them."""
+    device, rows, n, e, stride, dtype, mask = _loss_rows(logits, mask, counts=counts, totals=totals, upstream=upstream)
+    for name, t, size in (("counts", counts, e), ("totals", totals, 2)):
+        if t.dtype != torch.int64 or t.shape != (size,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int64 [{size}]")
     if upstream.dtype != torch.float32 or upstream.numel() != 1:
         raise ValueError("upstream must be a float32 scalar")
-    grad = torch.empty(n, e, dtype=rows.dtype, device=device)
-    with torch.cuda.device(device):
-        check(_lib.lib().gdpso_balance_grad(_lib.stream_handle(device), n, e, ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(mask), ptr(counts),
-                                            ptr(upstream), ptr(grad)))
-    return grad.reshape(logits.shape)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    _lib.run(device, _lib.lib().gdpso_balance_grad, n, e, rows.data_ptr(), stride, dtype, ptr(mask), counts.data_ptr(), totals.data_ptr(),
+             upstream.data_ptr(), grad.data_ptr())
+    return grad
 
 
-def _distill_args(logits, teacher_logits, teacher_indices, mask):
-    device, rows, mask = _loss_rows(logits, mask)
-    idx = _row_indices(teacher_indices, logits.shape[:-1], device, "teacher_indices")
-    _same_device(device, teacher_logits=teacher_logits)
-    if teacher_logits.dtype not in _LOGIT_TYPES or teacher_logits.shape != teacher_indices.shape:
+def _distill_args(logits, teacher_logits, teacher_indices, mask, **others):
+    args = _loss_rows(logits, mask, teacher_logits=teacher_logits, teacher_indices=teacher_indices, **others)
+    idx, k, index_bytes = _row_indices(teacher_indices, logits.shape[:-1], args[2], "teacher_indices")
+    t_dtype = _LOGIT_CODES.get(teacher_logits.dtype)
+    if t_dtype is None or teacher_logits.shape != teacher_indices.shape:
         raise ValueError(f"teacher_logits must be floating point of the shape of teacher_indices {tuple(teacher_indices.shape)}, got "
                          f"{teacher_logits.dtype} {tuple(teacher_logits.shape)}")
-    return device, rows, mask, idx, teacher_logits.detach().reshape(idx.shape).contiguous()
+    return (*args, k, idx, index_bytes, teacher_logits.contiguous(), t_dtype)
 
 
 def _distill(logits, teacher_logits, teacher_indices, mask, temperature, grad_scale):
-    device, rows, mask, idx, t = _distill_args(logits, teacher_logits, teacher_indices, mask)
-    (n, v), k = rows.shape, idx.shape[1]
+    device, rows, n, v, stride, dtype, mask, k, idx, index_bytes, t, t_dtype = _distill_args(logits, teacher_logits, teacher_indices, mask)
     loss = torch.empty((), dtype=torch.float32, device=device)
-    row_loss = torch.empty(n, dtype=torch.float32, device=device)
+    row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
     stats = torch.empty(2 * n + 1, dtype=torch.float32, device=device)
-    grad = None if grad_scale is None else torch.empty(n, v, dtype=rows.dtype, device=device)
+    grad = None if grad_scale is None else torch.empty(logits.shape, dtype=logits.dtype, device=device)
     L = _lib.lib()
-    with torch.cuda.device(device):
-        ws = torch.empty(L.gdpso_distill_workspace_bytes(n, v, k), dtype=torch.uint8, device=device)
-        check(L.gdpso_distill(_lib.stream_handle(device), n, v, k, ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(t), _dtype_code(t.dtype),
-                              ptr(idx), idx.element_size(), ptr(mask), temperature, 0.0 if grad_scale is None else grad_scale, ptr(loss), ptr(row_loss),
-                              ptr(stats), ptr(grad), ptr(ws), ws.numel()))
-    return loss, row_loss.reshape(logits.shape[:-1]), None if grad is None else grad.reshape(logits.shape), stats
+    size = L.gdpso_distill_workspace_bytes(n, v, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    _lib.run(device, L.gdpso_distill, n, v, k, rows.data_ptr(), stride, dtype, t.data_ptr(), t_dtype, idx.data_ptr(), index_bytes, ptr(mask), temperature,
+             0.0 if grad_scale is None else grad_scale, loss.data_ptr(), row_loss.data_ptr(), stats.data_ptr(), ptr(grad), ws.data_ptr(), size)
+    return loss, row_loss, grad, stats
 
 
 def distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, mask=None, temperature: float = 1.0, grad_scale=None):
@@ -536,19 +539,16 @@ def distill_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
                  mask=None, temperature: float = 1.0) -> torch.Tensor:
     """Gradient of ``upstream`` (a float32 scalar on the device) * distillation loss by the logits (gdpso_distill_grad);
     ``row_stats`` float32 [2 n + 1] as gdpso_distill leaves them for the same logits and temperature."""
-    device, rows, mask, idx, t = _distill_args(logits, teacher_logits, teacher_indices, mask)
-    (n, v), k = rows.shape, idx.shape[1]
-    _same_device(device, row_stats=row_stats, upstream=upstream)
+    device, rows, n, v, stride, dtype, mask, k, idx, index_bytes, t, t_dtype = _distill_args(logits, teacher_logits, teacher_indices, mask,
+                                                                                             row_stats=row_stats, upstream=upstream)
     if row_stats.dtype != torch.float32 or row_stats.shape != (2 * n + 1,) or not row_stats.is_contiguous():
         raise ValueError(f"row_stats must be contiguous float32 [{2 * n + 1}]")
     if upstream.dtype != torch.float32 or upstream.numel() != 1:
         raise ValueError("upstream must be a float32 scalar")
-    grad = torch.empty(n, v, dtype=rows.dtype, device=device)
-    with torch.cuda.device(device):
-        check(_lib.lib().gdpso_distill_grad(_lib.stream_handle(device), n, v, k, ptr(rows), _row_stride(rows), _dtype_code(rows.dtype), ptr(t),
-                                            _dtype_code(t.dtype), ptr(idx), idx.element_size(), ptr(mask), temperature, ptr(row_stats), ptr(upstream),
-                                            ptr(grad)))
-    return grad.reshape(logits.shape)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    _lib.run(device, _lib.lib().gdpso_distill_grad, n, v, k, rows.data_ptr(), stride, dtype, t.data_ptr(), t_dtype, idx.data_ptr(), index_bytes, ptr(mask),
+             temperature, row_stats.data_ptr(), upstream.data_ptr(), grad.data_ptr())
+    return grad
 
 
 # -------------------------------------------------------------------- fitness settings

@@ -46,17 +46,16 @@ class _CodeLogits(torch.autograd.Function):
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, indices, mask):
-        loss, counts, mean_prob, _ = engine._balance(logits, indices, mask, None)
-        ctx.save_for_backward(logits, counts, mask)
-        per_expert = counts[:-2]
-        ctx.mark_non_differentiable(per_expert, mean_prob)
-        return loss, per_expert, mean_prob
+        loss, counts, mean_prob, _, ws = engine._balance(logits, indices, mask, None)
+        ctx.save_for_backward(logits, counts, ws[:2].clone(), mask)
+        ctx.mark_non_differentiable(counts, mean_prob)
+        return loss, counts, mean_prob
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _counts, _mean_prob):
-        logits, counts, mask = ctx.saved_tensors
-        return engine.balance_grad(logits, counts, grad, mask), None, None
+        logits, counts, totals, mask = ctx.saved_tensors
+        return engine.balance_grad(logits, counts, totals, grad, mask), None, None
 
 
 class _Distill(torch.autograd.Function):

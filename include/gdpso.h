@@ -386,16 +386,16 @@ int gdpso_code_logits_grad(void *stream, int n, int d, int k, const float *grad_
  * contiguous.  indices [n, k]: int64 (index_bytes 8) or int32 (4); one outside [0, e) is not counted (a dropped
  * choice).  mask [n] or NULL: rows whose byte is 0 are left out whatever they hold; their gradient is 0.  A kept row
  * without a finite logit has p = 0 (its choices count); NaN and +inf propagate.  No row kept, or no choice counted: loss 0.
- * Outputs: loss [1], counts int64 [e + 2] (choices per code, then the rows kept, then the choices counted), mean_prob
+ * Outputs: loss [1], counts int64 [e] (choices per code), totals int64 [2] (rows kept, choices counted), mean_prob
  * [e] = P, grad [n, e] in `dtype` or NULL.  1 <= e <= GDPSO_BALANCE_MAX_E.  n == 0 is allowed.
- * gdpso_balance_grad: the gradient alone from the counts of an earlier call, times the DEVICE scalar *upstream. */
+ * gdpso_balance_grad: the gradient alone from counts and totals of an earlier call, times the DEVICE scalar *upstream. */
 #define GDPSO_BALANCE_MAX_E 16384
 size_t gdpso_balance_workspace_bytes(int n, int e);
 int gdpso_balance(void *stream, int n, int e, int k, const void *logits, long long row_stride, int dtype, const void *indices,
-                  int index_bytes, const unsigned char *mask, float grad_scale, float *loss, long long *counts, float *mean_prob,
-                  void *grad, void *workspace, size_t workspace_bytes);
+                  int index_bytes, const unsigned char *mask, float grad_scale, float *loss, long long *counts, long long *totals,
+                  float *mean_prob, void *grad, void *workspace, size_t workspace_bytes);
 int gdpso_balance_grad(void *stream, int n, int e, const void *logits, long long row_stride, int dtype, const unsigned char *mask,
-                       const long long *counts, const float *upstream, void *grad);
+                       const long long *counts, const long long *totals, const float *upstream, void *grad);
 
 /* Distillation from a teacher's top logits: q_i = softmax of the row's k teacher logits / t, p_i = softmax of the student's
  * row of v logits / t,

@@ -25,7 +25,8 @@ def test_workspaces(h):
     assert h.gdpso_balance_workspace_bytes(-1, 4) == h.gdpso_balance_workspace_bytes(4, 0) == 0
     assert h.gdpso_balance_workspace_bytes(0, 4) > 0
     assert h.gdpso_code_logits_grad_workspace_bytes(0, 4, 4) == 0
-    assert h.gdpso_code_logits_grad_workspace_bytes(5, 3, 4) >= 4 * 4 * 4
+    assert h.gdpso_code_logits_grad_workspace_bytes(5, 3, 4) == 0  # one split needs none
+    assert h.gdpso_code_logits_grad_workspace_bytes(5000, 3, 4) >= 2 * 4 * 4 * 4
 
 
 def test_code_logits_refusals(h):
@@ -40,9 +41,9 @@ def test_code_logits_refusals(h):
                 dict(t=float("inf")), dict(x=None), dict(c=None), dict(out=None)):
         assert call(**bad) == ARG, bad
     assert call(n=0, x=None, out=None) == 0
-    ws = h.gdpso_code_logits_grad_workspace_bytes(4, 8, 3)
+    ws = h.gdpso_code_logits_grad_workspace_bytes(4000, 8, 3)
 
-    def grad(n=4, d=8, k=3, g=P, x=P, c=P, dt=0, t=1.0, dx=P, dc=P, w=P, wb=ws):
+    def grad(n=4000, d=8, k=3, g=P, x=P, c=P, dt=0, t=1.0, dx=P, dc=P, w=P, wb=ws):
         return h.gdpso_code_logits_grad(None, n, d, k, g, x, c, dt, t, dx, dc, w, wb)
 
     for bad in (dict(n=-1), dict(d=0), dict(k=0), dict(dt=-1), dict(t=0.0), dict(g=None), dict(x=None), dict(c=None), dict(w=None)):
@@ -54,17 +55,17 @@ def test_balance_refusals(h):
     P = 64
     ws = h.gdpso_balance_workspace_bytes(4, 8)
 
-    def call(n=4, e=8, k=2, s=P, stride=8, dt=0, i=P, ib=8, loss=P, counts=P, mean=P, w=P, wb=ws):
-        return h.gdpso_balance(None, n, e, k, s, stride, dt, i, ib, None, 1.0, loss, counts, mean, None, w, wb)
+    def call(n=4, e=8, k=2, s=P, stride=8, dt=0, i=P, ib=8, loss=P, counts=P, totals=P, mean=P, w=P, wb=ws):
+        return h.gdpso_balance(None, n, e, k, s, stride, dt, i, ib, None, 1.0, loss, counts, totals, mean, None, w, wb)
 
     for bad in (dict(n=-1), dict(e=0), dict(e=16385, wb=2 ** 40), dict(k=0), dict(s=None), dict(stride=-1), dict(dt=3), dict(i=None), dict(ib=2), dict(loss=None),
-                dict(counts=None), dict(mean=None), dict(w=None)):
+                dict(counts=None), dict(totals=None), dict(mean=None), dict(w=None)):
         assert call(**bad) == ARG, bad
     assert call(wb=ws - 1) == WORKSPACE
     for bad in ((-1, 8, P, 8, 0), (4, 0, P, 8, 0), (4, 8, None, 8, 0), (4, 8, P, -8, 0), (4, 8, P, 8, 7)):
-        assert h.gdpso_balance_grad(None, *bad, None, P, P, P) == ARG, bad
-    assert h.gdpso_balance_grad(None, 4, 8, P, 8, 0, None, P, None, P) == ARG
-    assert h.gdpso_balance_grad(None, 0, 8, None, 8, 0, None, None, None, None) == 0
+        assert h.gdpso_balance_grad(None, *bad, None, P, P, P, P) == ARG, bad
+    assert h.gdpso_balance_grad(None, 4, 8, P, 8, 0, None, P, P, None, P) == ARG
+    assert h.gdpso_balance_grad(None, 0, 8, None, 8, 0, None, None, None, None, None) == 0
 
 
 def test_distill_refusals(h):
@@ -100,10 +101,10 @@ def test_python_balance(eng):
         with pytest.raises(ValueError):
             eng.balance(a, b, mask=m)
     up = torch.ones(())
-    for counts, u in ((torch.zeros(8, dtype=torch.int64), up), (torch.zeros(10), up), (torch.zeros(10, dtype=torch.int64), up.double()),
-                      (torch.zeros(10, dtype=torch.int64), torch.ones(2))):
+    ok, two = torch.zeros(8, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)
+    for counts, totals, u in ((ok[:7], two, up), (ok.float(), two, up), (ok, ok, up), (ok, two, up.double()), (ok, two, torch.ones(2))):
         with pytest.raises(ValueError):
-            eng.balance_grad(s, counts, u)
+            eng.balance_grad(s, counts, totals, u)
 
 
 def test_python_distill(eng):
