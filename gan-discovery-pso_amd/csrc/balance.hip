@@ -26,10 +26,10 @@ constexpr int JOIN_COLS = 16, JOIN_GROUPS = 64;
 constexpr int HIST_MAX = 64;
 constexpr int OWN_CHOICES = 4096;  // choices that every workgroup of the gradient counts for itself (16 a thread)
 
-// Counting workgroups: sixteen choices a thread keep the loads of a thread in flight together; the partial counts are
-// read again by every workgroup of the gradient, so there are at most 64 of them.
+// Counting workgroups: eight choices a thread; the partial counts are read again by every workgroup of the gradient, so there
+// are at most 64 of them.
 inline int hist_blocks(long long choices, int threads) {
-    const long long h = (choices + threads * 16 - 1) / (threads * 16);
+    const long long h = (choices + threads * 8 - 1) / (threads * 8);
     return h < 1 ? 1 : (h > HIST_MAX ? HIST_MAX : (int)h);
 }
 
@@ -54,12 +54,14 @@ __device__ void count_choices(const Choices &a, int block, int blocks, unsigned 
     unsigned rows = 0, counted = 0;
     const long long step = (long long)blocks * threads, first = (long long)block * threads + threadIdx.x;
     if (a.mask) {
+#pragma unroll 4
         for (long long i = first; i < a.n; i += step) {
-            if (!a.mask[i]) continue;
-            ++rows;
+            const bool keep = a.mask[i] != 0;
+            rows += keep;
+#pragma unroll 2
             for (int j = 0; j < a.k; ++j) {
                 const long long c = load_index(a.idx, a.index_bytes, i * a.k + j);
-                if (c >= 0 && c < a.e) {
+                if (keep && c >= 0 && c < a.e) {
                     ++counted;
                     atomicAdd(&mine[c], 1u);
                 }
@@ -125,26 +127,22 @@ struct BalArgs {
     bool own_counts;
 };
 
+// Sum of a column of the partial counts, several loads under way at a time.
+__device__ __forceinline__ unsigned sum_counts(const unsigned *__restrict__ part, int blocks, int stride) {
+    unsigned s = 0;
+#pragma unroll 16
+    for (int h = 0; h < blocks; ++h) s += part[(size_t)h * stride];
+    return s;
+}
 // f into LDS and the gradient's factor grad_scale * e / rows (0 when no row is kept).
 __device__ __forceinline__ float shares(const BalArgs &a, float *s_f, int threads) {
-    long long rows = 0, counted = 0;
-    if (a.counts) {
-        rows = a.totals[0];
-        counted = a.totals[1];
-    } else {
-        for (int h = 0; h < a.count_blocks; ++h) {
-            rows += a.count_part[(size_t)h * (a.e + 2) + a.e];
-            counted += a.count_part[(size_t)h * (a.e + 2) + a.e + 1];
-        }
-    }
+    __shared__ long long s_total[2];
+    if (threadIdx.x < 2) s_total[threadIdx.x] = a.counts ? a.totals[threadIdx.x] : sum_counts(a.count_part + a.e + threadIdx.x, a.count_blocks, a.e + 2);
+    for (int c = threadIdx.x; c < a.e; c += threads) s_f[c] = a.counts ? (float)a.counts[c] : (float)sum_counts(a.count_part + c, a.count_blocks, a.e + 2);
+    __syncthreads();
+    const long long rows = s_total[0], counted = s_total[1];
     const float inv = counted > 0 ? (float)(1. / (double)counted) : 0.f;
-    for (int c = threadIdx.x; c < a.e; c += threads) {
-        long long s = 0;
-        if (a.counts) s = a.counts[c];
-        else
-            for (int h = 0; h < a.count_blocks; ++h) s += a.count_part[(size_t)h * (a.e + 2) + c];
-        s_f[c] = (float)s * inv;
-    }
+    for (int c = threadIdx.x; c < a.e; c += threads) s_f[c] *= inv;
     __syncthreads();
     const float g = a.upstream ? *a.upstream : a.grad_scale;
     return rows > 0 ? g * (float)a.e / (float)rows : 0.f;
@@ -169,6 +167,7 @@ __global__ __launch_bounds__(TEAM_THREADS) void bal_team_kernel(BalArgs a, Choic
             unsigned *s_hist = (unsigned *)s_mem;
             count_choices(ch, 0, 1, s_hist, s_total, TEAM_THREADS);
             if (blockIdx.x == 0) write_counts(ch, 0, s_hist, s_total, TEAM_THREADS);
+            __syncthreads();  // from here on the counters' memory holds f
             const float inv = s_total[1] > 0 ? (float)(1. / (double)s_total[1]) : 0.f;
             for (int c = threadIdx.x; c < a.e; c += TEAM_THREADS) s_mem[c] = (float)s_hist[c] * inv;
             factor = s_total[0] > 0 ? a.grad_scale * (float)a.e / (float)s_total[0] : 0.f;
@@ -199,7 +198,7 @@ __global__ __launch_bounds__(TEAM_THREADS) void bal_team_kernel(BalArgs a, Choic
         RowRegs<E, TEAM, NCH> row;
         row.load(logits + i * a.row_stride, a.e, pos);
         const bool keep = !a.mask || a.mask[i] != 0;
-        const Shift s(c2, team_max<TEAM>(row.max()));
+        const Shift s(c2, team_max<TEAM>(row.max(a.e)));
         float ex[NCH][VEC], l = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
@@ -285,7 +284,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void bal_wide_kernel(BalArgs a) {
         RowRegs<E, WIDE_THREADS, NCH> row;
         row.load(logits + i * a.row_stride, a.e, pos);
         const bool keep = !a.mask || a.mask[i] != 0;
-        const Shift s(1.44269504f, wide_reduce(row.max(), s_red, true));
+        const Shift s(1.44269504f, wide_reduce(row.max(a.e), s_red, true));
         float ex[NCH][VEC], l = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
@@ -333,44 +332,54 @@ __global__ __launch_bounds__(JOIN_COLS *JOIN_GROUPS) void bal_join_kernel(int e,
                                                                          long long *__restrict__ counts, long long *__restrict__ totals, double *dots,
                                                                          unsigned *ticket,
                                                                          float *__restrict__ loss) {
-    __shared__ double s_col[JOIN_GROUPS][JOIN_COLS];
-    __shared__ unsigned s_cnt[JOIN_GROUPS][JOIN_COLS];
+    __shared__ double s_col[JOIN_COLS * JOIN_GROUPS / 64][JOIN_COLS];
+    __shared__ unsigned s_cnt[JOIN_COLS * JOIN_GROUPS / 64][JOIN_COLS];
     __shared__ long long s_total[2];
     __shared__ bool s_last;
-    const int col = threadIdx.x % JOIN_COLS, grp = threadIdx.x / JOIN_COLS;
+    const int col = threadIdx.x % JOIN_COLS, grp = threadIdx.x / JOIN_COLS, wave = threadIdx.x >> 6;
     const int c = blockIdx.x * JOIN_COLS + col;
     double s = 0.;
     unsigned cnt = 0;
     if (c < e) {
+        if (grp < count_blocks) cnt = count_part[(size_t)grp * (e + 2) + c];
 #pragma unroll 8
         for (int g = grp; g < row_blocks; g += JOIN_GROUPS) s += (double)col_part[(size_t)g * e + c];
-        if (grp < count_blocks) cnt = count_part[(size_t)grp * (e + 2) + c];
     }
-    s_col[grp][col] = s;
-    s_cnt[grp][col] = cnt;
-    if (threadIdx.x < 64) {
+    if (wave == 0) {
+        const int lane = threadIdx.x;
         long long rows = 0, counted = 0;
-        if ((int)threadIdx.x < count_blocks) {
-            rows = count_part[(size_t)threadIdx.x * (e + 2) + e];
-            counted = count_part[(size_t)threadIdx.x * (e + 2) + e + 1];
+        if (lane < count_blocks) {
+            rows = count_part[(size_t)lane * (e + 2) + e];
+            counted = count_part[(size_t)lane * (e + 2) + e + 1];
         }
         for (int o = 32; o > 0; o >>= 1) {
             rows += __shfl_xor(rows, o, 64);
             counted += __shfl_xor(counted, o, 64);
         }
-        if (threadIdx.x == 0) {
+        if (lane == 0) {
             s_total[0] = rows;
             s_total[1] = counted;
         }
     }
+    // a wave's four groups, then the waves, in order
+    for (int o = JOIN_COLS; o < 64; o <<= 1) {
+        s += __shfl_xor(s, o, 64);
+        cnt += __shfl_xor(cnt, o, 64);
+    }
+    if ((threadIdx.x & 63) < JOIN_COLS) {
+        s_col[wave][col] = s;
+        s_cnt[wave][col] = cnt;
+    }
     __syncthreads();
-    // 64 partial results a column: sixteen columns to sixteen lanes of one wave
     double dot = 0.;
     if (threadIdx.x < JOIN_COLS) {
         long long total = 0;
-        for (int g = 0; g < count_blocks; ++g) total += s_cnt[g][col];
         s = 0.;
-        for (int g = 0; g < JOIN_GROUPS; ++g) s += s_col[g][col];
+#pragma unroll
+        for (int w = 0; w < JOIN_COLS * JOIN_GROUPS / 64; ++w) {
+            s += s_col[w][col];
+            total += s_cnt[w][col];
+        }
         if (c < e) {
             const double mean = s_total[0] > 0 ? s / (double)s_total[0] : 0.;
             mean_prob[c] = (float)mean;
@@ -503,7 +512,7 @@ extern "C" int gdpso_balance(void *stream_, int n, int e, int k, const void *log
     int rc = balance_check("balance", n, e, logits, row_stride, dtype);
     if (rc) return rc;
     GDPSO_REQUIRE(k > 0, "balance: k > 0 is required");
-    GDPSO_REQUIRE((long long)n * k < (1ll << 37), "balance: too many choices for one call");
+    GDPSO_REQUIRE((long long)n * k < (1ll << 32), "balance: 2^32 choices or more in one call");
     GDPSO_REQUIRE(index_bytes == 4 || index_bytes == 8, "balance: indices are 4 or 8 bytes");
     GDPSO_REQUIRE((n == 0 || indices) && loss && counts && totals && mean_prob && workspace, "balance: null argument");
     if (workspace_bytes < gdpso_balance_workspace_bytes(n, e)) return fail(GDPSO_ERR_WORKSPACE, "balance: workspace too small");

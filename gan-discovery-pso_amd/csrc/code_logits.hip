@@ -288,13 +288,8 @@ __device__ __forceinline__ void put4(EO *row, long n, long cols, const float (&x
             if (n + e < cols) row[n + e] = r[e];
 }
 
-// One workgroup's tile of 64 MT x 16 NT outputs: each wave 16 MT rows of it and all its columns.  depth() stages of both
-// operands are on the way while one multiplies: a stage's matrix instructions take less time than memory to answer, the
-// more so in the small tiles that small products take.
-template <int NT>
-constexpr int depth() {
-    return NT == 2 ? 4 : 2;
-}
+// One workgroup's tile of 64 MT x 16 NT outputs: each wave 16 MT rows of it and all its columns.  Two stages of both
+// operands are on the way while one multiplies: a stage's matrix instructions take less time than memory to answer.
 template <Product OP, typename EM, typename EN, int PM, int PN, typename M, int MT, int NT, typename EO>
 __device__ __forceinline__ void product_tile(const ProductArgs &a, const int block, char *lds) {
     constexpr bool KC_M = OP != GRAD_CODE, KC_N = OP == LOGITS;
@@ -324,7 +319,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
     const int fr = lane & 15, fk = (lane >> 4) * 8;  // this lane's row and first summed element of a fragment
 
-    constexpr int DEPTH = depth<NT>();
+    constexpr int DEPTH = 2;
     OpM om[DEPTH];
     OpN on[DEPTH];
     float sq[OpN::NU] = {}, sum_m[MT] = {};
@@ -394,12 +389,6 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
             step(std::integral_constant<int, 0>{}, s);
             if (s + 1 >= stages) break;
             step(std::integral_constant<int, 1>{}, s + 1);
-            if constexpr (DEPTH == 4) {
-                if (s + 2 >= stages) break;
-                step(std::integral_constant<int, 2>{}, s + 2);
-                if (s + 3 >= stages) break;
-                step(std::integral_constant<int, 3>{}, s + 3);
-            }
         }
     }
     const long done = k0 + (long)stages * KT;
@@ -558,6 +547,112 @@ __global__ __launch_bounds__(CL_THREADS) void logits_kernel(ProductArgs a) {
     }
 }
 
+// A tile of 16 x 32 outputs of a small product, whose time is the length of its sum: the four waves take every fourth stage each,
+// with both operands straight from memory and no barrier, and add up in LDS at the end.
+constexpr int SMALL_NT = 2;
+template <Product OP, typename E, int P>
+__device__ __forceinline__ void small_tile(const ProductArgs &a, const int block, f32x4 (&s_acc)[4][SMALL_NT][64], float (&s_sum)[4][16]) {
+    constexpr bool KC_M = OP == GRAD_X;
+    constexpr int WAVES = CL_THREADS / 64, DEPTH = 2;
+    using OpM = RowsOperand<float, KC_M, 1, 3, bf16_t>;
+    using OpN = RowsOperand<E, false, SMALL_NT, P, bf16_t>;  // columns as rows: a lane holds two neighbouring ones
+    const int tm = block % a.tiles_m, rest = block / a.tiles_m, tn = rest % a.tiles_n, split = rest / a.tiles_n;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long m0 = (long)tm * 16, n0 = (long)tn * (16 * SMALL_NT);
+    const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
+    const int fr = lane & 15, fk = (lane >> 4) * 8;
+    const bool pairs_n = a.cols % SMALL_NT == 0;
+    unsigned off_m[1], off_n[SMALL_NT];
+    OpM::offsets(a.ld_m, m0, a.rows, fr, fk, true, off_m);
+    OpN::offsets(a.ld_n, n0, a.cols, fr, fk, pairs_n, off_n);
+    const float *const pm = (const float *)a.m + OpM::first_row(m0, a.rows, true) * (KC_M ? a.ld_m : 1);
+    const E *const pn = (const E *)a.n + OpN::first_row(n0, a.cols, pairs_n);
+    float sum_m = 0.f;
+    f32x4 acc[SMALL_NT] = {};
+    const auto multiply = [&](const OpM &m, const OpN &n) {
+        Frag<bf16_t> fm[3], fn[SMALL_NT][P];
+        if constexpr (OP == GRAD_CODE)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum_m += m.v[0][e];
+        cut<3, bf16_t>(m.v[0], fm);
+#pragma unroll
+        for (int j = 0; j < SMALL_NT; ++j) cut<P, bf16_t>(n.v[j], fn[j]);
+#pragma unroll
+        for (int order = 2; order >= 0; --order)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const int q = order - p;
+                if (q < 0 || q >= P) continue;
+#pragma unroll
+                for (int j = 0; j < SMALL_NT; ++j) acc[j] = mfma(fn[j][q], fm[p], acc[j]);
+            }
+    };
+    const int whole = (int)((kend - k0) / KT), mine = whole > wave ? (whole - wave + WAVES - 1) / WAVES : 0;  // whole stages, this wave's
+    const auto load = [&](OpM &m, OpN &n, int t) {
+        const long k = k0 + (long)(wave + min(t, mine - 1) * WAVES) * KT;
+        m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m, true);
+        n.load_whole(pn + k * a.ld_n, a.ld_n, off_n, pairs_n);
+    };
+    OpM om[DEPTH];
+    OpN on[DEPTH];
+    if (mine > 0) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) load(om[i], on[i], i);
+        for (int t = 0; t < mine; t += DEPTH) {
+            multiply(om[0], on[0]);
+            if (t + 1 >= mine) break;
+            load(om[0], on[0], t + 2);
+            multiply(om[1], on[1]);
+            load(om[1], on[1], t + 3);
+        }
+    }
+    const long done = k0 + (long)whole * KT;
+    if (done < kend && wave == whole % WAVES) {  // what is left of the sum
+        om[0].load_part(pm + (KC_M ? done : done * a.ld_m), a.ld_m, off_m, fk, (int)(kend - done));
+        on[0].load_part(pn + done * a.ld_n, a.ld_n, off_n, fk, (int)(kend - done));
+        multiply(om[0], on[0]);
+    }
+    if constexpr (OP == GRAD_CODE) {
+        sum_m += __shfl_xor(sum_m, 16, 64);
+        sum_m += __shfl_xor(sum_m, 32, 64);
+        if (lane < 16) s_sum[wave][lane] = sum_m;
+    }
+#pragma unroll
+    for (int j = 0; j < SMALL_NT; ++j) s_acc[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int j = 0; j < SMALL_NT; ++j) acc[j] = (s_acc[0][j][lane] + s_acc[1][j][lane]) + (s_acc[2][j][lane] + s_acc[3][j][lane]);
+    const long m = m0 + fr;
+    if (m >= a.rows) return;
+    if constexpr (OP == GRAD_CODE) sum_m = (s_sum[0][fr] + s_sum[1][fr]) + (s_sum[2][fr] + s_sum[3][fr]);
+    const bool part = OP == GRAD_CODE && a.splits > 1;
+    float *partial = (float *)a.out + split * (a.rows * a.cols + a.rows);
+    if (part && tn == 0 && lane < 16) partial[a.rows * a.cols + m] = sum_m;
+    // columns n0 + fr' * 2 + j for fr' = 4 (lane / 16) + e: eight neighbours a lane
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const long n = n0 + (lane >> 4) * 8 + h * 4;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = acc[e & 1][h * 2 + (e >> 1)];
+            if constexpr (OP == GRAD_X) x[e] *= a.scale;
+            if constexpr (OP == GRAD_CODE)
+                if (!part && n + e < a.cols) x[e] = a.scale * fmaf(-sum_m, (float)((const E *)a.code)[m * a.cols + n + e], x[e]);
+        }
+        if (part) put4(partial + m * a.cols, n, a.cols, x);
+        else put4((E *)a.out + m * a.cols, n, a.cols, x);
+    }
+}
+template <typename E, int P>
+__global__ __launch_bounds__(CL_THREADS) void grads_small_kernel(ProductArgs code, int code_blocks, ProductArgs x) {
+    __shared__ f32x4 s_acc[4][SMALL_NT][64];
+    __shared__ float s_sum[4][16];
+    if ((int)blockIdx.x < code_blocks) small_tile<GRAD_CODE, E, P>(code, blockIdx.x, s_acc, s_sum);
+    else small_tile<GRAD_X, E, P>(x, blockIdx.x - code_blocks, s_acc, s_sum);
+}
+
 // Both gradients in one launch, the codebook's workgroups first (they run longer).
 template <typename E, int P, int MT, int NT>
 __global__ __launch_bounds__(CL_THREADS, 2) void grads_kernel(ProductArgs code, int code_blocks, ProductArgs x) {
@@ -567,8 +662,7 @@ __global__ __launch_bounds__(CL_THREADS, 2) void grads_kernel(ProductArgs code, 
 }
 
 // Joins the splits' partial sums in a fixed order: 64 neighbouring elements a workgroup, the splits dealt to its waves.
-constexpr int JOIN_WAVES = 8;
-template <typename E>
+template <typename E, int JOIN_WAVES>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void code_join_kernel(int d, int k, int splits, const float *__restrict__ part, const E *__restrict__ cb,
                                                                     float scale, E *__restrict__ dcode) {
     __shared__ float s_acc[JOIN_WAVES][64], s_sum[JOIN_WAVES][64];
@@ -577,7 +671,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void code_join_kernel(int d, int k
     float acc = 0.f, sum = 0.f;
     if (e < size) {
         const float *p = part + e, *ps = part + size + e / d;
-#pragma unroll 4
+#pragma unroll 8
         for (int s = wave; s < splits; s += JOIN_WAVES) {
             acc += p[s * (size + k)];
             sum += ps[s * (size + k)];
@@ -600,22 +694,23 @@ constexpr int grad_parts() {
     return is_f32<E>() ? 3 : (__is_same(E, f16_t) ? 2 : 1);
 }
 
-// Gradient tiles of 64 MT rows by 16 NT columns.  All d columns in one tile up to 256 (the rows' operand, the large one, is
-// then read and cut once); with few rows tiles of 32 columns, so that more CUs share them.
+// Gradient tiles of 64 MT rows by 16 NT columns, all d columns in one tile up to 256: the rows' operand, the large one, is then
+// read and cut once.  {0, 0}: the small form.
+constexpr int SMALL_ROWS = 4096;
 struct Tile {
     int mt, nt;
 };
 inline Tile grad_tile(int n, int d) {
-    if (n <= 4096) return {1, 2};
+    if (n <= SMALL_ROWS) return {0, 0};
     const int nt = d <= 32 ? 2 : (d <= 64 ? 4 : (d <= 128 ? 8 : 16));
     // 128 rows a workgroup once they fill the chip; 256 columns leave registers for 64
     return {nt < 16 && n >= 32768 ? 2 : 1, nt};
 }
-// Splits of the summed rows of the codebook's gradient: about two workgroups a CU, at least 128 rows each (the partial
-// sums that a split writes and the join reads have to stay small beside its rows).  Up to 512 rows one split does without
-// the join's launch.
+// Splits of the summed rows of the codebook's gradient.  Small: 512 rows, four stages a wave, and up to there one split does
+// without the join's launch.  Else about two workgroups a CU, at least 128 rows each (the partial sums that a split writes
+// and the join reads have to stay small beside its rows).
 inline int code_splits(int n, int d, int k) {
-    if (n <= 512) return n > 0 ? 1 : 0;
+    if (n <= SMALL_ROWS) return ceil_div(n, 512);
     const Tile t = grad_tile(n, d);
     const long tiles = (long)ceil_div(k, 64 * t.mt) * ceil_div(d, 16 * t.nt);
     const long want = ceil_div(512, tiles), most = ceil_div(n, 128);
@@ -662,6 +757,17 @@ int launch_logits(hipStream_t stream, ProductArgs a) {
 template <typename E>
 int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
     constexpr int P = grad_parts<E>();
+    if (t.mt == 0) {
+        code.tiles_m = ceil_div(code.rows, 16);
+        x.tiles_m = ceil_div(x.rows, 16);
+        code.tiles_n = x.tiles_n = ceil_div(x.cols, 16 * SMALL_NT);
+        const long code_blocks = code.out ? (long)code.splits * code.tiles_m * code.tiles_n : 0;
+        const long grid = code_blocks + (x.out ? (long)x.tiles_m * x.tiles_n : 0);
+        GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many codes for one call");
+        hipLaunchKernelGGL((grads_small_kernel<E, P>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x);
+        GDPSO_HIP(hipGetLastError());
+        return GDPSO_OK;
+    }
     code.tiles_m = ceil_div(code.rows, 64 * t.mt);
     code.tiles_n = ceil_div(code.cols, 16 * t.nt);
     x.tiles_m = ceil_div(x.rows, 64 * t.mt);
@@ -738,8 +844,13 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
         if (rc) return rc;
     }
     if (grad_codebook && splits != 1) {  // no rows: zeros
-        GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E>), dim3(ceil_div((long)k * d, 64)), dim3(64 * JOIN_WAVES), 0, stream, d, k, splits,
-                                                   (const float *)workspace, (const E *)codebook, scale, (E *)grad_codebook));
+        const dim3 grid(ceil_div((long)k * d, 64));
+        if (splits > 64)  // many splits of few elements: more waves a workgroup
+            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 16>), grid, dim3(64 * 16), 0, stream, d, k, splits, (const float *)workspace,
+                                                       (const E *)codebook, scale, (E *)grad_codebook));
+        else
+            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 4>), grid, dim3(64 * 4), 0, stream, d, k, splits, (const float *)workspace,
+                                                       (const E *)codebook, scale, (E *)grad_codebook));
         GDPSO_HIP(hipGetLastError());
     }
     return GDPSO_OK;

@@ -118,13 +118,13 @@ __global__ __launch_bounds__(1024) void dist_kept_kernel(int n, const unsigned c
 }
 
 // ------------------------------------------------------------------------------------- rows of up to 2048 columns
-template <typename E, int TEAM, int NCH, bool VALUE, bool GRAD>
-__global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
-    constexpr int VEC = vec_of<E>(), TEAMS = TEAM_THREADS / TEAM, WORDS = (TEAM * NCH * VEC + 31) / 32;
+template <typename E, int THREADS, int TEAM, int NCH, bool VALUE, bool GRAD>
+__global__ __launch_bounds__(THREADS) void dist_team_kernel(DistArgs a) {
+    constexpr int VEC = vec_of<E>(), TEAMS = THREADS / TEAM, WORDS = (TEAM * NCH * VEC + 31) / 32;
     __shared__ unsigned s_bits[GRAD ? TEAMS : 1][GRAD ? WORDS : 1];
     __shared__ double s_loss[VALUE ? TEAMS : 1];
     const int lane = threadIdx.x & 63, pos = threadIdx.x & (TEAM - 1), team = threadIdx.x / TEAM;
-    const float inv = inv_kept<TEAM_THREADS>(a);
+    const float inv = inv_kept<THREADS>(a);
     float factor = 0.f;
     if constexpr (GRAD) {
         factor = grad_factor(a, inv);
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
                 a.stats[2 * i] = 0.f;
                 a.stats[2 * i + 1] = 0.f;
             }
-            if constexpr (GRAD) RowRegs<E, TEAM, NCH>::store(grow, a.v, pos, [](int, int) { return 0.f; });
+            if constexpr (GRAD) RowRegs<E, TEAM, NCH>::clear(grow, a.v, pos);
             continue;
         }
         RowRegs<E, TEAM, NCH> r;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
             }
         };
         float m, l;
-        if constexpr (VALUE) m = team_max<TEAM>(r.max());
+        if constexpr (VALUE) m = team_max<TEAM>(r.max(a.v));
         else {
             m = a.stats[2 * i];
             l = a.stats[2 * i + 1];
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(TEAM_THREADS) void dist_team_kernel(DistArgs a) {
         __syncthreads();
         if (threadIdx.x == 0)
             for (int w = 1; w < TEAMS; ++w) sum += s_loss[w];
-        finish_loss<TEAM_THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
+        finish_loss<THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
     }
 }
 
@@ -288,7 +288,7 @@ struct Entries {
 };
 
 template <typename E, int THREADS, int NCH, bool GRAD>
-__global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
+__global__ __launch_bounds__(THREADS, 4) void dist_row_kernel(DistArgs a) {
     __shared__ PairRed<THREADS> s_max, s_sum;
     __shared__ Entries s_e[2];  // by turns: a wave may still read the last row's while the next row's are stored
     __shared__ float s_terms[THREADS / 64];
@@ -312,10 +312,10 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
                 a.stats[2 * i] = 0.f;
                 a.stats[2 * i + 1] = 0.f;
             }
-            if constexpr (GRAD) RowRegs<E, THREADS, NCH>::store(grow, a.v, tid, [](int, int) { return 0.f; });
+            if constexpr (GRAD) RowRegs<E, THREADS, NCH, true>::clear(grow, a.v, tid);
             continue;
         }
-        RowRegs<E, THREADS, NCH> r;
+        RowRegs<E, THREADS, NCH, true> r;
         r.load(row, a.v, tid);
         Entries &ent = s_e[turn];
         turn ^= 1;  // only rows that pass the barriers below take turns
@@ -328,13 +328,15 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
             ent.t[j] = t;
             tm = fmaxf(tm, t);
         }
-        float m = r.max();
+        float m = r.max(a.v);
         wide_max2<THREADS>(s_max, m, tm);
+        r.again();
         if (tid == 0) s_repeats = 0;  // read by all before that barrier, set by any behind the next
         const Shift s(a.c, m), ts(a.c, tm);
-        float l = r.sum_exp(s), tl = 0.f;
+        float l = r.sum_exp(s, a.v), tl = 0.f;
         for (int j = tid; j < a.k; j += THREADS) tl += ts.exp(ent.t[j]);
         wide_sum2<THREADS>(s_sum, l, tl);
+        r.again();
         const bool empty = l == 0.f || tl == 0.f;
         const float inv_l = empty ? 0.f : 1.f / l, inv_tl = empty ? 0.f : 1.f / tl;
         float terms = 0.f;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(DistArgs a) {
                 if (atomicOr(&s_bits[(c & (BITS - 1)) >> 5], bit) & bit) s_repeats = 1;
             }
         }
-        if constexpr (GRAD) RowRegs<E, THREADS, NCH>::store(grow, a.v, tid, [&](int j, int v) { return empty ? 0.f : factor * (s.exp(r.at(j, v)) * inv_l); });
+        if constexpr (GRAD) r.map(grow, a.v, tid, [&](float x) { return empty ? 0.f : factor * (s.exp(x) * inv_l); });
         if (tid < (a.k + 63) / 64 * 64 || tid < 64) {
             terms = team_sum<64>(terms);
             if ((tid & 63) == 0) s_terms[tid >> 6] = terms;
@@ -402,11 +404,12 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_part_kernel(DistArgs a) {
         return;
     }
     if (a.mask && !a.mask[i]) return;
-    RowRegs<E, SEG_THREADS, SEG_NCH> r;
+    RowRegs<E, SEG_THREADS, SEG_NCH, true> r;
     r.load((const E *)a.logits + i * a.row_stride + lo, len, threadIdx.x);
-    float m = r.max(), none = 0.f;
+    float m = r.max(len), none = 0.f;
     wide_max2<SEG_THREADS>(s_max, m, none);
-    float l = r.sum_exp(Shift(a.c, m));
+    r.again();
+    float l = r.sum_exp(Shift(a.c, m), len);
     wide_sum2<SEG_THREADS>(s_sum, l, none);
     if (threadIdx.x == 0) a.parts[blockIdx.x] = make_float2(m, l);
 }
@@ -433,10 +436,10 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
             }
             finish_loss<SEG_THREADS>(a, 0., (int)i, a.n, *a.inv_rows);
         }
-        if constexpr (GRAD) RowRegs<E, SEG_THREADS, SEG_NCH>::store(grow + lo, len, tid, [](int, int) { return 0.f; });
+        if constexpr (GRAD) RowRegs<E, SEG_THREADS, SEG_NCH, true>::clear(grow + lo, len, tid);
         return;
     }
-    RowRegs<E, SEG_THREADS, SEG_NCH> r;
+    RowRegs<E, SEG_THREADS, SEG_NCH, true> r;
     if constexpr (GRAD) r.load(row + lo, len, tid);
     float tm = -INFINITY, m = -INFINITY;
     for (int j = tid; j < a.k; j += SEG_THREADS) {
@@ -484,7 +487,7 @@ __global__ __launch_bounds__(SEG_THREADS) void dist_apply_kernel(DistArgs a) {
     }
     const float inv = *a.inv_rows, factor = grad_factor(a, inv);
     if constexpr (GRAD) {
-        RowRegs<E, SEG_THREADS, SEG_NCH>::store(grow + lo, len, tid, [&](int j, int v) { return empty ? 0.f : factor * (s.exp(r.at(j, v)) * inv_l); });
+        r.map(grow + lo, len, tid, [&](float x) { return empty ? 0.f : factor * (s.exp(x) * inv_l); });
     }
     if (VALUE && seg == 0) {
         terms = team_sum<64>(terms);
@@ -530,7 +533,7 @@ __global__ __launch_bounds__(1024) void dist_finish_kernel(DistArgs a, int parts
     for (int i = threadIdx.x; i < parts; i += 1024) s += a.loss_part[i];
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = s;
-    const float inv = inverse(a.mask ? count_kept<1024>(a.mask, a.n) : a.n);
+    const float inv = a.kept == KEPT_READ ? *a.inv_rows : inverse(a.mask ? count_kept<1024>(a.mask, a.n) : a.n);
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) s += s_sum[w];
@@ -557,7 +560,7 @@ enum Way { BY_TEAM, BY_ROW, BY_SEGMENT };
 struct Plan {
     Way way;
     int team, chunks;  // BY_TEAM: lanes a row, chunks a lane
-    int threads;       // BY_ROW: threads a row (chunks a thread in `chunks`)
+    int threads;       // of a workgroup (BY_ROW: threads a row, chunks a thread in `chunks`)
     int seg, segs;
 };
 inline Plan plan_rows(int n, int v, int vec) {
@@ -568,11 +571,13 @@ inline Plan plan_rows(int n, int v, int vec) {
         while (p.team < chunks && p.team < 64) p.team <<= 1;
         p.chunks = 1;
         while (p.team * p.chunks < chunks) p.chunks <<= 1;
+        // rows that 1024 threads finish in two rounds are left to one workgroup
+        p.threads = p.team <= 8 && n > 2 * (TEAM_THREADS / p.team) && n <= 2 * (1024 / p.team) ? 1024 : TEAM_THREADS;
         return p;
     }
     p.way = BY_ROW;
     if (chunks <= 256 * 8) p.threads = 256, p.chunks = 8;
-    else if (chunks <= 1024 * 8) p.threads = 1024, p.chunks = 8;
+    else if (chunks <= 512 * 16) p.threads = 512, p.chunks = 16;
     else if (chunks <= 1024 * 16) p.threads = 1024, p.chunks = 16;
     else p.way = BY_SEGMENT;
     // few rows of many columns: as workgroups of a row they would occupy one CU each
@@ -588,10 +593,9 @@ inline Plan plan_rows(int n, int v, int vec) {
 constexpr int DIST_BLOCKS = 2048;
 inline int dist_blocks(const Plan &p, int n) {
     if (p.way == BY_SEGMENT) return n > 0 ? n : 1;
-    const long rows = p.way == BY_TEAM ? TEAM_THREADS / p.team : 1;
+    const long rows = p.way == BY_TEAM ? p.threads / p.team : 1;
     const long want = ((long)n + rows - 1) / rows;
-    // up to four rounds of rows one workgroup goes alone: that is less than the launch that would join several
-    if (p.way == BY_TEAM && want <= 4) return 1;
+    if (p.way == BY_TEAM && want <= 2) return 1;  // a second round of rows costs less than the launch that joins workgroups
     return (int)(want < 1 ? 1 : std::min<long>(want, DIST_BLOCKS));
 }
 // Workspace: ticket, sums of row losses, segments
@@ -604,20 +608,27 @@ inline size_t space_bytes(const Plan &p, int n) {
 template <typename E, bool VALUE, bool GRAD>
 int launch_team(hipStream_t stream, const DistArgs &a, const Plan &p) {
     const dim3 grid(dist_blocks(p, a.n));
-#define DIST_TEAM(T, C) hipLaunchKernelGGL((dist_team_kernel<E, T, C, VALUE, GRAD>), grid, dim3(TEAM_THREADS), 0, stream, a)
-    switch (p.team * 16 + p.chunks) {
-        case 1 * 16 + 1: DIST_TEAM(1, 1); break;
-        case 2 * 16 + 1: DIST_TEAM(2, 1); break;
-        case 4 * 16 + 1: DIST_TEAM(4, 1); break;
-        case 8 * 16 + 1: DIST_TEAM(8, 1); break;
-        case 16 * 16 + 1: DIST_TEAM(16, 1); break;
-        case 32 * 16 + 1: DIST_TEAM(32, 1); break;
-        case 64 * 16 + 1: DIST_TEAM(64, 1); break;
-        case 64 * 16 + 2: DIST_TEAM(64, 2); break;
-        case 64 * 16 + 4: DIST_TEAM(64, 4); break;
-        default:
-            if constexpr (is_f32<E>()) DIST_TEAM(64, 8);
-            break;
+#define DIST_TEAM(N, T, C) hipLaunchKernelGGL((dist_team_kernel<E, N, T, C, VALUE, GRAD>), grid, dim3(N), 0, stream, a)
+    if (p.threads == 1024) {
+        if (p.team == 1) DIST_TEAM(1024, 1, 1);
+        else if (p.team == 2) DIST_TEAM(1024, 2, 1);
+        else if (p.team == 4) DIST_TEAM(1024, 4, 1);
+        else DIST_TEAM(1024, 8, 1);
+    } else {
+        switch (p.team * 16 + p.chunks) {
+            case 1 * 16 + 1: DIST_TEAM(256, 1, 1); break;
+            case 2 * 16 + 1: DIST_TEAM(256, 2, 1); break;
+            case 4 * 16 + 1: DIST_TEAM(256, 4, 1); break;
+            case 8 * 16 + 1: DIST_TEAM(256, 8, 1); break;
+            case 16 * 16 + 1: DIST_TEAM(256, 16, 1); break;
+            case 32 * 16 + 1: DIST_TEAM(256, 32, 1); break;
+            case 64 * 16 + 1: DIST_TEAM(256, 64, 1); break;
+            case 64 * 16 + 2: DIST_TEAM(256, 64, 2); break;
+            case 64 * 16 + 4: DIST_TEAM(256, 64, 4); break;
+            default:
+                if constexpr (is_f32<E>()) DIST_TEAM(256, 64, 8);
+                break;
+        }
     }
 #undef DIST_TEAM
     GDPSO_HIP(hipGetLastError());
@@ -630,7 +641,7 @@ int launch_distill(hipStream_t stream, const DistArgs &a, const Plan &p) {
     if (VALUE && p.way == BY_ROW) {
         const dim3 grid(dist_blocks(p, a.n));
         if (p.threads == 256) hipLaunchKernelGGL((dist_row_kernel<E, 256, 8, GRAD>), grid, dim3(256), 0, stream, a);
-        else if (p.chunks == 8) hipLaunchKernelGGL((dist_row_kernel<E, 1024, 8, GRAD>), grid, dim3(1024), 0, stream, a);
+        else if (p.threads == 512) hipLaunchKernelGGL((dist_row_kernel<E, 512, 16, GRAD>), grid, dim3(512), 0, stream, a);
         else hipLaunchKernelGGL((dist_row_kernel<E, 1024, 16, GRAD>), grid, dim3(1024), 0, stream, a);
     } else {
         const long blocks = (long)a.n * a.segs;

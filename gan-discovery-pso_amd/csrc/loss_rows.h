@@ -68,46 +68,117 @@ __device__ __forceinline__ float team_sum(float v) {
     return team_reduce<TEAM>(v, [](float a, float b) { return a + b; });
 }
 
-// NCH chunks of a row per thread.
-template <typename E, int TEAM, int NCH>
+// NCH chunks of a row per thread.  TAIL: the columns behind the last whole chunk are held one a thread instead of as a cut
+// chunk (teams of more threads than a chunk has elements): many chunks that each might be the cut one cost a
+// workgroup's rows twice the registers.
+template <typename E, int TEAM, int NCH, bool TAIL = false>
 struct RowRegs {
     static constexpr int VEC = vec_of<E>();
     using V = typename VecAt<E, VEC>::type;
-    V raw[NCH];
+    using W = __attribute__((ext_vector_type(4))) unsigned;
+    W raw[NCH];
+    E tail;
 
     __device__ __forceinline__ static int column(int j, int pos) { return (j * TEAM + pos) * VEC; }
     __device__ __forceinline__ void load(const E *__restrict__ row, int e, int pos) {
+        if constexpr (TAIL) {
+            static_assert(TEAM >= VEC, "a thread for every column of the tail");
+            constexpr unsigned none = is_f32<E>() ? 0xff800000u : (__is_same(E, bf16_t) ? 0xff80ff80u : 0xfc00fc00u);  // -inf
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+                const int c = column(j, pos);
+                raw[j] = W{none, none, none, none};
+                if (c + VEC <= e) raw[j] = __builtin_bit_cast(W, *(const V *)(row + c));
+            }
+            const int whole = e / VEC * VEC;
+            tail = whole + pos < e ? row[whole + pos] : (E)-INFINITY;
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             const int c = column(j, pos);
-            if (c + VEC <= e) raw[j] = *(const V *)(row + c);
+            V x;
+            if (c + VEC <= e) x = *(const V *)(row + c);
             else
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) raw[j][v] = c + v < e ? row[c + v] : (E)-INFINITY;
+                for (int v = 0; v < VEC; ++v) x[v] = c + v < e ? row[c + v] : (E)-INFINITY;
+            raw[j] = __builtin_bit_cast(W, x);
         }
     }
-    __device__ __forceinline__ float at(int j, int v) const { return (float)raw[j][v]; }
-    __device__ __forceinline__ float max() const {
-        float m = -INFINITY;
+    __device__ __forceinline__ float at(int j, int v) const {
+        if constexpr (is_f32<E>()) {
+            const unsigned word = raw[j][v];  // (bit_cast of the element itself would read element 0)
+            return __builtin_bit_cast(float, word);
+        } else if constexpr (__is_same(E, bf16_t)) return __builtin_bit_cast(float, v & 1 ? raw[j][v >> 1] & 0xffff0000u : raw[j][v >> 1] << 16);
+        else return (float)__builtin_bit_cast(f16_t, (unsigned short)(raw[j][v >> 1] >> (v & 1) * 16));
+    }
+    // Between two passes over the row: keeps the compiler from carrying 16-bit logits in their widened form (twice the
+    // registers) from one to the next.
+    __device__ __forceinline__ void again() {
+        if constexpr (!is_f32<E>())
 #pragma unroll
-        for (int j = 0; j < NCH; ++j)
+            for (int j = 0; j < NCH; ++j) {
+                unsigned a = raw[j][0], b = raw[j][1], c = raw[j][2], d = raw[j][3];
+                asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+                raw[j] = W{a, b, c, d};
+            }
+    }
+    // chunk j lies beyond the row for the whole team: the same for every thread, so a branch skips its arithmetic
+    __device__ __forceinline__ static bool beyond(int j, int e) { return j > 0 && j * TEAM * VEC >= e; }
+    __device__ __forceinline__ float max(int e) const {
+        float m = TAIL ? (float)tail : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            if (beyond(j, e)) continue;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) m = fmaxf(m, at(j, v));
+        }
         return m;
     }
-    __device__ __forceinline__ float sum_exp(const Shift &s) const {
-        float l = 0.f;
+    __device__ __forceinline__ float sum_exp(const Shift &s, int e) const {
+        float l = TAIL ? s.exp((float)tail) : 0.f;
 #pragma unroll
-        for (int j = 0; j < NCH; ++j)
+        for (int j = 0; j < NCH; ++j) {
+            if (beyond(j, e)) continue;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) l += s.exp(at(j, v));
+        }
         return l;
+    }
+    // row[c] = f(logit)
+    template <typename F>
+    __device__ __forceinline__ void map(E *__restrict__ row, int e, int pos, F f) const {
+        static_assert(TAIL, "rows with a tail");
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            if (beyond(j, e)) continue;
+            const int c = column(j, pos);
+            V x;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) x[v] = (E)f(at(j, v));
+            if (c + VEC <= e) *(V *)(row + c) = x;
+        }
+        const int whole = e / VEC * VEC;
+        if (whole + pos < e) row[whole + pos] = (E)f((float)tail);
+    }
+    // row[c] = 0
+    __device__ __forceinline__ static void clear(E *__restrict__ row, int e, int pos) {
+#pragma unroll 1
+        for (int j = 0; j < NCH; ++j) {
+            const int c = column(j, pos);
+            if (c + VEC <= e) *(V *)(row + c) = V{};
+            else
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    if (c + v < e) row[c + v] = (E)0.f;
+        }
     }
     // row[c] = f(j, v)
     template <typename F>
     __device__ __forceinline__ static void store(E *__restrict__ row, int e, int pos, F f) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
+            if (beyond(j, e)) continue;
             const int c = column(j, pos);
             V x;
 #pragma unroll

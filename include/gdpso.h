@@ -387,7 +387,7 @@ int gdpso_code_logits_grad(void *stream, int n, int d, int k, const float *grad_
  * choice).  mask [n] or NULL: rows whose byte is 0 are left out whatever they hold; their gradient is 0.  A kept row
  * without a finite logit has p = 0 (its choices count); NaN and +inf propagate.  No row kept, or no choice counted: loss 0.
  * Outputs: loss [1], counts int64 [e] (choices per code), totals int64 [2] (rows kept, choices counted), mean_prob
- * [e] = P, grad [n, e] in `dtype` or NULL.  1 <= e <= GDPSO_BALANCE_MAX_E.  n == 0 is allowed.
+ * [e] = P, grad [n, e] in `dtype` or NULL.  1 <= e <= GDPSO_BALANCE_MAX_E, n k < 2^32.  n == 0 is allowed.
  * gdpso_balance_grad: the gradient alone from counts and totals of an earlier call, times the DEVICE scalar *upstream. */
 #define GDPSO_BALANCE_MAX_E 16384
 size_t gdpso_balance_workspace_bytes(int n, int e);
