@@ -83,74 +83,84 @@ enum Product { LOGITS, GRAD_X, GRAD_CODE };
 // memory into registers, a stage ahead, and no value passes through LDS.  KC: the summed side is contiguous, a lane reads
 // its eight values of a row in one piece; else the rows' side is, and a lane reads MT neighbouring rows at eight summed
 // indices (tile t of the wave then holds rows t, MT + t, 2 MT + t ...).
+//
+// Loads have one form for every position, without a branch, and what they return stays as it came until it is cut: only then
+// does the compiler leave later stages' loads on the way while it waits for this one's.  Rows beyond the matrix are
+// clamped into it; a vector of MT rows is clamped as a whole and may so begin before the lane's first row (shift()).
 template <typename E, bool KC, int MT, int P, typename M>
 struct RowsOperand {
-    E v[MT][8];
+    static constexpr int W = KC ? 16 / (int)sizeof(E) : MT;      // elements a load
+    static constexpr int LOADS = KC ? MT * (8 / W) : 8;
+    static constexpr int ROWS = KC ? 1 : MT;                     // fewest rows of the matrix
+    typename VecAt<E, W>::type raw[LOADS];
 
     __device__ __forceinline__ static long row(long wave_row0, int i, int fr) { return KC ? wave_row0 + i * 16 + fr : wave_row0 + fr * MT + i; }
-    // The wave's first row and, from there, the byte offsets of this lane's piece of a stage.  Rows beyond the last one are
-    // clamped into the matrix (nothing uses their results); a vector over MT neighbouring rows (`pairs`) is clamped as a
-    // whole, so that it ends with the matrix's last row.  Whole stages load without a branch, so that the compiler can
-    // leave later stages' loads on the way while it waits for this one's.
-    __device__ __forceinline__ static long first_row(long wave_row0, long rows, bool pairs) { return min(wave_row0, rows - (!KC && pairs ? MT : 1)); }
-    __device__ __forceinline__ static void offsets(long ld, long wave_row0, long rows, int fr, int fk, bool pairs, unsigned (&off)[MT]) {
+    __device__ __forceinline__ static long clamped(long r, long rows) { return min(r, rows - ROWS); }
+    // The row that value i of this lane belongs to, and whether it is this lane's to write.
+    __device__ __forceinline__ static long held(long wave_row0, long rows, int i, int fr, bool &mine) {
+        const long r = row(wave_row0, i, fr);
+        if constexpr (KC) {
+            mine = r < rows;
+            return r;
+        } else {
+            const long first = row(wave_row0, 0, fr), h = clamped(first, rows) + i;
+            mine = h >= first;
+            return h;
+        }
+    }
+    __device__ __forceinline__ static long first_row(long wave_row0, long rows) { return clamped(wave_row0, rows); }
+    // Byte offsets of this lane's loads from the wave's first row at a stage's first summed element.
+    __device__ __forceinline__ static void offsets(long ld, long wave_row0, long rows, int fr, int fk, unsigned (&off)[KC ? MT : 1]) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const long last = !KC && pairs ? rows - MT + i : rows - 1;
-            const long r = min(row(wave_row0, i, fr), last) - first_row(wave_row0, rows, pairs);
+        for (int i = 0; i < (KC ? MT : 1); ++i) {
+            const long r = clamped(row(wave_row0, i, fr), rows) - first_row(wave_row0, rows);
             off[i] = (unsigned)((KC ? r * ld + fk : fk * ld + r) * (long)sizeof(E));
         }
     }
-    // stage: the wave's first row at the stage's first summed element; pairs: a lane's MT rows are neighbours after clamping
-    __device__ __forceinline__ void load_whole(const E *__restrict__ stage, long ld, const unsigned (&off)[MT], bool pairs) {
-        if constexpr (KC) {
-            constexpr int W = 16 / sizeof(E);
+    __device__ __forceinline__ void load_whole(const E *__restrict__ stage, long ld, const unsigned (&off)[KC ? MT : 1]) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int w = 0; w < 8 / W; ++w) {
-                    const auto x = at_bytes<typename VecAt<E, W>::type>(stage + w * W, off[i]);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) v[i][w * W + e] = x[e];
-                }
-        } else if (pairs) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const auto x = at_bytes<typename VecAt<E, MT>::type>(stage + e * ld, off[0]);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) v[i][e] = x[i];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) v[i][e] = at_bytes<E>(stage + e * ld, off[i]);
+        for (int l = 0; l < LOADS; ++l) {
+            if constexpr (KC) raw[l] = at_bytes<typename VecAt<E, W>::type>(stage + l % (8 / W) * W, off[l / (8 / W)]);
+            else raw[l] = at_bytes<typename VecAt<E, W>::type>(stage + l * ld, off[0]);
         }
     }
     // The stage that the sum's end cuts: `left` elements of it are there, the others read as 0.
-    __device__ __forceinline__ void load_part(const E *__restrict__ stage, long ld, const unsigned (&off)[MT], int fk, int left) {
+    __device__ __forceinline__ void load_part(const E *__restrict__ stage, long ld, const unsigned (&off)[KC ? MT : 1], int fk, int left) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int back = max(0, fk + e - (left - 1));  // elements beyond the last one that is there
+        for (int l = 0; l < LOADS; ++l)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const long step = ((long)e - back) * (KC ? 1 : ld) * (long)sizeof(E);
-                const E x = at_bytes<E>(stage, (unsigned)(off[i] + step));
-                v[i][e] = back == 0 ? x : (E)0.f;
+            for (int w = 0; w < (KC ? W : 1); ++w) {
+                const int e = KC ? l % (8 / W) * W + w : l;
+                const int back = max(0, fk + e - (left - 1));  // elements beyond the last one that is there
+                if constexpr (KC) {
+                    const E x = at_bytes<E>(stage, (unsigned)(off[l / (8 / W)] + ((long)e - back) * (long)sizeof(E)));
+                    raw[l][w] = back == 0 ? x : (E)0.f;
+                } else {
+                    const auto x = at_bytes<typename VecAt<E, W>::type>(stage, (unsigned)(off[0] + ((long)e - back) * ld * (long)sizeof(E)));
+#pragma unroll
+                    for (int c = 0; c < W; ++c) raw[l][c] = back == 0 ? x[c] : (E)0.f;
+                }
             }
-        }
+    }
+    // the eight values of row i
+    __device__ __forceinline__ void values(int i, E (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = KC ? raw[i * (8 / W) + e / W][e % W] : raw[e][i];
     }
 };
 
 // The operand on the output columns' side, shared by the waves: BN columns by KT of the summed side per stage, through
 // registers (a stage ahead) into P planes of parts in LDS, [P][BN][LROW].  KC: the summed side is contiguous in
-// memory; else the columns' side is, and the eight values of a fragment are gathered from eight rows by one thread.
+// memory; else the columns' side is, and the eight values of a fragment are gathered from eight rows by one thread, CW
+// neighbouring columns at a time.  Loads as RowsOperand's: columns beyond the matrix are clamped into it, a vector of CW
+// as a whole, and land in LDS where they belong (what belongs to no column of the matrix is never used).
 template <typename E, bool KC, int BN, int P, typename M>
 struct ColsOperand {
     static constexpr int CW = KC ? 1 : (BN * 4 > CL_THREADS ? BN * 4 / CL_THREADS : 1);  // columns a unit
     static constexpr int UNITS = BN * 4 / CW;
     static constexpr int NU = (UNITS + CL_THREADS - 1) / CL_THREADS;
-    E v[NU][CW][8];
+    static constexpr int W = KC ? 16 / (int)sizeof(E) : CW, LOADS = KC ? 8 / W : 8;
+    typename VecAt<E, W>::type raw[NU][LOADS];
 
     __device__ __forceinline__ static bool unit(int i, int &col, int &kc) {
         const int u = threadIdx.x + i * CL_THREADS;
@@ -163,86 +173,81 @@ struct ColsOperand {
         }
         return UNITS % CL_THREADS == 0 || u < UNITS;
     }
-    // As RowsOperand::offsets and load_whole, from the tile's first column; threads without a unit repeat another's.
-    __device__ __forceinline__ static void offsets(long ld, long col0, long cols, bool pairs, unsigned (&off)[NU][CW]) {
+    // Columns from the tile's first one to the first one that unit i holds: a clamped vector may begin before the tile.
+    __device__ __forceinline__ static int base(long col0, long cols, int i, int &kc) {
+        int c0;
+        unit(i, c0, kc);
+        kc &= 3;
+        return (int)(min(col0 + c0, cols - CW) - col0);
+    }
+    // The column that a stage's address and the offsets count from.
+    __device__ __forceinline__ static long origin(long col0) { return CW == 1 ? col0 : max(col0 - CW, 0l); }
+    __device__ __forceinline__ static void offsets(long ld, long col0, long cols, unsigned (&off)[NU]) {
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            int c0, kc;
-            unit(i, c0, kc);
-            kc &= 3;
-#pragma unroll
-            for (int c = 0; c < CW; ++c) {
-                const long col = min(col0 + c0 + c, !KC && pairs ? cols - CW + c : cols - 1) - col0;
-                off[i][c] = (unsigned)((KC ? col * ld + kc * 8 : kc * 8 * ld + col) * (long)sizeof(E));
-            }
+            int kc;
+            const long col = base(col0, cols, i, kc) + col0 - origin(col0);
+            off[i] = (unsigned)((KC ? col * ld + kc * 8 : kc * 8 * ld + col) * (long)sizeof(E));
         }
     }
-    __device__ __forceinline__ void load_whole(const E *__restrict__ stage, long ld, const unsigned (&off)[NU][CW], bool pairs) {
+    __device__ __forceinline__ void load_whole(const E *__restrict__ stage, long ld, const unsigned (&off)[NU]) {
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            if constexpr (KC) {
-                constexpr int W = 16 / sizeof(E);
+        for (int i = 0; i < NU; ++i)
 #pragma unroll
-                for (int w = 0; w < 8 / W; ++w) {
-                    const auto x = at_bytes<typename VecAt<E, W>::type>(stage + w * W, off[i][0]);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) v[i][0][w * W + e] = x[e];
-                }
-            } else if (pairs) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const auto x = at_bytes<typename VecAt<E, CW>::type>(stage + e * ld, off[i][0]);
-#pragma unroll
-                    for (int c = 0; c < CW; ++c) v[i][c][e] = x[c];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int c = 0; c < CW; ++c) v[i][c][e] = at_bytes<E>(stage + e * ld, off[i][c]);
-            }
-        }
+            for (int l = 0; l < LOADS; ++l) raw[i][l] = at_bytes<typename VecAt<E, W>::type>(KC ? stage + l * W : stage + l * ld, off[i]);
     }
-    __device__ __forceinline__ void load_part(const E *__restrict__ stage, long ld, const unsigned (&off)[NU][CW], int left) {
+    __device__ __forceinline__ void load_part(const E *__restrict__ stage, long ld, const unsigned (&off)[NU], int left) {
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             int c0, kc;
             unit(i, c0, kc);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int back = max(0, (kc & 3) * 8 + e - (left - 1));
+            for (int l = 0; l < LOADS; ++l)
 #pragma unroll
-                for (int c = 0; c < CW; ++c) {
-                    const long step = ((long)e - back) * (KC ? 1 : ld) * (long)sizeof(E);
-                    const E x = at_bytes<E>(stage, (unsigned)(off[i][c] + step));
-                    v[i][c][e] = back == 0 ? x : (E)0.f;
+                for (int w = 0; w < (KC ? W : 1); ++w) {
+                    const int e = KC ? l * W + w : l;
+                    const int back = max(0, (kc & 3) * 8 + e - (left - 1));
+                    const unsigned at = (unsigned)(off[i] + ((long)e - back) * (KC ? 1 : ld) * (long)sizeof(E));
+                    if constexpr (KC) {
+                        const E x = at_bytes<E>(stage, at);
+                        raw[i][l][w] = back == 0 ? x : (E)0.f;
+                    } else {
+                        const auto x = at_bytes<typename VecAt<E, W>::type>(stage, at);
+#pragma unroll
+                        for (int c = 0; c < W; ++c) raw[i][l][c] = back == 0 ? x[c] : (E)0.f;
+                    }
                 }
-            }
         }
     }
+    __device__ __forceinline__ E value(int i, int c, int e) const { return KC ? raw[i][e / W][e % W] : raw[i][e][c]; }
     __device__ __forceinline__ void add_squares(float (&sums)[NU]) const {
         using E2 = __attribute__((ext_vector_type(2))) E;
 #pragma unroll
         for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                const E2 x = {v[i][0][e], v[i][0][e + 1]};
+                const E2 x = {value(i, 0, e), value(i, 0, e + 1)};
                 if constexpr (is_f32<E>()) sums[i] = fmaf(x[1], x[1], fmaf(x[0], x[0], sums[i]));
                 else if constexpr (__is_same(E, bf16_t)) sums[i] = __builtin_amdgcn_fdot2_f32_bf16(x, x, sums[i], false);
                 else sums[i] = __builtin_amdgcn_fdot2(x, x, sums[i], false);
             }
     }
-    __device__ __forceinline__ void store(M *lds) const {
+    __device__ __forceinline__ void store(M *lds, long col0, long cols) const {
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             int c0, kc;
             if (!unit(i, c0, kc)) continue;
+            const int row = CW == 1 ? c0 : base(col0, cols, i, kc);
 #pragma unroll
             for (int c = 0; c < CW; ++c) {
-                Frag<M> parts[P];
-                cut<P, M>(v[i][c], parts);
+                E v[8];
 #pragma unroll
-                for (int p = 0; p < P; ++p) *(Frag<M> *)(lds + (p * BN + c0 + c) * LROW + kc * 8) = parts[p];
+                for (int e = 0; e < 8; ++e) v[e] = value(i, c, e);
+                Frag<M> parts[P];
+                cut<P, M>(v, parts);
+                if (CW == 1 || row + c >= 0)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) *(Frag<M> *)(lds + (p * BN + row + c) * LROW + kc * 8) = parts[p];
             }
         }
     }
@@ -330,24 +335,25 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     OpN on[DEPTH];
     float sq[OpN::NU] = {}, sum_m[MT] = {};
     f32x4 acc[MT][NT] = {};
-    // a lane's MT rows (a unit's CW columns) are all there or none where their number divides evenly
-    const bool pairs_m = a.rows % MT == 0, pairs_n = a.cols % OpN::CW == 0;
-    unsigned off_m[MT], off_n[OpN::NU][OpN::CW];
-    OpM::offsets(a.ld_m, m0, a.rows, fr, fk, pairs_m, off_m);
-    OpN::offsets(a.ld_n, n0, a.cols, pairs_n, off_n);
-    const EM *const pm = (const EM *)a.m + OpM::first_row(m0, a.rows, pairs_m) * (KC_M ? a.ld_m : 1);
-    const EN *const pn = (const EN *)a.n + (KC_N ? n0 * a.ld_n : n0);
+    unsigned off_m[KC_M ? MT : 1];
+    unsigned off_n[OpN::NU];
+    OpM::offsets(a.ld_m, m0, a.rows, fr, fk, off_m);
+    OpN::offsets(a.ld_n, n0, a.cols, off_n);
+    const EM *const pm = (const EM *)a.m + OpM::first_row(m0, a.rows) * (KC_M ? a.ld_m : 1);
+    const EN *const pn = (const EN *)a.n + OpN::origin(n0) * (KC_N ? a.ld_n : 1);
     const auto stage = [&](OpN &n, int buf, bool there) {
-        n.store(&s_n[buf][0][0][0]);
+        n.store(&s_n[buf][0][0][0], n0, a.cols);
         if (OP == LOGITS && there) n.add_squares(sq);
     };
     const auto rows_fragments = [&](const OpM &m, Frag<M> (&fm)[MT][PM]) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
+            EM v[8];
+            m.values(i, v);
             if constexpr (OP == GRAD_CODE)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum_m[i] += (float)m.v[i][e];
-            cut<PM, M>(m.v[i], fm[i]);
+                for (int e = 0; e < 8; ++e) sum_m[i] += (float)v[e];
+            cut<PM, M>(v, fm[i]);
         }
     };
     const auto multiply = [&](const Frag<M> (&fm)[MT][PM], int buf) {
@@ -373,8 +379,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     const int stages = (int)((kend - k0) / KT);
     const auto load = [&](OpM &m, OpN &n, int s) {
         const long k = k0 + (long)min(s, stages - 1) * KT;
-        m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m, pairs_m);
-        n.load_whole(pn + (KC_N ? k : k * a.ld_n), a.ld_n, off_n, pairs_n);
+        m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m);
+        n.load_whole(pn + (KC_N ? k : k * a.ld_n), a.ld_n, off_n);
     };
     // stage s: its rows' operand is in om[CUR], its columns' in plane CUR & 1
     const auto step = [&](auto which, int s) {
@@ -426,8 +432,9 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     // A lane holds four consecutive columns of one row of each 16 x 16 tile.
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const long m = OpM::row(m0, i, fr);
-        if (m >= a.rows) continue;
+        bool mine;
+        const long m = OpM::held(m0, a.rows, i, fr, mine);
+        if (!mine) continue;
         if (part && tn == 0 && lane < 16) partial[a.rows * a.cols + m] = sum_m[i];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -479,13 +486,13 @@ __global__ __launch_bounds__(CL_THREADS) void logits_kernel(ProductArgs a) {
     const int col_tiles = (int)((a.cols + BN - 1) / BN);
     OpN on[NS];
     const auto load_codes = [&](int t) {
-        unsigned off[OpN::NU][OpN::CW];
-        OpN::offsets(a.ld_n, (long)t * BN, a.cols, false, off);
+        unsigned off[OpN::NU];
+        OpN::offsets(a.ld_n, (long)t * BN, a.cols, off);
         const E *p = (const E *)a.n + (long)t * BN * a.ld_n;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int left = (int)a.sum - s * KT;  // only the last stage may be cut
-            if (s + 1 < NS || left >= KT) on[s].load_whole(p + s * KT, a.ld_n, off, true);
+            if (s + 1 < NS || left >= KT) on[s].load_whole(p + s * KT, a.ld_n, off);
             else on[s].load_part(p + s * KT, a.ld_n, off, left);
         }
     };
@@ -493,7 +500,7 @@ __global__ __launch_bounds__(CL_THREADS) void logits_kernel(ProductArgs a) {
         float sq[OpN::NU] = {};
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            on[s].store(&s_n[buf][s][0][0][0]);
+            on[s].store(&s_n[buf][s][0][0][0], 0, 0);
             on[s].add_squares(sq);
         }
         norms<OpN>(sq, [&](int c) { return norm_at(buf, c); });
@@ -502,19 +509,23 @@ __global__ __launch_bounds__(CL_THREADS) void logits_kernel(ProductArgs a) {
     {
         OpM om[NS];
         unsigned off[MT];
-        OpM::offsets(a.ld_m, m0, a.rows, fr, fk, false, off);
-        const E *p = (const E *)a.m + OpM::first_row(m0, a.rows, false) * a.ld_m;
+        OpM::offsets(a.ld_m, m0, a.rows, fr, fk, off);
+        const E *p = (const E *)a.m + OpM::first_row(m0, a.rows) * a.ld_m;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int left = (int)a.sum - s * KT;
-            if (s + 1 < NS || left >= KT) om[s].load_whole(p + s * KT, a.ld_m, off, true);
+            if (s + 1 < NS || left >= KT) om[s].load_whole(p + s * KT, a.ld_m, off);
             else om[s].load_part(p + s * KT, a.ld_m, off, fk, left);
         }
         load_codes(first);
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) cut<P, M>(om[s].v[i], fm[s][i]);
+            for (int i = 0; i < MT; ++i) {
+                E v[8];
+                om[s].values(i, v);
+                cut<P, M>(v, fm[s][i]);
+            }
     }
     if (AHEAD) keep_codes(0);
     int buf = 0;
@@ -572,28 +583,37 @@ __device__ __forceinline__ void small_tile(const ProductArgs &a, const int block
     constexpr bool KC_M = OP == GRAD_X;
     constexpr int WAVES = CL_THREADS / 64, DEPTH = 2;
     using OpM = RowsOperand<float, KC_M, 1, 3, bf16_t>;
-    using OpN = RowsOperand<E, false, SMALL_NT, P, bf16_t>;  // columns as rows: a lane holds two neighbouring ones
+    using OpN = RowsOperand<E, false, 1, P, bf16_t>;  // sixteen columns as rows
     const int tm = block % a.tiles_m, rest = block / a.tiles_m, tn = rest % a.tiles_n, split = rest / a.tiles_n;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long m0 = (long)tm * 16, n0 = (long)tn * (16 * SMALL_NT);
     const long k0 = split * a.sum_per_split, kend = min(k0 + a.sum_per_split, a.sum);
     const int fr = lane & 15, fk = (lane >> 4) * 8;
-    const bool pairs_n = a.cols % SMALL_NT == 0;
-    unsigned off_m[1], off_n[SMALL_NT];
-    OpM::offsets(a.ld_m, m0, a.rows, fr, fk, true, off_m);
-    OpN::offsets(a.ld_n, n0, a.cols, fr, fk, pairs_n, off_n);
-    const float *const pm = (const float *)a.m + OpM::first_row(m0, a.rows, true) * (KC_M ? a.ld_m : 1);
-    const E *const pn = (const E *)a.n + OpN::first_row(n0, a.cols, pairs_n);
+    unsigned off_m[1], off_n[SMALL_NT][1];
+    OpM::offsets(a.ld_m, m0, a.rows, fr, fk, off_m);
+    const float *const pm = (const float *)a.m + OpM::first_row(m0, a.rows) * (KC_M ? a.ld_m : 1);
+    const E *pn[SMALL_NT];
+#pragma unroll
+    for (int j = 0; j < SMALL_NT; ++j) {
+        OpN::offsets(a.ld_n, n0 + j * 16, a.cols, fr, fk, off_n[j]);
+        pn[j] = (const E *)a.n + OpN::first_row(n0 + j * 16, a.cols);
+    }
     float sum_m = 0.f;
     f32x4 acc[SMALL_NT] = {};
-    const auto multiply = [&](const OpM &m, const OpN &n) {
+    const auto multiply = [&](const OpM &m, const OpN (&n)[SMALL_NT]) {
         Frag<bf16_t> fm[3], fn[SMALL_NT][P];
+        float v[8];
+        m.values(0, v);
         if constexpr (OP == GRAD_CODE)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum_m += m.v[0][e];
-        cut<3, bf16_t>(m.v[0], fm);
+            for (int e = 0; e < 8; ++e) sum_m += v[e];
+        cut<3, bf16_t>(v, fm);
 #pragma unroll
-        for (int j = 0; j < SMALL_NT; ++j) cut<P, bf16_t>(n.v[j], fn[j]);
+        for (int j = 0; j < SMALL_NT; ++j) {
+            E w[8];
+            n[j].values(0, w);
+            cut<P, bf16_t>(w, fn[j]);
+        }
 #pragma unroll
         for (int order = 2; order >= 0; --order)
 #pragma unroll
@@ -605,13 +625,14 @@ __device__ __forceinline__ void small_tile(const ProductArgs &a, const int block
             }
     };
     const int whole = (int)((kend - k0) / KT), mine = whole > wave ? (whole - wave + WAVES - 1) / WAVES : 0;  // whole stages, this wave's
-    const auto load = [&](OpM &m, OpN &n, int t) {
+    const auto load = [&](OpM &m, OpN (&n)[SMALL_NT], int t) {
         const long k = k0 + (long)(wave + min(t, mine - 1) * WAVES) * KT;
-        m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m, true);
-        n.load_whole(pn + k * a.ld_n, a.ld_n, off_n, pairs_n);
+        m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m);
+#pragma unroll
+        for (int j = 0; j < SMALL_NT; ++j) n[j].load_whole(pn[j] + k * a.ld_n, a.ld_n, off_n[j]);
     };
     OpM om[DEPTH];
-    OpN on[DEPTH];
+    OpN on[DEPTH][SMALL_NT];
     if (mine > 0) {
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) load(om[i], on[i], i);
@@ -626,7 +647,8 @@ __device__ __forceinline__ void small_tile(const ProductArgs &a, const int block
     const long done = k0 + (long)whole * KT;
     if (done < kend && wave == whole % WAVES) {  // what is left of the sum
         om[0].load_part(pm + (KC_M ? done : done * a.ld_m), a.ld_m, off_m, fk, (int)(kend - done));
-        on[0].load_part(pn + done * a.ld_n, a.ld_n, off_n, fk, (int)(kend - done));
+#pragma unroll
+        for (int j = 0; j < SMALL_NT; ++j) on[0][j].load_part(pn[j] + done * a.ld_n, a.ld_n, off_n[j], fk, (int)(kend - done));
         multiply(om[0], on[0]);
     }
     if constexpr (OP == GRAD_CODE) {
@@ -646,14 +668,13 @@ __device__ __forceinline__ void small_tile(const ProductArgs &a, const int block
     const bool part = OP == GRAD_CODE && a.splits > 1;
     float *partial = (float *)a.out + split * (a.rows * a.cols + a.rows);
     if (part && tn == 0 && lane < 16) partial[a.rows * a.cols + m] = sum_m;
-    // columns n0 + fr' * 2 + j for fr' = 4 (lane / 16) + e: eight neighbours a lane
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const long n = n0 + (lane >> 4) * 8 + h * 4;
+    for (int j = 0; j < SMALL_NT; ++j) {
+        const long n = n0 + j * 16 + (lane >> 4) * 4;
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            x[e] = acc[e & 1][h * 2 + (e >> 1)];
+            x[e] = acc[j][e];
             if constexpr (OP == GRAD_X) x[e] *= a.scale;
             if constexpr (OP == GRAD_CODE)
                 if (!part && n + e < a.cols) x[e] = a.scale * fmaf(-sum_m, (float)((const E *)a.code)[m * a.cols + n + e], x[e]);
@@ -717,18 +738,18 @@ constexpr int SMALL_ROWS = 4096;
 struct Tile {
     int mt, nt;
 };
-inline Tile grad_tile(int n, int d) {
+inline Tile grad_tile(int n, int d, int k) {
     if (n <= SMALL_ROWS) return {0, 0};
     const int nt = d <= 32 ? 2 : (d <= 64 ? 4 : (d <= 128 ? 8 : 16));
     // 128 rows a workgroup once they fill the chip; 256 columns leave registers for 64
-    return {nt < 16 && n >= 32768 ? 2 : 1, nt};
+    return {nt < 16 && n >= 32768 && k > 1 ? 2 : 1, nt};
 }
 // Splits of the summed rows of the codebook's gradient.  Small: 512 rows, four stages a wave, and up to there one split does
 // without the join's launch.  Else about two workgroups a CU, at least 128 rows each (the partial sums that a split writes
 // and the join reads have to stay small beside its rows).
 inline int code_splits(int n, int d, int k) {
     if (n <= SMALL_ROWS) return ceil_div(n, 512);
-    const Tile t = grad_tile(n, d);
+    const Tile t = grad_tile(n, d, k);
     const long tiles = (long)ceil_div(k, 64 * t.mt) * ceil_div(d, 16 * t.nt);
     const long want = ceil_div(512, tiles), most = ceil_div(n, 128);
     return (int)(want < most ? want : most);
@@ -857,7 +878,7 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
         const long per = ceil_div(ceil_div(n, splits), KT) * (long)KT;
         const ProductArgs code = {grad_logits, inputs, splits > 1 && grad_codebook ? workspace : grad_codebook, k, d, n, k, d, 0, 0, splits, per, scale, codebook};
         const ProductArgs x = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale, nullptr};
-        GDPSO_WITH_DTYPE(dtype, rc = launch_grads<E>(stream, code, x, grad_tile(n, d)));
+        GDPSO_WITH_DTYPE(dtype, rc = launch_grads<E>(stream, code, x, grad_tile(n, d, k)));
         if (rc) return rc;
     }
     if (grad_codebook && splits != 1) {  // no rows: zeros
