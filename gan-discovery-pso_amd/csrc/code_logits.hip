@@ -150,7 +150,7 @@ struct RowsOperand {
 };
 
 // The operand on the output columns' side, shared by the waves: BN columns by KT of the summed side per stage, through
-// registers (a stage ahead) into P planes of parts in LDS, [P][BN][LROW].  KC: the summed side is contiguous in
+// registers (a stage ahead) into P planes of parts in LDS, [P][PLANE][LROW].  KC: the summed side is contiguous in
 // memory; else the columns' side is, and the eight values of a fragment are gathered from eight rows by one thread, CW
 // neighbouring columns at a time.  Loads as RowsOperand's: columns beyond the matrix are clamped into it, a vector of CW
 // as a whole, and land in LDS where they belong (what belongs to no column of the matrix is never used).
@@ -160,6 +160,8 @@ struct ColsOperand {
     static constexpr int UNITS = BN * 4 / CW;
     static constexpr int NU = (UNITS + CL_THREADS - 1) / CL_THREADS;
     static constexpr int W = KC ? 16 / (int)sizeof(E) : CW, LOADS = KC ? 8 / W : 8;
+    static constexpr int AHEAD = CW > 1 ? CW : 0;  // rows of a plane ahead of the tile's columns, for vectors that begin before it
+    static constexpr int PLANE = BN + AHEAD;       // rows of a plane
     typename VecAt<E, W>::type raw[NU][LOADS];
 
     __device__ __forceinline__ static bool unit(int i, int &col, int &kc) {
@@ -237,7 +239,7 @@ struct ColsOperand {
         for (int i = 0; i < NU; ++i) {
             int c0, kc;
             if (!unit(i, c0, kc)) continue;
-            const int row = CW == 1 ? c0 : base(col0, cols, i, kc);
+            const int row = AHEAD + (CW == 1 ? c0 : base(col0, cols, i, kc));
 #pragma unroll
             for (int c = 0; c < CW; ++c) {
                 E v[8];
@@ -245,10 +247,50 @@ struct ColsOperand {
                 for (int e = 0; e < 8; ++e) v[e] = value(i, c, e);
                 Frag<M> parts[P];
                 cut<P, M>(v, parts);
-                if (CW == 1 || row + c >= 0)
 #pragma unroll
-                    for (int p = 0; p < P; ++p) *(Frag<M> *)(lds + (p * BN + row + c) * LROW + kc * 8) = parts[p];
+                for (int p = 0; p < P; ++p) *(Frag<M> *)(lds + (p * PLANE + row + c) * LROW + kc * 8) = parts[p];
             }
+        }
+    }
+};
+
+// The same for the gradients of 16-bit codes and latents, from planes that planes_kernel has cut and transposed: P planes of bf16, each
+// [pitch / KT][cols][KT] with `pitch` the sum's length rounded up to whole stages, zeros behind its end.  A stage passes
+// through registers as it is.  Gathering 16-bit values anew in every workgroup took half of these gradients' time
+// (50007 x 1024 x 256, bf16: both 234 us, 181 from planes); with fp32 the six matrix instructions a product hide it, and the
+// planes' own launch is a loss (65536 x 512 x 64: 68 us, 67 from planes and 14 for those).
+template <int BN, int P>
+struct PlanesOperand {
+    static constexpr int UNITS = BN * 4, NU = (UNITS + CL_THREADS - 1) / CL_THREADS, AHEAD = 0, PLANE = BN;
+    bf16x8 raw[NU][P];
+
+    __device__ __forceinline__ static void unit(int i, int &col, int &kc) {
+        const int u = threadIdx.x + i * CL_THREADS;
+        col = u >> 2;
+        kc = u & 3;
+    }
+    __device__ __forceinline__ static void offsets(long, long col0, long cols, unsigned (&off)[NU]) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            int c, kc;
+            unit(i, c, kc);
+            off[i] = (unsigned)(((min(col0 + c, cols - 1) - col0) * KT + kc * 8) * 2);
+        }
+    }
+    __device__ __forceinline__ void load(const bf16_t *__restrict__ stage, long plane, const unsigned (&off)[NU]) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int p = 0; p < P; ++p) raw[i][p] = at_bytes<bf16x8>(stage + p * plane, off[i]);
+    }
+    __device__ __forceinline__ void store(bf16_t *lds, long, long) const {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            int c, kc;
+            unit(i, c, kc);
+            if (UNITS % CL_THREADS == 0 || c < BN)
+#pragma unroll
+                for (int p = 0; p < P; ++p) *(bf16x8 *)(lds + (p * BN + c) * LROW + kc * 8) = raw[i][p];
         }
     }
 };
@@ -274,16 +316,23 @@ struct ProductArgs {
     const void *m, *n;  // operands: output rows' side and output columns' side
     void *out;          // result; GRAD_CODE with several splits: partial sums, float [split][rows * cols + rows]
     long rows, cols, sum;
-    long ld_m, ld_n;
+    long ld_m, ld_n;    // ld_n: GRAD_*: pitch of the planes, whose size is cols * ld_n
     int tiles_m, tiles_n, splits;
     long sum_per_split;  // a multiple of KT
     float scale;
     const void *code;    // GRAD_CODE with one split: the codebook
 };
+// How a tile's columns' operand lies in memory and in LDS.
+template <typename E>
+constexpr bool from_planes() {
+    return !is_f32<E>();
+}
+template <Product OP, typename E, int P, typename M, int NT>
+using ColumnsOperand = std::conditional_t<OP != LOGITS && from_planes<E>(), PlanesOperand<NT * 16, P>, ColsOperand<E, OP == LOGITS, NT * 16, P, M>>;
 // LDS of a tile: two stages of the columns' operand, and the norms of its codes.
-template <Product OP, int PN, int NT>
+template <Product OP, typename E, int P, int NT>
 constexpr int tile_lds() {
-    return 2 * PN * NT * 16 * LROW * 2 + (OP == LOGITS ? NT * 16 * 4 : 0);
+    return 2 * P * ColumnsOperand<OP, E, P, bf16_t, NT>::PLANE * LROW * 2 + (OP == LOGITS ? NT * 16 * 4 : 0);
 }
 
 // Four consecutive columns of a row.
@@ -303,12 +352,13 @@ __device__ __forceinline__ void put4(EO *row, long n, long cols, const float (&x
 // operands are on the way while one multiplies: a stage's matrix instructions take less time than memory to answer.
 template <Product OP, typename EM, typename EN, int PM, int PN, typename M, int MT, int NT, typename EO>
 __device__ __forceinline__ void product_tile(const ProductArgs &a, const int block, char *lds) {
-    constexpr bool KC_M = OP != GRAD_CODE, KC_N = OP == LOGITS;
+    constexpr bool KC_M = OP != GRAD_CODE, KC_N = OP == LOGITS, PLANES = OP != LOGITS && from_planes<EN>();
     constexpr int BN = NT * 16;
     using OpM = RowsOperand<EM, KC_M, MT, PM, M>;
-    using OpN = ColsOperand<EN, KC_N, BN, PN, M>;
-    M(*s_n)[PN][BN][LROW] = (M(*)[PN][BN][LROW])lds;
-    float *s_norm = (float *)(lds + 2 * PN * BN * LROW * sizeof(M));
+    using OpN = ColumnsOperand<OP, EN, PN, M, NT>;
+    using MN = std::conditional_t<PLANES, bf16_t, EN>;  // what the columns' operand lies in memory as
+    M(*s_n)[PN][OpN::PLANE][LROW] = (M(*)[PN][OpN::PLANE][LROW])lds;
+    float *s_norm = (float *)(lds + 2 * PN * OpN::PLANE * LROW * sizeof(M));
     // Workgroups b and b + 8 run on one XCD: the tiles that share rows (GRAD_CODE: a split) go to the same one, whose L2
     // then serves the shared operand once.
     const int xcd = block & 7, slot = block >> 3;
@@ -340,10 +390,13 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     OpM::offsets(a.ld_m, m0, a.rows, fr, fk, off_m);
     OpN::offsets(a.ld_n, n0, a.cols, off_n);
     const EM *const pm = (const EM *)a.m + OpM::first_row(m0, a.rows) * (KC_M ? a.ld_m : 1);
-    const EN *const pn = (const EN *)a.n + OpN::origin(n0) * (KC_N ? a.ld_n : 1);
+    const MN *pn = (const MN *)a.n;
+    if constexpr (PLANES) pn += n0 * KT;
+    else pn += OpN::origin(n0) * (KC_N ? a.ld_n : 1);
     const auto stage = [&](OpN &n, int buf, bool there) {
         n.store(&s_n[buf][0][0][0], n0, a.cols);
-        if (OP == LOGITS && there) n.add_squares(sq);
+        if constexpr (OP == LOGITS)
+            if (there) n.add_squares(sq);
     };
     const auto rows_fragments = [&](const OpM &m, Frag<M> (&fm)[MT][PM]) {
 #pragma unroll
@@ -361,7 +414,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
         for (int j = 0; j < NT; ++j) {
             Frag<M> fn[PN];
 #pragma unroll
-            for (int p = 0; p < PN; ++p) fn[p] = *(const Frag<M> *)&s_n[buf][p][j * 16 + fr][fk];
+            for (int p = 0; p < PN; ++p) fn[p] = *(const Frag<M> *)&s_n[buf][p][OpN::AHEAD + j * 16 + fr][fk];
             // the small products first
 #pragma unroll
             for (int order = 2; order >= 0; --order)
@@ -380,7 +433,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     const auto load = [&](OpM &m, OpN &n, int s) {
         const long k = k0 + (long)min(s, stages - 1) * KT;
         m.load_whole(pm + (KC_M ? k : k * a.ld_m), a.ld_m, off_m);
-        n.load_whole(pn + (KC_N ? k : k * a.ld_n), a.ld_n, off_n);
+        if constexpr (PLANES) n.load(pn + k * a.cols, a.cols * a.ld_n, off_n);
+        else n.load_whole(pn + (KC_N ? k : k * a.ld_n), a.ld_n, off_n);
     };
     // stage s: its rows' operand is in om[CUR], its columns' in plane CUR & 1
     const auto step = [&](auto which, int s) {
@@ -407,7 +461,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
     if (done < kend) {  // what is left of the sum
         const int left = (int)(kend - done);
         om[0].load_part(pm + (KC_M ? done : done * a.ld_m), a.ld_m, off_m, fk, left);
-        on[0].load_part(pn + (KC_N ? done : done * a.ld_n), a.ld_n, off_n, left);
+        if constexpr (PLANES) on[0].load(pn + done * a.cols, a.cols * a.ld_n, off_n);
+        else on[0].load_part(pn + (KC_N ? done : done * a.ld_n), a.ld_n, off_n, left);
         Frag<M> fm[MT][PM];
         rows_fragments(om[0], fm);
         __syncthreads();
@@ -458,7 +513,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
 // The logits of long rows (those whose fragments logits_kernel could not keep in registers).
 template <typename E, int P, typename M, int MT, int NT>
 __global__ __launch_bounds__(CL_THREADS, 2) void logits_tile_kernel(ProductArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[tile_lds<LOGITS, P, NT>()];
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds<LOGITS, E, P, NT>()];
     product_tile<LOGITS, E, E, P, P, M, MT, NT, float>(a, blockIdx.x, lds);
 }
 
@@ -691,12 +746,64 @@ __global__ __launch_bounds__(CL_THREADS) void grads_small_kernel(ProductArgs cod
     else small_tile<GRAD_X, E, P>(x, blockIdx.x - code_blocks, s_acc, s_sum);
 }
 
-// Both gradients in one launch, the codebook's workgroups first (they run longer).
-template <typename E, int P, int MT, int NT>
+// Cuts and transposes a matrix [rows][cols] into P planes [pitch / KT][cols][KT] of bf16, zeros behind the last row: 64 x 64
+// elements a workgroup, through LDS.  The codebook's workgroups first, then the latents'.
+struct PlanesArgs {
+    const void *src[2];
+    bf16_t *dst[2];
+    long rows[2], pitch[2];
+    int cols, first;  // workgroups of the first matrix
+};
+template <typename E, int P>
+__global__ __launch_bounds__(CL_THREADS) void planes_kernel(PlanesArgs a) {
+    using V = typename VecAt<E, 8>::type;
+    __shared__ E s_x[64][64 + 2];
+    const int which = (int)blockIdx.x >= a.first, block = blockIdx.x - (which ? a.first : 0);
+    const int col_tiles = (a.cols + 63) / 64;
+    const long r0 = (long)(block / col_tiles) * 64, rows = a.rows[which], pitch = a.pitch[which];
+    const int c0 = block % col_tiles * 64;
+    const E *src = (const E *)a.src[which];
+    const int c = (threadIdx.x & 7) * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int lr = i * 32 + (threadIdx.x >> 3);
+        const long r = r0 + lr;
+        const E *p = src + r * a.cols + c0 + c;
+        V x = {};
+        if (r < rows && c0 + c + 8 <= a.cols) x = *(const V *)p;
+        else if (r < rows)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c0 + c + e < a.cols) x[e] = p[e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_x[lr][c + e] = x[e];
+    }
+    __syncthreads();
+    const int oc = threadIdx.x >> 2, orow = (threadIdx.x & 3) * 16;
+    if (c0 + oc >= a.cols) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const long r = r0 + orow + h * 8;
+        if (r >= pitch) break;
+        E v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = s_x[orow + h * 8 + e][oc];
+        Frag<bf16_t> parts[P];
+        cut<P, bf16_t>(v, parts);
+#pragma unroll
+        for (int p = 0; p < P; ++p) *(bf16x8 *)(a.dst[which] + p * a.cols * pitch + (r / KT * a.cols + c0 + oc) * KT + r % KT) = parts[p];
+    }
+}
+
+// Both gradients in one launch, the codebook's workgroups first (they run longer).  PG: parts of the logits' gradient.  For
+// results of 16 bits two are enough where sums are long: they leave 2^-17 of a value out, and an fp32 sum of m products may be
+// off by m 2^-24 of their magnitudes by itself, which is as much from m = 128 on; either is far below the result's own
+// rounding, 2^-9 or 2^-12.
+template <typename E, int PG, int P, int MT, int NT>
 __global__ __launch_bounds__(CL_THREADS, 2) void grads_kernel(ProductArgs code, int code_blocks, ProductArgs x) {
-    __shared__ __attribute__((aligned(16))) char lds[tile_lds<GRAD_X, P, NT>()];
-    if ((int)blockIdx.x < code_blocks) product_tile<GRAD_CODE, float, E, 3, P, bf16_t, MT, NT, E>(code, blockIdx.x, lds);
-    else product_tile<GRAD_X, float, E, 3, P, bf16_t, MT, NT, E>(x, blockIdx.x - code_blocks, lds);
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds<GRAD_X, E, P, NT>()];
+    if ((int)blockIdx.x < code_blocks) product_tile<GRAD_CODE, float, E, PG, P, bf16_t, MT, NT, E>(code, blockIdx.x, lds);
+    else product_tile<GRAD_X, float, E, PG, P, bf16_t, MT, NT, E>(x, blockIdx.x - code_blocks, lds);
 }
 
 // Joins the splits' partial sums in a fixed order: 64 neighbouring elements a workgroup, the splits dealt to its waves.
@@ -792,28 +899,10 @@ int launch_logits(hipStream_t stream, ProductArgs a) {
 }
 
 // code.out or x.out null: that gradient is not wanted
-template <typename E>
-int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
+template <typename E, int PG>
+int launch_grads(hipStream_t stream, const ProductArgs &code, const ProductArgs &x, Tile t, long code_blocks, long grid) {
     constexpr int P = grad_parts<E>();
-    if (t.mt == 0) {
-        code.tiles_m = ceil_div(code.rows, 16);
-        x.tiles_m = ceil_div(x.rows, 16);
-        code.tiles_n = x.tiles_n = ceil_div(x.cols, 16 * SMALL_NT);
-        const long code_blocks = code.out ? (long)code.splits * code.tiles_m * code.tiles_n : 0;
-        const long grid = code_blocks + (x.out ? (long)x.tiles_m * x.tiles_n : 0);
-        GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many codes for one call");
-        hipLaunchKernelGGL((grads_small_kernel<E, P>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x);
-        GDPSO_HIP(hipGetLastError());
-        return GDPSO_OK;
-    }
-    code.tiles_m = ceil_div(code.rows, 64 * t.mt);
-    code.tiles_n = ceil_div(code.cols, 16 * t.nt);
-    x.tiles_m = ceil_div(x.rows, 64 * t.mt);
-    x.tiles_n = code.tiles_n;
-    const long code_blocks = code.out ? (long)ceil_div(code.splits, 8) * 8 * code.tiles_m * code.tiles_n : 0;
-    const long grid = code_blocks + (x.out ? (long)ceil_div(x.tiles_m, 8) * 8 * x.tiles_n : 0);
-    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
-#define CL_GRADS(MT, NT) hipLaunchKernelGGL((grads_kernel<E, P, MT, NT>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x)
+#define CL_GRADS(MT, NT) hipLaunchKernelGGL((grads_kernel<E, PG, P, MT, NT>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x)
     if (t.mt == 2) {
         if (t.nt == 2) CL_GRADS(2, 2);
         else if (t.nt == 4) CL_GRADS(2, 4);
@@ -827,6 +916,27 @@ int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
 #undef CL_GRADS
     GDPSO_HIP(hipGetLastError());
     return GDPSO_OK;
+}
+template <typename E>
+int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
+    const bool small = t.mt == 0;
+    const int tile_m = small ? 16 : 64 * t.mt, tile_n = 16 * (small ? SMALL_NT : t.nt);
+    code.tiles_m = ceil_div(code.rows, tile_m);
+    x.tiles_m = ceil_div(x.rows, tile_m);
+    code.tiles_n = x.tiles_n = ceil_div(x.cols, tile_n);
+    // the larger form deals splits and row tiles to the XCDs in eights
+    const long splits = small ? code.splits : (code.splits + 7) / 8 * 8, row_tiles = small ? x.tiles_m : (x.tiles_m + 7) / 8 * 8;
+    const long code_blocks = code.out ? splits * code.tiles_m * code.tiles_n : 0;
+    const long grid = code_blocks + (x.out ? row_tiles * x.tiles_n : 0);
+    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
+    if (small) {
+        hipLaunchKernelGGL((grads_small_kernel<E, grad_parts<E>()>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x);
+        GDPSO_HIP(hipGetLastError());
+        return GDPSO_OK;
+    }
+    if constexpr (!is_f32<E>())
+        if (x.sum >= 128) return launch_grads<E, 2>(stream, code, x, t, code_blocks, grid);
+    return launch_grads<E, 3>(stream, code, x, t, code_blocks, grid);
 }
 
 int code_check(const char *what, int n, int d, int k, int dtype, float temperature) {
@@ -855,10 +965,42 @@ extern "C" int gdpso_code_logits(void *stream_, int n, int d, int k, const void 
     return rc;
 }
 
+namespace gdpso {
+namespace {
+// Workspace of the gradients: planes of the codebook and of the latents (as fp16 needs them, whatever the type), then the splits'
+// partial sums.  The small form has no planes.
+struct GradSpace {
+    size_t codes, latents, part, bytes;
+};
+inline long plane_pitch(long rows) { return (rows + KT - 1) / KT * KT; }
+inline GradSpace grad_space(int n, int d, int k) {
+    GradSpace s = {0, 0, 0, 0};
+    if (n <= 0) return s;
+    if (n > SMALL_ROWS) {
+        s.latents = (size_t)2 * d * plane_pitch(k) * 2;
+        s.part = s.latents + (size_t)2 * d * plane_pitch(n) * 2;
+    }
+    const int splits = code_splits(n, d, k);
+    s.bytes = s.part + (splits > 1 ? (size_t)splits * k * (d + 1) * sizeof(float) : 0);
+    return s;
+}
+template <typename E>
+int launch_planes(hipStream_t stream, const PlanesArgs &a, bool codes, bool latents) {
+    PlanesArgs b = a;
+    const int col_tiles = ceil_div(a.cols, 64);
+    b.first = codes ? ceil_div(a.rows[0], 64) * col_tiles : 0;
+    const long grid = b.first + (latents ? (long)ceil_div(a.rows[1], 64) * col_tiles : 0);
+    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
+    hipLaunchKernelGGL((planes_kernel<E, grad_parts<E>()>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, b);
+    GDPSO_HIP(hipGetLastError());
+    return GDPSO_OK;
+}
+}  // namespace
+}  // namespace gdpso
+
 extern "C" size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k) {
     if (n <= 0 || d <= 0 || k <= 0) return 0;
-    const int splits = code_splits(n, d, k);
-    return splits > 1 ? (size_t)splits * k * (d + 1) * sizeof(float) : 0;
+    return grad_space(n, d, k).bytes;
 }
 
 extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const float *grad_logits, const void *inputs, const void *codebook, int dtype,
@@ -867,28 +1009,39 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
     if (rc) return rc;
     GDPSO_REQUIRE(n == 0 || (grad_logits && inputs), "code_logits_grad: null argument");
     GDPSO_REQUIRE(codebook, "code_logits_grad: null argument");
-    const size_t need = grad_codebook ? gdpso_code_logits_grad_workspace_bytes(n, d, k) : 0;
-    GDPSO_REQUIRE(need == 0 || workspace, "code_logits_grad: null workspace");
-    if (workspace_bytes < need)
-        return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
+    const GradSpace space = grad_space(n, d, k);
+    GDPSO_REQUIRE(space.bytes == 0 || workspace, "code_logits_grad: null workspace");
+    if (workspace_bytes < space.bytes) return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     const float scale = 2.f / temperature;
     const int splits = code_splits(n, d, k);
+    float *part = (float *)((char *)workspace + space.part);
     if (n > 0 && (grad_inputs || grad_codebook)) {
         const long per = ceil_div(ceil_div(n, splits), KT) * (long)KT;
-        const ProductArgs code = {grad_logits, inputs, splits > 1 && grad_codebook ? workspace : grad_codebook, k, d, n, k, d, 0, 0, splits, per, scale, codebook};
-        const ProductArgs x = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale, nullptr};
+        ProductArgs code = {grad_logits, inputs, splits > 1 && grad_codebook ? part : grad_codebook, k, d, n, k, d, 0, 0, splits, per, scale, codebook};
+        ProductArgs x = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale, nullptr};
+        if (n > SMALL_ROWS && dtype != DT_F32) {
+            const PlanesArgs planes = {{codebook, inputs}, {(bf16_t *)workspace, (bf16_t *)((char *)workspace + space.latents)}, {k, n},
+                                       {plane_pitch(k), plane_pitch(n)}, d, 0};
+            rc = dtype == DT_BF16 ? launch_planes<bf16_t>(stream, planes, grad_inputs != nullptr, grad_codebook != nullptr)
+                                  : launch_planes<f16_t>(stream, planes, grad_inputs != nullptr, grad_codebook != nullptr);
+            if (rc) return rc;
+            x.n = planes.dst[0];
+            x.ld_n = planes.pitch[0];
+            code.n = planes.dst[1];
+            code.ld_n = planes.pitch[1];
+        }
         GDPSO_WITH_DTYPE(dtype, rc = launch_grads<E>(stream, code, x, grad_tile(n, d, k)));
         if (rc) return rc;
     }
     if (grad_codebook && splits != 1) {  // no rows: zeros
         const dim3 grid(ceil_div((long)k * d, 64));
         if (splits > 64)  // many splits of few elements: more waves a workgroup
-            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 16>), grid, dim3(64 * 16), 0, stream, d, k, splits, (const float *)workspace,
-                                                       (const E *)codebook, scale, (E *)grad_codebook));
+            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 16>), grid, dim3(64 * 16), 0, stream, d, k, splits, part, (const E *)codebook, scale,
+                                                       (E *)grad_codebook));
         else
-            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 4>), grid, dim3(64 * 4), 0, stream, d, k, splits, (const float *)workspace,
-                                                       (const E *)codebook, scale, (E *)grad_codebook));
+            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 4>), grid, dim3(64 * 4), 0, stream, d, k, splits, part, (const E *)codebook, scale,
+                                                       (E *)grad_codebook));
         GDPSO_HIP(hipGetLastError());
     }
     return GDPSO_OK;

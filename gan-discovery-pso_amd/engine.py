@@ -422,7 +422,7 @@ def code_logits_grad(grad_logits: torch.Tensor, inputs: torch.Tensor, codebook: 
     dx = torch.empty(inputs.shape, dtype=x.dtype, device=device) if want_inputs else None
     dcb = torch.empty((k, d), dtype=x.dtype, device=device) if want_codebook else None
     L = _lib.lib()
-    size = L.gdpso_code_logits_grad_workspace_bytes(n, d, k) if want_codebook else 0
+    size = L.gdpso_code_logits_grad_workspace_bytes(n, d, k)
     ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.run(device, L.gdpso_code_logits_grad, n, d, k, g.data_ptr(), x.data_ptr(), cb.data_ptr(), dtype, temperature, ptr(dx), ptr(dcb), ptr(ws), size)
     return dx, dcb

@@ -369,8 +369,8 @@ int gdpso_vq_nearest_static(void *stream, int n, int d, int k, const float *inpu
  * gdpso_vq_nearest finds.  gdpso_code_logits_grad: given d loss / d logits (fp32 [n, k]), the gradients
  *   grad_inputs[i]   = (2 / t) sum_c g[i,c] code_c
  *   grad_codebook[c] = (2 / t) (sum_i g[i,c] x_i - code_c sum_i g[i,c])
- * in `dtype`; either may be NULL.  d <= 4096, k <= 2^20, temperature in [1e-6, 1e6].  The workspace
- * (gdpso_code_logits_grad_workspace_bytes) is needed for grad_codebook only. */
+ * in `dtype`; either may be NULL.  d <= 4096, k <= 2^20, temperature in [1e-6, 1e6].  Workspace:
+ * gdpso_code_logits_grad_workspace_bytes, 16-byte aligned (0 bytes: may be NULL). */
 int gdpso_code_logits(void *stream, int n, int d, int k, const void *inputs, const void *codebook, int dtype, float temperature,
                       float *logits);
 size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k);

@@ -41,9 +41,9 @@ def test_code_logits_refusals(h):
                 dict(t=float("inf")), dict(x=None), dict(c=None), dict(out=None)):
         assert call(**bad) == ARG, bad
     assert call(n=0, x=None, out=None) == 0
-    ws = h.gdpso_code_logits_grad_workspace_bytes(4000, 8, 3)
+    ws = h.gdpso_code_logits_grad_workspace_bytes(5000, 8, 3)
 
-    def grad(n=4000, d=8, k=3, g=P, x=P, c=P, dt=0, t=1.0, dx=P, dc=P, w=P, wb=ws):
+    def grad(n=5000, d=8, k=3, g=P, x=P, c=P, dt=0, t=1.0, dx=P, dc=P, w=P, wb=ws):
         return h.gdpso_code_logits_grad(None, n, d, k, g, x, c, dt, t, dx, dc, w, wb)
 
     for bad in (dict(n=-1), dict(d=0), dict(k=0), dict(dt=-1), dict(t=0.0), dict(g=None), dict(x=None), dict(c=None), dict(w=None)):
