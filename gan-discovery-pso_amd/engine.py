@@ -370,6 +370,9 @@ def vq_seed_codebook(codebook: torch.Tensor, positions: torch.Tensor, row0: int 
 _LOGIT_CODES = {torch.float32: _lib.DTYPES["f32"], torch.bfloat16: _lib.DTYPES["bf16"], torch.float16: _lib.DTYPES["f16"]}
 
 
+_MAX_INT = 2 ** 31  # sizes cross the C ABI as int, which ctypes would wrap around
+
+
 def _cuda_device(t: torch.Tensor, **others):
     """The device of ``t``, on which all the others (None aside) have to be."""
     device = t.device
@@ -398,6 +401,8 @@ def _code_args(inputs: torch.Tensor, codebook: torch.Tensor, **others):
     dtype = _LOGIT_CODES.get(inputs.dtype)
     if dtype is None or codebook.dtype != inputs.dtype:
         raise ValueError(f"inputs and codebook must share one of float32, bfloat16, float16 (got {inputs.dtype} and {codebook.dtype})")
+    if inputs.numel() // d >= _MAX_INT or k >= _MAX_INT:
+        raise ValueError("2^31 rows or more in one call")
     return device, _matrix(inputs, d), _matrix(codebook, d), k, d, dtype
 
 
@@ -443,6 +448,8 @@ def _loss_rows(logits: torch.Tensor, mask, **others):
     if rows.stride(1) != 1 and e > 1:
         rows = rows.detach().contiguous()
     n = rows.shape[0]
+    if n >= _MAX_INT or e >= _MAX_INT:
+        raise ValueError("2^31 rows or columns, or more, in one call")
     stride = rows.stride(0) if n > 1 else e
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != shape[:-1]:

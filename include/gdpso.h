@@ -362,7 +362,7 @@ int gdpso_vq_nearest_static(void *stream, int n, int d, int k, const float *inpu
  * device, row-major; `dtype` (GDPSO_DTYPE_*) is the type of latents and codebook, or of the logits and their gradient.
  * Sums, softmax statistics and code logits are fp32; a gradient is rounded once, when it is stored.  No call
  * allocates, synchronises or reads anything back, so all can be captured into a HIP graph; results do not depend on the
- * order in which workgroups run.
+ * order in which workgroups run.  Workspaces are 16-byte aligned; two calls that may overlap need one each.
  *
  * gdpso_code_logits: logits[i,c] = (2 <x_i, code_c> - |code_c|^2) / temperature, fp32 [n, k]: minus the squared distance
  * over the temperature up to a constant per row, so softmax over the codes is the soft assignment whose maximum
@@ -370,7 +370,7 @@ int gdpso_vq_nearest_static(void *stream, int n, int d, int k, const float *inpu
  *   grad_inputs[i]   = (2 / t) sum_c g[i,c] code_c
  *   grad_codebook[c] = (2 / t) (sum_i g[i,c] x_i - code_c sum_i g[i,c])
  * in `dtype`; either may be NULL.  d <= 4096, k <= 2^20, temperature in [1e-6, 1e6].  Workspace:
- * gdpso_code_logits_grad_workspace_bytes, 16-byte aligned (0 bytes: may be NULL). */
+ * gdpso_code_logits_grad_workspace_bytes (0 bytes: may be NULL). */
 int gdpso_code_logits(void *stream, int n, int d, int k, const void *inputs, const void *codebook, int dtype, float temperature,
                       float *logits);
 size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k);

@@ -435,6 +435,41 @@ def test_autograd_forms(eng, fn):
         assert torch.equal(logits.grad, ref[2])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,k", [(40, 3000, 6), (3, 70000, 300), (9, 200003, 16), (200, 17000, 5)])
+def test_distill_backward_of_long_rows(fn, n, v, k, dtype):
+    """The backward pass reads the statistics of the forward pass, whichever way the rows were held there."""
+    logits = rand(n, n, v, scale=2.0, dtype=dtype)
+    t_logits, t_idx = teacher_of(logits, k, 3)
+    logits[0] = -math.inf
+    t_idx[1, 1:] = t_idx[1, 0]
+    t_idx[2, 0] = -1
+    mask = torch.ones(n, dtype=torch.bool, device=DEV)
+    mask[n // 2] = False
+    logits[n // 2] = math.nan if n > 8 else 0.0
+    clean = logits.clone()
+    clean[n // 2] = 0
+    leaf = logits.clone().requires_grad_()
+    loss = fn.distill(leaf, t_logits, t_idx, mask, 1.5)
+    (float(n) * loss).backward()
+    want = distill64(clean, t_logits, t_idx, mask, 1.5, float(n))
+    assert_within(loss, want[0], want[3] + store_error(want[0], torch.float32), "loss")
+    assert_within(leaf.grad, want[2], want[5] + store_error(want[2], dtype), "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,e,k", [(300, 5000, 2), (70, 1500, 1), (9000, 24, 3)])
+def test_balance_backward(fn, n, e, k, dtype):
+    logits = rand(n, n, e, scale=2.0, dtype=dtype).requires_grad_()
+    idx, mask = randint(3, 0, e, n, k), randint(4, 0, 5, n) > 0
+    loss, counts, _ = fn.balance(logits, idx, mask)
+    (float(n) * loss).backward()
+    want = balance64(logits.detach(), idx, mask, float(n))
+    assert torch.equal(counts.cpu(), want[1])
+    assert_within(loss, want[0], want[4] + store_error(want[0], torch.float32), "loss")
+    assert_within(logits.grad, want[3], want[6] + store_error(want[3], dtype), "grad")
+
+
 def test_gradients_against_differences(eng):
     """Central differences of the definitions in 64 bits."""
     n, e = 6, 9

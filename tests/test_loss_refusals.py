@@ -107,6 +107,17 @@ def test_python_balance(eng):
             eng.balance_grad(s, counts, totals, u)
 
 
+def test_python_sizes_beyond_int(eng):
+    """Rows beyond 2^31 would wrap around in the C ABI's int (strides of 0: no memory behind them)."""
+    n = 2 ** 31 + 3
+    with pytest.raises(ValueError):
+        eng.code_logits(torch.zeros(1, 1).expand(n, 1), torch.zeros(1, 1))
+    with pytest.raises(ValueError):
+        eng.balance(torch.zeros(1, 2).expand(n, 2), torch.zeros(1, dtype=torch.int64).expand(n))
+    with pytest.raises(ValueError):
+        eng.distill(torch.zeros(1, 2).expand(n, 2), torch.zeros(1, 1).expand(n, 1), torch.zeros(1, 1, dtype=torch.int64).expand(n, 1))
+
+
 def test_python_distill(eng):
     s, t, i = torch.zeros(4, 8), torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int64)
     for a, b, c, m in ((s.double(), t, i, None), (s, t.double(), i, None), (s, t[:, :1], i, None), (s, t, i.short(), None), (s, t[:3], i[:3], None),
