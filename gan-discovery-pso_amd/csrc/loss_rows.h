@@ -145,7 +145,8 @@ struct RowRegs {
         }
         return l;
     }
-    // row[c] = f(logit)
+    // row[c] = f(logit), past the caches: a long row's gradient is not read again before later rows have pushed it out
+    // (8192 x 50007 bf16: 412 us, 408 with `clear` alone so, 401 with both)
     template <typename F>
     __device__ __forceinline__ void map(E *__restrict__ row, int e, int pos, F f) const {
         static_assert(TAIL, "rows with a tail");
@@ -156,7 +157,7 @@ struct RowRegs {
             V x;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) x[v] = (E)f(at(j, v));
-            if (c + VEC <= e) *(V *)(row + c) = x;
+            if (c + VEC <= e) __builtin_nontemporal_store(x, (V *)(row + c));
         }
         const int whole = e / VEC * VEC;
         if (whole + pos < e) row[whole + pos] = (E)f((float)tail);
@@ -166,7 +167,7 @@ struct RowRegs {
 #pragma unroll 1
         for (int j = 0; j < NCH; ++j) {
             const int c = column(j, pos);
-            if (c + VEC <= e) *(V *)(row + c) = V{};
+            if (c + VEC <= e) __builtin_nontemporal_store(V{}, (V *)(row + c));
             else
 #pragma unroll
                 for (int v = 0; v < VEC; ++v)
