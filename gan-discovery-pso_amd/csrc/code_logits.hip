@@ -314,7 +314,7 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __buil
 
 struct ProductArgs {
     const void *m, *n;  // operands: output rows' side and output columns' side
-    void *out;          // result; GRAD_CODE with several splits: partial sums, float [split][rows * cols + rows]
+    void *out;          // result; with several splits partial sums, float [split][rows * cols + rows] (GRAD_X: [rows * cols])
     long rows, cols, sum;
     long ld_m, ld_n;    // ld_n: GRAD_*: pitch of the planes, whose size is cols * ld_n
     int tiles_m, tiles_n, splits;
@@ -370,9 +370,10 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
         tn = slot % per / a.tiles_m;
         if (split >= a.splits) return;
     } else {
-        split = 0;
-        tm = slot / a.tiles_n * 8 + xcd;
-        tn = slot % a.tiles_n;
+        const int per = a.tiles_n * a.splits, rest = slot % per;
+        tm = slot / per * 8 + xcd;
+        tn = rest % a.tiles_n;
+        split = rest / a.tiles_n;
         if (tm >= a.tiles_m) return;
     }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -482,15 +483,15 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
             sum_m[i] += __shfl_xor(sum_m[i], 32, 64);
         }
     }
-    const bool part = OP == GRAD_CODE && a.splits > 1;
-    float *partial = (float *)a.out + split * (a.rows * a.cols + a.rows);
+    const bool part = OP != LOGITS && a.splits > 1;
+    float *partial = (float *)a.out + split * (a.rows * a.cols + (OP == GRAD_CODE ? a.rows : 0));
     // A lane holds four consecutive columns of one row of each 16 x 16 tile.
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         bool mine;
         const long m = OpM::held(m0, a.rows, i, fr, mine);
         if (!mine) continue;
-        if (part && tn == 0 && lane < 16) partial[a.rows * a.cols + m] = sum_m[i];
+        if (OP == GRAD_CODE && part && tn == 0 && lane < 16) partial[a.rows * a.cols + m] = sum_m[i];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int nl = j * 16 + (lane >> 4) * 4;
@@ -500,7 +501,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, const int blo
             for (int e = 0; e < 4; ++e) {
                 x[e] = acc[i][j][e];
                 if constexpr (OP == LOGITS) x[e] = fmaf(2.f, x[e], -s_norm[nl + e]) * a.scale;
-                if constexpr (OP == GRAD_X) x[e] *= a.scale;
+                if constexpr (OP == GRAD_X) x[e] *= part ? 1.f : a.scale;
                 if constexpr (OP == GRAD_CODE)
                     if (!part && n + e < a.cols) x[e] = a.scale * fmaf(-sum_m[i], (float)((const EN *)a.code)[m * a.cols + n + e], x[e]);
             }
@@ -796,7 +797,7 @@ __global__ __launch_bounds__(CL_THREADS) void planes_kernel(PlanesArgs a) {
 }
 
 // Both gradients in one launch, the codebook's workgroups first (they run longer).  PG: parts of the logits' gradient.  For
-// results of 16 bits two are enough where sums are long: they leave 2^-17 of a value out, and an fp32 sum of m products may be
+// results of 16 bits two are enough where both sums are long: they leave 2^-17 of a value out, and an fp32 sum of m products may be
 // off by m 2^-24 of their magnitudes by itself, which is as much from m = 128 on; either is far below the result's own
 // rounding, 2^-9 or 2^-12.
 template <typename E, int PG, int P, int MT, int NT>
@@ -806,20 +807,51 @@ __global__ __launch_bounds__(CL_THREADS, 2) void grads_kernel(ProductArgs code, 
     else product_tile<GRAD_X, float, E, PG, P, bf16_t, MT, NT, E>(x, blockIdx.x - code_blocks, lds);
 }
 
-// Joins the splits' partial sums in a fixed order: 64 neighbouring elements a workgroup, the splits dealt to its waves.
+// Joins the splits' partial sums in a fixed order.  The codebook's gradient: 64 neighbouring elements a workgroup, the splits
+// dealt to its waves.  Behind its workgroups those of the latents' gradient, whose splits are few: four elements a thread.
+struct JoinArgs {
+    int d, k, splits, x_splits;
+    const float *part, *x_part;
+    const void *code;
+    float scale;
+    void *dcode, *dx;
+    long x_size;
+    int code_blocks;
+};
 template <typename E, int JOIN_WAVES>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void code_join_kernel(int d, int k, int splits, const float *__restrict__ part, const E *__restrict__ cb,
-                                                                    float scale, E *__restrict__ dcode) {
+__global__ __launch_bounds__(64 * JOIN_WAVES) void join_kernel(JoinArgs a) {
     __shared__ float s_acc[JOIN_WAVES][64], s_sum[JOIN_WAVES][64];
+    if ((int)blockIdx.x >= a.code_blocks) {
+        const long e = (((long)blockIdx.x - a.code_blocks) * (64 * JOIN_WAVES) + threadIdx.x) * 4;
+        if (e >= a.x_size) return;
+        float x[4] = {};
+        if (e + 4 <= a.x_size) {
+#pragma unroll 4
+            for (int s = 0; s < a.x_splits; ++s) {
+                const auto v = *(const typename VecAt<float, 4>::type *)(a.x_part + s * a.x_size + e);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] += v[c];
+            }
+        } else {
+            for (int s = 0; s < a.x_splits; ++s)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (e + c < a.x_size) x[c] += a.x_part[s * a.x_size + e + c];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] *= a.scale;
+        put4((E *)a.dx, e, a.x_size, x);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long size = (long)k * d, e = (long)blockIdx.x * 64 + lane;
+    const long size = (long)a.k * a.d, e = (long)blockIdx.x * 64 + lane;
     float acc = 0.f, sum = 0.f;
     if (e < size) {
-        const float *p = part + e, *ps = part + size + e / d;
+        const float *p = a.part + e, *ps = a.part + size + e / a.d;
 #pragma unroll 8
-        for (int s = wave; s < splits; s += JOIN_WAVES) {
-            acc += p[s * (size + k)];
-            sum += ps[s * (size + k)];
+        for (int s = wave; s < a.splits; s += JOIN_WAVES) {
+            acc += p[s * (size + a.k)];
+            sum += ps[s * (size + a.k)];
         }
     }
     s_acc[wave][lane] = acc;
@@ -830,7 +862,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void code_join_kernel(int d, int k
             acc += s_acc[w][lane];
             sum += s_sum[w][lane];
         }
-        dcode[e] = (E)(scale * fmaf(-sum, (float)cb[e], acc));
+        ((E *)a.dcode)[e] = (E)(a.scale * fmaf(-sum, (float)((const E *)a.code)[e], acc));
     }
 }
 
@@ -839,27 +871,46 @@ constexpr int grad_parts() {
     return is_f32<E>() ? 3 : (__is_same(E, f16_t) ? 2 : 1);
 }
 
-// Gradient tiles of 64 MT rows by 16 NT columns, all d columns in one tile up to 256: the rows' operand, the large one, is then
-// read and cut once.  {0, 0}: the small form.
+// Gradient tiles of 64 MT rows by 16 NT columns.  {0, 0}: the small form, while its sixteenfold reading of both operands costs less than
+// the longer run through larger tiles (fp32, small and large: 512 x 1024 x 256 14 and 31 us, 2048 x 512 x 256 26 and 30,
+// 4096 x 1024 x 64 27 and 21, 4096 x 1024 x 256 81 and 49).
+//
+// All columns in one tile up to 128, 16-bit types 256: the rows' operand, the large one, is read and cut once.  With fp32's three parts
+// 256 columns leave one wave a SIMD and are read from LDS more than the matrix instructions hide: two tiles of 128 (50000 x 512 x 256:
+// 290 us in one, 171 so).  128 rows once they fill the chip or the products are large (fp32, 64 and 128 rows: 8192 x 512 x 256 46 and
+// 56 us, 32000 x 512 x 256 136 and 109, 8192 x 8192 x 64 201 and 139); the tile of 256 columns later (bf16: 20000 x 2048 x 256 134
+// and 140 us, 50000 x 2048 x 256 294 and 272, 20000 x 8192 x 256 615 and 406; fp16's two parts would spill).  `parts` of a code: 3 for fp32,
+// 2 for fp16, 1 for bf16.
 constexpr int SMALL_ROWS = 4096;
 struct Tile {
     int mt, nt;
 };
-inline Tile grad_tile(int n, int d, int k) {
-    if (n <= SMALL_ROWS) return {0, 0};
-    const int nt = d <= 32 ? 2 : (d <= 64 ? 4 : (d <= 128 ? 8 : 16));
-    // 128 rows a workgroup once they fill the chip; 256 columns leave registers for 64
-    return {nt < 16 && n >= 32768 && k > 1 ? 2 : 1, nt};
+inline Tile grad_tile(int n, int d, int k, int parts) {
+    const double work = (double)n * k * d;
+    if (n <= SMALL_ROWS && work < 0x1p28) return {0, 0};
+    const int nt = d <= 32 ? 2 : (d <= 64 ? 4 : (d <= 128 || parts == 3 ? 8 : 16));
+    const bool large = nt == 16 ? parts == 1 && work >= 0x1p34 : n >= 32768 || work >= 0x3p30;
+    return {large && k > 1 ? 2 : 1, nt};
 }
+inline bool small_form(int n, int d, int k) { return grad_tile(n, d, k, 3).mt == 0; }
 // Splits of the summed rows of the codebook's gradient.  Small: 512 rows, four stages a wave, and up to there one split does
 // without the join's launch.  Else about two workgroups a CU, at least 128 rows each (the partial sums that a split writes
 // and the join reads have to stay small beside its rows).
-inline int code_splits(int n, int d, int k) {
-    if (n <= SMALL_ROWS) return ceil_div(n, 512);
-    const Tile t = grad_tile(n, d, k);
+inline int code_splits(int n, int d, int k, int parts) {
+    if (small_form(n, d, k)) return ceil_div(n, 512);
+    const Tile t = grad_tile(n, d, k, parts);
     const long tiles = (long)ceil_div(k, 64 * t.mt) * ceil_div(d, 16 * t.nt);
     const long want = ceil_div(512, tiles), most = ceil_div(n, 128);
     return (int)(want < most ? want : most);
+}
+// Splits of the summed codes of the latents' gradient, where row tiles alone leave the chip idle: about two workgroups a CU, and the
+// partial sums, written and read again, stay smaller than the share of the logits' gradient that they are made of.
+inline int x_splits(int n, int d, int k, int parts) {
+    if (small_form(n, d, k)) return 1;
+    const Tile t = grad_tile(n, d, k, parts);
+    const long tiles = (long)ceil_div(n, 64 * t.mt) * ceil_div(d, 16 * t.nt);
+    const long want = 512 / tiles, most = k / std::max(128, 2 * d);
+    return (int)std::max(1l, std::min(want, most));
 }
 
 template <typename E>
@@ -906,12 +957,13 @@ int launch_grads(hipStream_t stream, const ProductArgs &code, const ProductArgs 
     if (t.mt == 2) {
         if (t.nt == 2) CL_GRADS(2, 2);
         else if (t.nt == 4) CL_GRADS(2, 4);
-        else CL_GRADS(2, 8);
+        else if (t.nt == 8) CL_GRADS(2, 8);
+        else if constexpr (P == 1) CL_GRADS(2, 16);
     } else {
         if (t.nt == 2) CL_GRADS(1, 2);
         else if (t.nt == 4) CL_GRADS(1, 4);
         else if (t.nt == 8) CL_GRADS(1, 8);
-        else CL_GRADS(1, 16);
+        else if constexpr (!is_f32<E>()) CL_GRADS(1, 16);
     }
 #undef CL_GRADS
     GDPSO_HIP(hipGetLastError());
@@ -925,7 +977,7 @@ int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
     x.tiles_m = ceil_div(x.rows, tile_m);
     code.tiles_n = x.tiles_n = ceil_div(x.cols, tile_n);
     // the larger form deals splits and row tiles to the XCDs in eights
-    const long splits = small ? code.splits : (code.splits + 7) / 8 * 8, row_tiles = small ? x.tiles_m : (x.tiles_m + 7) / 8 * 8;
+    const long splits = small ? code.splits : (code.splits + 7) / 8 * 8, row_tiles = small ? x.tiles_m : (x.tiles_m + 7) / 8 * 8 * x.splits;
     const long code_blocks = code.out ? splits * code.tiles_m * code.tiles_n : 0;
     const long grid = code_blocks + (x.out ? row_tiles * x.tiles_n : 0);
     GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
@@ -935,7 +987,7 @@ int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
         return GDPSO_OK;
     }
     if constexpr (!is_f32<E>())
-        if (x.sum >= 128) return launch_grads<E, 2>(stream, code, x, t, code_blocks, grid);
+        if (x.sum >= 128 && code.sum >= 128) return launch_grads<E, 2>(stream, code, x, t, code_blocks, grid);
     return launch_grads<E, 3>(stream, code, x, t, code_blocks, grid);
 }
 
@@ -967,21 +1019,22 @@ extern "C" int gdpso_code_logits(void *stream_, int n, int d, int k, const void 
 
 namespace gdpso {
 namespace {
-// Workspace of the gradients: planes of the codebook and of the latents (as fp16 needs them, whatever the type), then the splits'
+// Workspace of the gradients: planes of the codebook and of the latents (16-bit types, two parts as fp16 needs them), then the splits'
 // partial sums.  The small form has no planes.
 struct GradSpace {
-    size_t codes, latents, part, bytes;
+    size_t latents, part, x_part, bytes;  // offsets; the codebook's planes come first
 };
 inline long plane_pitch(long rows) { return (rows + KT - 1) / KT * KT; }
-inline GradSpace grad_space(int n, int d, int k) {
+inline GradSpace grad_space(int n, int d, int k, int parts) {
     GradSpace s = {0, 0, 0, 0};
     if (n <= 0) return s;
-    if (n > SMALL_ROWS) {
+    if (parts < 3 && !small_form(n, d, k)) {
         s.latents = (size_t)2 * d * plane_pitch(k) * 2;
         s.part = s.latents + (size_t)2 * d * plane_pitch(n) * 2;
     }
-    const int splits = code_splits(n, d, k);
-    s.bytes = s.part + (splits > 1 ? (size_t)splits * k * (d + 1) * sizeof(float) : 0);
+    const int splits = code_splits(n, d, k, parts), xs = x_splits(n, d, k, parts);
+    s.x_part = s.part + (splits > 1 ? (size_t)splits * k * (d + 1) * sizeof(float) : 0);
+    s.bytes = s.x_part + (xs > 1 ? (size_t)xs * n * d * sizeof(float) : 0);
     return s;
 }
 template <typename E>
@@ -1000,7 +1053,7 @@ int launch_planes(hipStream_t stream, const PlanesArgs &a, bool codes, bool late
 
 extern "C" size_t gdpso_code_logits_grad_workspace_bytes(int n, int d, int k) {
     if (n <= 0 || d <= 0 || k <= 0) return 0;
-    return grad_space(n, d, k).bytes;
+    return std::max({grad_space(n, d, k, 1).bytes, grad_space(n, d, k, 2).bytes, grad_space(n, d, k, 3).bytes});  // whatever the type
 }
 
 extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const float *grad_logits, const void *inputs, const void *codebook, int dtype,
@@ -1009,18 +1062,20 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
     if (rc) return rc;
     GDPSO_REQUIRE(n == 0 || (grad_logits && inputs), "code_logits_grad: null argument");
     GDPSO_REQUIRE(codebook, "code_logits_grad: null argument");
-    const GradSpace space = grad_space(n, d, k);
+    const int parts = dtype == DT_F32 ? 3 : (dtype == DT_F16 ? 2 : 1);
+    const GradSpace space = grad_space(n, d, k, parts);
     GDPSO_REQUIRE(space.bytes == 0 || workspace, "code_logits_grad: null workspace");
     if (workspace_bytes < space.bytes) return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     const float scale = 2.f / temperature;
-    const int splits = code_splits(n, d, k);
-    float *part = (float *)((char *)workspace + space.part);
+    const int splits = code_splits(n, d, k, parts), xs = x_splits(n, d, k, parts);
+    float *const part = (float *)((char *)workspace + space.part), *const x_part = (float *)((char *)workspace + space.x_part);
     if (n > 0 && (grad_inputs || grad_codebook)) {
         const long per = ceil_div(ceil_div(n, splits), KT) * (long)KT;
         ProductArgs code = {grad_logits, inputs, splits > 1 && grad_codebook ? part : grad_codebook, k, d, n, k, d, 0, 0, splits, per, scale, codebook};
-        ProductArgs x = {grad_logits, codebook, grad_inputs, n, d, k, k, d, 0, 0, 1, ceil_div(k, KT) * (long)KT, scale, nullptr};
-        if (n > SMALL_ROWS && dtype != DT_F32) {
+        const long x_per = ceil_div(ceil_div(k, xs), KT) * (long)KT;
+        ProductArgs x = {grad_logits, codebook, xs > 1 && grad_inputs ? x_part : grad_inputs, n, d, k, k, d, 0, 0, xs, x_per, scale, nullptr};
+        if (parts < 3 && !small_form(n, d, k)) {
             const PlanesArgs planes = {{codebook, inputs}, {(bf16_t *)workspace, (bf16_t *)((char *)workspace + space.latents)}, {k, n},
                                        {plane_pitch(k), plane_pitch(n)}, d, 0};
             rc = dtype == DT_BF16 ? launch_planes<bf16_t>(stream, planes, grad_inputs != nullptr, grad_codebook != nullptr)
@@ -1031,17 +1086,19 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
             code.n = planes.dst[1];
             code.ld_n = planes.pitch[1];
         }
-        GDPSO_WITH_DTYPE(dtype, rc = launch_grads<E>(stream, code, x, grad_tile(n, d, k)));
+        GDPSO_WITH_DTYPE(dtype, rc = launch_grads<E>(stream, code, x, grad_tile(n, d, k, parts)));
         if (rc) return rc;
     }
-    if (grad_codebook && splits != 1) {  // no rows: zeros
-        const dim3 grid(ceil_div((long)k * d, 64));
-        if (splits > 64)  // many splits of few elements: more waves a workgroup
-            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 16>), grid, dim3(64 * 16), 0, stream, d, k, splits, part, (const E *)codebook, scale,
-                                                       (E *)grad_codebook));
+    const bool join_code = grad_codebook && splits != 1, join_x = grad_inputs && xs > 1;  // no rows: zeros
+    if (join_code || join_x) {
+        const int waves = splits > 64 ? 16 : 4;  // many splits of few elements: more waves a workgroup
+        const long code_blocks = join_code ? ceil_div((long)k * d, 64) : 0, x_size = (long)n * d;
+        const long grid = code_blocks + (join_x ? ceil_div(x_size, 64 * 4 * waves) : 0);
+        const JoinArgs a = {d, k, splits, xs, part, x_part, codebook, scale, grad_codebook, grad_inputs, x_size, (int)code_blocks};
+        if (waves == 16)
+            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((join_kernel<E, 16>), dim3((unsigned)grid), dim3(64 * 16), 0, stream, a));
         else
-            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((code_join_kernel<E, 4>), grid, dim3(64 * 4), 0, stream, d, k, splits, part, (const E *)codebook, scale,
-                                                       (E *)grad_codebook));
+            GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((join_kernel<E, 4>), dim3((unsigned)grid), dim3(64 * 4), 0, stream, a));
         GDPSO_HIP(hipGetLastError());
     }
     return GDPSO_OK;

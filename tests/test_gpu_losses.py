@@ -69,7 +69,7 @@ def check_distill(out, logits, t_logits, t_idx, mask, t, scale):
 CODE_SIZES = [(1, 1, 1), (1, 512, 64), (5, 37, 3), (512, 256, 100), (67, 130, 257), (33, 1000, 16), (130, 8, 1030), (1025, 65, 33),
               (2049, 128, 128), (300, 129, 40), (7, 64, 4096), (5000, 70, 40), (5001, 130, 100), (4999, 66, 200), (5003, 40, 300), (33000, 64, 64),
               (32773, 65, 33), (40001, 130, 128), (32769, 31, 20), (5005, 50, 131), (4999, 66, 257), (33001, 257, 101),
-              (32770, 1, 65)]
+              (32770, 1, 65), (600, 2000, 257), (4099, 2005, 129), (4096, 3001, 66), (1000, 16411, 30), (33000, 129, 200), (6001, 2051, 300)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
