@@ -10,9 +10,14 @@
 // The products run on the 16-bit matrix instructions, sixteen times the rate of the fp32 ones, without giving up
 // fp32 accuracy: a value is cut into bf16 parts, each the rounded rest of the one before, so that an fp32 value is three
 // parts (3 x 8 bits), an fp16 value two, a bf16 value itself, and the product of two values is the sum of the products of
-// their parts.  Those of order 2^-24 and below are left out (two middle parts of order 2^-16 are kept): six matrix
-// instructions for fp32 x fp32, five for fp32 x fp16, three for fp32 x bf16.  Parts multiply exactly and add up in fp32.  The
-// forward product of two 16-bit operands needs no cutting.
+// their parts.  Those of order 2^-24 and below are left out: six matrix instructions for fp32 x fp32, five for fp32 x fp16,
+// three for fp32 x bf16; four and two where the logits' gradient may do with two parts (grads_kernel).  Parts multiply exactly and
+// add up in fp32.  The forward product of two 16-bit operands needs no cutting.
+//
+// What bounds them: the fp32 logits or their gradient, [n, k], against which latents and codes are small, and with fp32 operands the
+// matrix instructions as much.  Latents 65536 x 64, 512 codes, fp32: logits 35 us (134 MB written, 3.8 TB/s, and 26 GFLOP of bf16 products), both
+// gradients 65 and the join 5 (the same 134 MB read for each, 4.1 TB/s, and 52 GFLOP).  50007 x 256 and 1024 codes, bf16: logits 71 us
+// (205 MB, 2.9 TB/s), planes 13, gradients 150 (2 x 205 MB, 2.7 TB/s, and 105 GFLOP), join 8.
 #include "loss_rows.h"
 
 #include <algorithm>
@@ -919,11 +924,18 @@ int launch_logits(hipStream_t stream, ProductArgs a) {
     using M = std::conditional_t<is_f32<E>(), bf16_t, E>;
     const int stages = ceil_div(a.sum, KT);
     const bool held = stages <= (is_f32<E>() ? 4 : 8);
-    // 128 rows a workgroup once they fill the chip, else 64, and then several workgroups share a tile's codes
-    const int mt = a.rows >= 32768 ? 2 : 1, bn = held ? 64 : 128;
+    // 128 rows a workgroup from 8192 on, where 64 of them occupy the chip (fp32, 64 and 128 rows: 16000 x 256 x 100 19 and 13 us,
+    // 26000 x 512 x 256 57 and 50); below, 64, and always as many workgroups to a tile of rows as fill the chip twice, each with its
+    // share of the codes.  Many codes of up to two stages, where a workgroup's own start is short: four times, four tiles each at least (bf16, 65536 x 1024 x 64:
+    // 73 us twice, 56 four times; 65536 x 512 x 256 34 and 39).
+    const int mt = a.rows >= 8192 ? 2 : 1, bn = held ? 64 : 128;
     a.tiles_m = ceil_div(a.rows, 64 * mt);
     const int col_tiles = ceil_div(a.cols, bn);
-    a.tiles_n = held ? std::min(col_tiles, std::max(1, ceil_div(512, a.tiles_m))) : col_tiles;
+    a.tiles_n = col_tiles;
+    if (held) {
+        const int more = stages <= 2 && col_tiles >= 16 ? std::min(ceil_div(1024, a.tiles_m), col_tiles / 4) : 1;
+        a.tiles_n = std::min(col_tiles, std::max(ceil_div(512, a.tiles_m), more));
+    }
     const long grid = (long)ceil_div(a.tiles_m, 8) * 8 * a.tiles_n;
     GDPSO_REQUIRE(grid < (1l << 31), "code_logits: too many rows for one call");
 #define CL_LOGITS(NS)                                                                                                                        \
