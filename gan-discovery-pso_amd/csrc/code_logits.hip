@@ -1076,8 +1076,9 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
     GDPSO_REQUIRE(codebook, "code_logits_grad: null argument");
     const int parts = dtype == DT_F32 ? 3 : (dtype == DT_F16 ? 2 : 1);
     const GradSpace space = grad_space(n, d, k, parts);
-    GDPSO_REQUIRE(space.bytes == 0 || workspace, "code_logits_grad: null workspace");
-    if (workspace_bytes < space.bytes) return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
+    const size_t need = gdpso_code_logits_grad_workspace_bytes(n, d, k);
+    GDPSO_REQUIRE(need == 0 || workspace, "code_logits_grad: null workspace");
+    if (workspace_bytes < need) return fail(GDPSO_ERR_WORKSPACE, "code_logits_grad: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     const float scale = 2.f / temperature;
     const int splits = code_splits(n, d, k, parts), xs = x_splits(n, d, k, parts);
