@@ -122,7 +122,7 @@ template <typename E, int THREADS, int TEAM, int NCH, bool VALUE, bool GRAD>
 __global__ __launch_bounds__(THREADS) void dist_team_kernel(DistArgs a) {
     constexpr int VEC = vec_of<E>(), TEAMS = THREADS / TEAM, WORDS = (TEAM * NCH * VEC + 31) / 32;
     __shared__ unsigned s_bits[GRAD ? TEAMS : 1][GRAD ? WORDS : 1];
-    __shared__ double s_loss[VALUE ? TEAMS : 1];
+    __shared__ double s_loss[VALUE ? THREADS / 64 : 1];
     const int lane = threadIdx.x & 63, pos = threadIdx.x & (TEAM - 1), team = threadIdx.x / TEAM;
     const float inv = inv_kept<THREADS>(a);
     float factor = 0.f;
@@ -232,10 +232,11 @@ __global__ __launch_bounds__(THREADS) void dist_team_kernel(DistArgs a) {
         }
     }
     if constexpr (VALUE) {
-        if (pos == 0) s_loss[team] = sum;
+        for (int o = TEAM; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);  // a team's first lane holds its rows' sum
+        if (lane == 0) s_loss[threadIdx.x >> 6] = sum;
         __syncthreads();
         if (threadIdx.x == 0)
-            for (int w = 1; w < TEAMS; ++w) sum += s_loss[w];
+            for (int w = 1; w < THREADS / 64; ++w) sum += s_loss[w];
         finish_loss<THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
     }
 }

@@ -384,6 +384,10 @@ def _cuda_device(t: torch.Tensor, **others):
     return device
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _matrix(t: torch.Tensor, cols: int) -> torch.Tensor:
     """[..., cols] as contiguous rows; a copy only where the strides need one."""
     if t.dim() == 2 and t.is_contiguous():
@@ -424,8 +428,8 @@ def code_logits_grad(grad_logits: torch.Tensor, inputs: torch.Tensor, codebook: 
     if grad_logits.dtype != torch.float32 or grad_logits.shape != (*inputs.shape[:-1], k):
         raise ValueError(f"grad_logits must be float32 {(*inputs.shape[:-1], k)}, got {grad_logits.dtype} {tuple(grad_logits.shape)}")
     g = _matrix(grad_logits, k)
-    dx = torch.empty(inputs.shape, dtype=x.dtype, device=device) if want_inputs else None
-    dcb = torch.empty((k, d), dtype=x.dtype, device=device) if want_codebook else None
+    dx = _like(inputs) if want_inputs else None
+    dcb = _like(codebook) if want_codebook else None
     L = _lib.lib()
     size = L.gdpso_code_logits_grad_workspace_bytes(n, d, k)
     ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
@@ -476,7 +480,7 @@ def _balance(logits, indices, mask, grad_scale):
     loss = torch.empty((), dtype=torch.float32, device=device)
     counts = torch.empty(e, dtype=torch.int64, device=device)
     mean_prob = torch.empty(e, dtype=torch.float32, device=device)
-    grad = None if grad_scale is None else torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    grad = None if grad_scale is None else _like(logits)
     L = _lib.lib()
     size = L.gdpso_balance_workspace_bytes(n, e)
     ws = torch.empty((size + 7) // 8 + 2, dtype=torch.int64, device=device)  # two totals, then the call's workspace
@@ -503,7 +507,7 @@ def balance_grad(logits: torch.Tensor, counts: torch.Tensor, totals: torch.Tenso
             raise ValueError(f"{name} must be contiguous int64 [{size}]")
     if upstream.dtype != torch.float32 or upstream.numel() != 1:
         raise ValueError("upstream must be a float32 scalar")
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    grad = _like(logits)
     _lib.run(device, _lib.lib().gdpso_balance_grad, n, e, rows.data_ptr(), stride, dtype, ptr(mask), counts.data_ptr(), totals.data_ptr(),
              upstream.data_ptr(), grad.data_ptr())
     return grad
@@ -523,13 +527,14 @@ def _distill(logits, teacher_logits, teacher_indices, mask, temperature, grad_sc
     device, rows, n, v, stride, dtype, mask, k, idx, index_bytes, t, t_dtype = _distill_args(logits, teacher_logits, teacher_indices, mask)
     loss = torch.empty((), dtype=torch.float32, device=device)
     row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=device)
-    grad = None if grad_scale is None else torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    grad = None if grad_scale is None else _like(logits)
     L = _lib.lib()
     size = L.gdpso_distill_workspace_bytes(n, v, k)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    at = (2 * n + 4) // 4 * 4  # 2 n + 1 statistics, then the call's workspace
+    stats = torch.empty(at + (size + 3) // 4, dtype=torch.float32, device=device)
+    base = stats.data_ptr()
     _lib.run(device, L.gdpso_distill, n, v, k, rows.data_ptr(), stride, dtype, t.data_ptr(), t_dtype, idx.data_ptr(), index_bytes, ptr(mask), temperature,
-             0.0 if grad_scale is None else grad_scale, loss.data_ptr(), row_loss.data_ptr(), stats.data_ptr(), ptr(grad), ws.data_ptr(), size)
+             0.0 if grad_scale is None else grad_scale, loss.data_ptr(), row_loss.data_ptr(), base, ptr(grad), base + 4 * at, size)
     return loss, row_loss, grad, stats
 
 
@@ -552,7 +557,7 @@ def distill_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
         raise ValueError(f"row_stats must be contiguous float32 [{2 * n + 1}]")
     if upstream.dtype != torch.float32 or upstream.numel() != 1:
         raise ValueError("upstream must be a float32 scalar")
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    grad = _like(logits)
     _lib.run(device, _lib.lib().gdpso_distill_grad, n, v, k, rows.data_ptr(), stride, dtype, t.data_ptr(), t_dtype, idx.data_ptr(), index_bytes, ptr(mask),
              temperature, row_stats.data_ptr(), upstream.data_ptr(), grad.data_ptr())
     return grad

@@ -61,8 +61,8 @@ class _Balance(torch.autograd.Function):
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_indices, mask, temperature):
-        loss, _, _, stats = engine._distill(logits, teacher_logits, teacher_indices, mask, temperature, None)
-        ctx.save_for_backward(logits, teacher_logits, teacher_indices, mask, stats)
+        loss, loss_rows, _, stats = engine._distill(logits, teacher_logits, teacher_indices, mask, temperature, None)
+        ctx.save_for_backward(logits, teacher_logits, teacher_indices, mask, stats[:2 * loss_rows.numel() + 1])
         ctx.temperature = temperature
         return loss
 
