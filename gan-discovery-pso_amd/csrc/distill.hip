@@ -4,8 +4,8 @@
 //   d loss / d s[i,c] = (t / rows) (p[i,c] - sum of q_ij with idx_ij = c)
 //
 // The work is one softmax over a long row and k corrections, bound by reading the logits and writing the gradient once
-// each.  Rows are therefore held in registers between the two: by 1 ... 64 lanes up to 2048 columns (dist_team_kernel), by a
-// workgroup of 256 or 1024 threads up to 131072 columns of 16-bit logits or 65536 of fp32 (dist_row_kernel).  Longer rows,
+// each.  Rows are therefore held in registers between the two: by 1 ... 64 lanes up to 2048 fp32 or 4096 16-bit columns
+// (dist_team_kernel), by a workgroup of 256 ... 1024 threads up to 131072 or 65536 (dist_row_kernel).  Longer rows,
 // and few long rows (whose workgroups would leave most CUs idle), are cut into segments: one launch leaves every
 // segment's maximum and sum, a second joins them and writes (dist_part_kernel, dist_apply_kernel).
 //
@@ -24,7 +24,9 @@ namespace {
 
 constexpr int DIST_MAX_K = GDPSO_DISTILL_MAX_K;
 constexpr int TEAM_THREADS = 256;
-constexpr int TEAM_MAX_V = 2048;
+// Chunks of 16 bytes that the lanes of a wave hold, eight each (127765 x 2101 bf16: 566 us so, 673 by workgroups; fp32 rows of that
+// length would be sixteen chunks a lane: 632, 589 by workgroups).
+constexpr int TEAM_MAX_CHUNKS = 512;
 constexpr int SEG_THREADS = 256, SEG_NCH = 8;  // a segment: at most 8192 fp32 or 16384 16-bit columns
 constexpr int BITS = 1 << 16;
 constexpr float LN2 = 0.69314718f;
@@ -111,13 +113,25 @@ __device__ __forceinline__ float row_loss_of(const DistArgs &a, float terms, flo
     return l == 0.f || tl == 0.f ? 0.f : a.temperature * a.temperature * LN2 * (terms + (log2f(l) - log2f(tl)));
 }
 
+// The group of rows that a workgroup takes at u = its index, index + grid ...  Workgroups b, b + 8 ... run on one XCD, and a padded
+// batch keeps and leaves out rows in runs, so groups dealt out in order leave some XCDs nothing but masked rows wherever eight groups
+// divide a run.  Short rows: the groups of every eight neighbours are dealt to the XCDs starting at another one than the eight before
+// (256 columns fp32, every other 32 rows masked: 236 us in order, 163 so).  Rows of whole workgroups: each XCD has its eighth in one
+// piece (half masked, 8192 x 50007 bf16: 350 us in order, 354 dealt, 314 in pieces; 53676 x 5001 fp32, where a workgroup is 256
+// threads: 435 dealt, 480 in pieces).
+inline __host__ __device__ long long dealt_end(long long groups) { return (groups + 7) & ~7ll; }
+template <bool PIECES>
+__device__ __forceinline__ long long dealt(long long u, long long end) {  // may lie behind the last group
+    return PIECES ? (u & 7) * (end >> 3) + (u >> 3) : (u & ~7ll) + ((u + (u >> 3)) & 7);
+}
+
 // 1 / rows that the mask keeps
 __global__ __launch_bounds__(1024) void dist_kept_kernel(int n, const unsigned char *__restrict__ mask, float *__restrict__ inv_rows) {
     const float inv = inverse(count_kept<1024>(mask, n));
     if (threadIdx.x == 0) *inv_rows = inv;
 }
 
-// ------------------------------------------------------------------------------------- rows of up to 2048 columns
+// ------------------------------------------------------------------------------------- rows of lanes
 template <typename E, int THREADS, int TEAM, int NCH, bool VALUE, bool GRAD>
 __global__ __launch_bounds__(THREADS) void dist_team_kernel(DistArgs a) {
     constexpr int VEC = vec_of<E>(), TEAMS = THREADS / TEAM, WORDS = (TEAM * NCH * VEC + 31) / 32;
@@ -131,7 +145,10 @@ __global__ __launch_bounds__(THREADS) void dist_team_kernel(DistArgs a) {
         for (int w = pos; w < WORDS; w += TEAM) s_bits[team][w] = 0;
     }
     double sum = 0.;
-    for (long long i = (long long)blockIdx.x * TEAMS + team; i < a.n; i += (long long)gridDim.x * TEAMS) {
+    const long long end = dealt_end((a.n + TEAMS - 1ll) / TEAMS);
+    for (long long u = blockIdx.x; u < end; u += gridDim.x) {
+        const long long i = dealt<false>(u, end) * TEAMS + team;
+        if (i >= a.n) continue;
         const E *row = (const E *)a.logits + i * a.row_stride;
         E *grow = (E *)a.grad + i * a.v;
         if (a.mask && !a.mask[i]) {
@@ -304,7 +321,10 @@ __global__ __launch_bounds__(THREADS, 4) void dist_row_kernel(DistArgs a) {
     }
     double sum = 0.;
     int turn = 0;
-    for (long long i = blockIdx.x; i < a.n; i += gridDim.x) {
+    const long long end = dealt_end(a.n);
+    for (long long u = blockIdx.x; u < end; u += gridDim.x) {
+        const long long i = dealt<(THREADS >= 512)>(u, end);
+        if (i >= a.n) continue;
         const E *row = (const E *)a.logits + i * a.row_stride;
         E *grow = (E *)a.grad + i * a.v;
         if (a.mask && !a.mask[i]) {
@@ -567,11 +587,15 @@ struct Plan {
 inline Plan plan_rows(int n, int v, int vec) {
     Plan p = {BY_TEAM, 0, 0, 0, 0, 0};
     const int chunks = ceil_div(v, vec);
-    if (v <= TEAM_MAX_V) {
+    if (chunks <= TEAM_MAX_CHUNKS) {
         p.team = 1;
         while (p.team < chunks && p.team < 64) p.team <<= 1;
         p.chunks = 1;
         while (p.team * p.chunks < chunks) p.chunks <<= 1;
+        // Many rows: fewer lanes a row and up to four chunks a lane, so that a wave deals with several rows' teachers at once (65536 x
+        // 512 fp32: 75 us with 64 lanes, 67 with 32; 262144 x 256: 434 and 238).  Few rows have to spread over the chip instead.
+        if (n >= 8192)
+            while (p.team > 16 && p.chunks < 4) p.team >>= 1, p.chunks <<= 1;
         // rows that 1024 threads finish in two rounds are left to one workgroup
         p.threads = p.team <= 8 && n > 2 * (TEAM_THREADS / p.team) && n <= 2 * (1024 / p.team) ? 1024 : TEAM_THREADS;
         return p;
@@ -591,13 +615,17 @@ inline Plan plan_rows(int n, int v, int vec) {
     return p;
 }
 
-constexpr int DIST_BLOCKS = 2048;
+// Workgroups at most, an odd number of eights, so that a workgroup's later rows fall elsewhere in a padded batch's pattern than its
+// first: few rows a workgroup, so that those with masked rows leave their place to others (8192 x 50007 bf16, half masked: 2048
+// workgroups 375 us, 8192 351), but a team's teacher entries and LDS are set up once for several (fp32, 262144 x 256, half masked: 4088
+// workgroups 163 us, 8184 247).
+constexpr int DIST_TEAM_BLOCKS = 4088, DIST_ROW_BLOCKS = 16376;
 inline int dist_blocks(const Plan &p, int n) {
     if (p.way == BY_SEGMENT) return n > 0 ? n : 1;
     const long rows = p.way == BY_TEAM ? p.threads / p.team : 1;
     const long want = ((long)n + rows - 1) / rows;
     if (p.way == BY_TEAM && want <= 2) return 1;  // a second round of rows costs less than the launch that joins workgroups
-    return (int)(want < 1 ? 1 : std::min<long>(want, DIST_BLOCKS));
+    return (int)(want < 1 ? 1 : std::min<long>(want, p.way == BY_TEAM ? DIST_TEAM_BLOCKS : DIST_ROW_BLOCKS));
 }
 // Workspace: ticket, sums of row losses, segments
 constexpr size_t TICKET_BYTES = 16;
@@ -616,19 +644,21 @@ int launch_team(hipStream_t stream, const DistArgs &a, const Plan &p) {
         else if (p.team == 4) DIST_TEAM(1024, 4, 1);
         else DIST_TEAM(1024, 8, 1);
     } else {
-        switch (p.team * 16 + p.chunks) {
-            case 1 * 16 + 1: DIST_TEAM(256, 1, 1); break;
-            case 2 * 16 + 1: DIST_TEAM(256, 2, 1); break;
-            case 4 * 16 + 1: DIST_TEAM(256, 4, 1); break;
-            case 8 * 16 + 1: DIST_TEAM(256, 8, 1); break;
-            case 16 * 16 + 1: DIST_TEAM(256, 16, 1); break;
-            case 32 * 16 + 1: DIST_TEAM(256, 32, 1); break;
-            case 64 * 16 + 1: DIST_TEAM(256, 64, 1); break;
-            case 64 * 16 + 2: DIST_TEAM(256, 64, 2); break;
-            case 64 * 16 + 4: DIST_TEAM(256, 64, 4); break;
-            default:
-                if constexpr (is_f32<E>()) DIST_TEAM(256, 64, 8);
-                break;
+        switch (p.team * 32 + p.chunks) {
+            case 1 * 32 + 1: DIST_TEAM(256, 1, 1); break;
+            case 2 * 32 + 1: DIST_TEAM(256, 2, 1); break;
+            case 4 * 32 + 1: DIST_TEAM(256, 4, 1); break;
+            case 8 * 32 + 1: DIST_TEAM(256, 8, 1); break;
+            case 16 * 32 + 1: DIST_TEAM(256, 16, 1); break;
+            case 32 * 32 + 1: DIST_TEAM(256, 32, 1); break;
+            case 64 * 32 + 1: DIST_TEAM(256, 64, 1); break;
+            case 64 * 32 + 2: DIST_TEAM(256, 64, 2); break;
+            case 16 * 32 + 2: DIST_TEAM(256, 16, 2); break;
+            case 16 * 32 + 4: DIST_TEAM(256, 16, 4); break;
+            case 32 * 32 + 4: DIST_TEAM(256, 32, 4); break;
+            case 64 * 32 + 4: DIST_TEAM(256, 64, 4); break;
+            case 64 * 32 + 8: DIST_TEAM(256, 64, 8); break;
+            default: break;
         }
     }
 #undef DIST_TEAM

@@ -68,30 +68,37 @@ __device__ __forceinline__ float team_sum(float v) {
     return team_reduce<TEAM>(v, [](float a, float b) { return a + b; });
 }
 
-// NCH chunks of a row per thread.  TAIL: the columns behind the last whole chunk are held one a thread instead of as a cut
-// chunk (teams of more threads than a chunk has elements): many chunks that each might be the cut one cost a
-// workgroup's rows twice the registers.
-template <typename E, int TEAM, int NCH, bool TAIL = false>
+// NCH chunks of a row per thread.  ENDS, for teams of more threads than two chunks have elements: chunks of 16-bit columns begin at
+// the row's first multiple of 16 bytes, and the few columns ahead of them and behind the last whole one are held one a thread.  Rows
+// of an odd number of columns are off 16 bytes (8192 x 50007 bf16, loss alone: 246 us at element alignment, 227 so; fp32 gains
+// nothing), and many chunks that each might be the cut one cost a workgroup's rows twice the registers.
+template <typename E, int TEAM, int NCH, bool ENDS = false>
 struct RowRegs {
     static constexpr int VEC = vec_of<E>();
     using V = typename VecAt<E, VEC>::type;
     using W = __attribute__((ext_vector_type(4))) unsigned;
     W raw[NCH];
-    E tail;
+    E single;  // ENDS: the column ahead of the chunks or behind them that this thread holds, if any
+    int head;  // ENDS: columns ahead of the chunks
 
+    // Columns of a row ahead of its first multiple of 16 bytes, the column behind its last whole chunk, and thread pos' column among
+    // those outside the chunks (e or more: none).
+    __device__ __forceinline__ static int head_of(const E *row, int e) { return is_f32<E>() ? 0 : min((int)(-(uintptr_t)row / sizeof(E) % VEC), e); }
+    __device__ __forceinline__ static int outside(int head, int e, int pos) { return pos < head ? pos : head + (e - head) / VEC * VEC + pos - head; }
     __device__ __forceinline__ static int column(int j, int pos) { return (j * TEAM + pos) * VEC; }
     __device__ __forceinline__ void load(const E *__restrict__ row, int e, int pos) {
-        if constexpr (TAIL) {
-            static_assert(TEAM >= VEC, "a thread for every column of the tail");
+        if constexpr (ENDS) {
+            static_assert(TEAM >= 2 * VEC, "a thread for every column outside the chunks");
             constexpr unsigned none = is_f32<E>() ? 0xff800000u : (__is_same(E, bf16_t) ? 0xff80ff80u : 0xfc00fc00u);  // -inf
+            head = head_of(row, e);
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
-                const int c = column(j, pos);
+                const int c = head + column(j, pos);
                 raw[j] = W{none, none, none, none};
                 if (c + VEC <= e) raw[j] = __builtin_bit_cast(W, *(const V *)(row + c));
             }
-            const int whole = e / VEC * VEC;
-            tail = whole + pos < e ? row[whole + pos] : (E)-INFINITY;
+            const int c = outside(head, e, pos);
+            single = c < e ? row[c] : (E)-INFINITY;
             return;
         }
 #pragma unroll
@@ -126,7 +133,7 @@ struct RowRegs {
     // chunk j lies beyond the row for the whole team: the same for every thread, so a branch skips its arithmetic
     __device__ __forceinline__ static bool beyond(int j, int e) { return j > 0 && j * TEAM * VEC >= e; }
     __device__ __forceinline__ float max(int e) const {
-        float m = TAIL ? (float)tail : -INFINITY;
+        float m = ENDS ? (float)single : -INFINITY;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             if (beyond(j, e)) continue;
@@ -136,7 +143,7 @@ struct RowRegs {
         return m;
     }
     __device__ __forceinline__ float sum_exp(const Shift &s, int e) const {
-        float l = TAIL ? s.exp((float)tail) : 0.f;
+        float l = ENDS ? s.exp((float)single) : 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             if (beyond(j, e)) continue;
@@ -149,21 +156,32 @@ struct RowRegs {
     // (8192 x 50007 bf16: 412 us, 408 with `clear` alone so, 401 with both)
     template <typename F>
     __device__ __forceinline__ void map(E *__restrict__ row, int e, int pos, F f) const {
-        static_assert(TAIL, "rows with a tail");
+        static_assert(ENDS, "long rows");
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             if (beyond(j, e)) continue;
-            const int c = column(j, pos);
+            const int c = head + column(j, pos);
             V x;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) x[v] = (E)f(at(j, v));
             if (c + VEC <= e) __builtin_nontemporal_store(x, (V *)(row + c));
         }
-        const int whole = e / VEC * VEC;
-        if (whole + pos < e) row[whole + pos] = (E)f((float)tail);
+        const int c = outside(head, e, pos);
+        if (c < e) row[c] = (E)f((float)single);
     }
     // row[c] = 0
     __device__ __forceinline__ static void clear(E *__restrict__ row, int e, int pos) {
+        if constexpr (ENDS) {
+            const int head = head_of(row, e);
+#pragma unroll 1
+            for (int j = 0; j < NCH; ++j) {
+                const int c = head + column(j, pos);
+                if (c + VEC <= e) __builtin_nontemporal_store(V{}, (V *)(row + c));
+            }
+            const int c = outside(head, e, pos);
+            if (c < e) row[c] = (E)0.f;
+            return;
+        }
 #pragma unroll 1
         for (int j = 0; j < NCH; ++j) {
             const int c = column(j, pos);

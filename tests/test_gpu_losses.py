@@ -312,6 +312,18 @@ def test_distill_strides_and_shapes(eng):
     assert float(empty[0]) == 0 and empty[1].numel() == 0 and tuple(empty[2].shape) == (0, 50)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(40, 2049), (130, 16399), (6, 40003), (150, 33001)])
+def test_distill_long_rows_at_every_alignment(eng, n, v, dtype):
+    """Rows that begin at any offset from 16 bytes, while their gradient's rows begin at others."""
+    for first in (0, 1, 3, 6):
+        logits = rand(v + first, n, v + 5 + first, scale=2.0, dtype=dtype)[:, first:first + v]
+        t_logits, t_idx = teacher_of(logits, 5, first)
+        t_idx[0, 0], t_idx[1, 0] = 0, v - 1
+        mask = torch.arange(n, device=DEV) % 5 != 3
+        check_distill(eng.distill(logits, t_logits, t_idx, mask=mask, grad_scale=float(n)), logits, t_logits, t_idx, mask, 1.0, float(n))
+
+
 def test_offsets_beyond_32_bits(eng):
     """33,000 rows of 131,072 logits are 4.3e9 elements: the last rows come out as in a small call."""
     n, v, k = 33000, 131072, 4
