@@ -25,7 +25,9 @@ constexpr int WIDE_THREADS = 512; // rows of up to 16384 columns: 32 values a th
 constexpr int HIST_THREADS = 1024;
 constexpr int JOIN_COLS = 16, JOIN_GROUPS = 64;
 constexpr int HIST_MAX = 64;
-constexpr int OWN_CHOICES = 4096;  // choices that every workgroup of the gradient counts for itself (16 a thread)
+// Choices that every workgroup of the gradient counts for itself, 16 a thread (a call with 4096 choices: 17.8 us, 19.9 with a launch
+// that counts).
+constexpr int OWN_CHOICES = 4096;
 
 // Counting workgroups: eight choices a thread; the partial counts are read again by every workgroup of the gradient, so there
 // are at most 64 of them.

@@ -381,6 +381,67 @@ def test_on_another_stream(eng):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+def test_two_streams_at_once(eng):
+    """Calls that overlap on two streams, each with a workspace of its own."""
+    sizes = [(4000, 513, 5), (70, 70001, 9), (9000, 33, 3), (300, 5003, 20)]
+    data = []
+    for n, v, k in sizes:
+        logits = rand(n, n, v, scale=2.0, dtype=torch.bfloat16)
+        data.append((logits, *teacher_of(logits, k, 3), randint(4, 0, v, n, 2)))
+    x, code, g = rand(1, 6000, 70), rand(2, 90, 70), rand(3, 6000, 90)
+
+    def work():
+        out = []
+        for logits, t, i, choice in data:
+            out += eng.distill(logits, t, i, grad_scale=1.0)
+            if logits.shape[1] <= 16384:
+                out += eng.balance(logits, choice, grad_scale=1.0)
+        return out + [eng.code_logits(x, code), *eng.code_logits_grad(g, x, code)]
+
+    want = work()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(3):
+        for s, out in zip(streams, got):
+            with torch.cuda.stream(s):
+                out.append(work())
+    torch.cuda.synchronize()
+    for out in got:
+        for run in out:
+            assert all(torch.equal(a, b) for a, b in zip(run, want))
+
+
+def test_two_graphs_replay_in_any_order(eng):
+    """Two captured calls keep their workspaces apart, also when they are replayed one beside the other's results."""
+    sets = []
+    for seed in (1, 2):
+        logits = rand(seed, 40, 40000, scale=2.0)
+        t, i = teacher_of(logits, 6, seed)
+        x, code, g = rand(seed + 10, 5000, 40), rand(seed + 20, 300, 40), rand(seed + 30, 5000, 300)
+        choice = randint(seed, 0, 300, 5000, 2)
+
+        def step(logits=logits, t=t, i=i, x=x, code=code, g=g, choice=choice):
+            return [*eng.distill(logits, t, i, grad_scale=2.0), *eng.balance(g, choice, grad_scale=3.0), *eng.code_logits_grad(g, x, code)]
+
+        want = [v.clone() for v in step()]
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step()
+        sets.append((graph, out, want, step))  # (a graph's inputs have to live as long as it does: step holds them)
+    for order in ((0, 1), (1, 0), (1, 1, 0), (0, 0, 1)):
+        for which in order:
+            for v in sets[which][1]:
+                v.fill_(7)
+            sets[which][0].replay()
+        eng.code_logits(rand(5, 100, 16), rand(6, 30, 16))
+        torch.cuda.synchronize()
+        for _, out, want, _ in sets:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_captured_steps_replay(eng):
     """Two graphs of a whole training step, replayed in turn with new inputs and eager work between: every replay equals the
     eager result on the same inputs."""
