@@ -414,7 +414,7 @@ def code_logits(inputs: torch.Tensor, codebook: torch.Tensor, temperature: float
     """Logits of the soft assignment of ``inputs`` [..., D] to the rows of ``codebook`` [K, D] (gdpso_code_logits):
     (2 <x, code> - |code|^2) / temperature, float32 [..., K], whatever the type of the inputs."""
     device, x, cb, k, d, dtype = _code_args(inputs, codebook)
-    out = torch.empty((*inputs.shape[:-1], k), dtype=torch.float32, device=device)
+    out = x.new_empty((*inputs.shape[:-1], k), dtype=torch.float32)
     _lib.run(device, _lib.lib().gdpso_code_logits, x.shape[0], d, k, x.data_ptr(), cb.data_ptr(), dtype, temperature, out.data_ptr())
     return out
 
@@ -432,7 +432,7 @@ def code_logits_grad(grad_logits: torch.Tensor, inputs: torch.Tensor, codebook: 
     dcb = _like(codebook) if want_codebook else None
     L = _lib.lib()
     size = L.gdpso_code_logits_grad_workspace_bytes(n, d, k)
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     _lib.run(device, L.gdpso_code_logits_grad, n, d, k, g.data_ptr(), x.data_ptr(), cb.data_ptr(), dtype, temperature, ptr(dx), ptr(dcb), ptr(ws), size)
     return dx, dcb
 
@@ -477,13 +477,13 @@ def _row_indices(indices: torch.Tensor, lead, n: int, what: str):
 def _balance(logits, indices, mask, grad_scale):
     device, rows, n, e, stride, dtype, mask = _loss_rows(logits, mask, indices=indices)
     idx, k, index_bytes = _row_indices(indices, logits.shape[:-1], n, "indices")
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    counts = torch.empty(e, dtype=torch.int64, device=device)
-    mean_prob = torch.empty(e, dtype=torch.float32, device=device)
+    loss = rows.new_empty((), dtype=torch.float32)
+    counts = rows.new_empty(e, dtype=torch.int64)
+    mean_prob = rows.new_empty(e, dtype=torch.float32)
     grad = None if grad_scale is None else _like(logits)
     L = _lib.lib()
     size = L.gdpso_balance_workspace_bytes(n, e)
-    ws = torch.empty((size + 7) // 8 + 2, dtype=torch.int64, device=device)  # two totals, then the call's workspace
+    ws = rows.new_empty((size + 7) // 8 + 2, dtype=torch.int64)  # two totals, then the call's workspace
     base = ws.data_ptr()
     _lib.run(device, L.gdpso_balance, n, e, k, rows.data_ptr(), stride, dtype, idx.data_ptr(), index_bytes, ptr(mask),
              0.0 if grad_scale is None else grad_scale, loss.data_ptr(), counts.data_ptr(), base, mean_prob.data_ptr(), ptr(grad), base + 16, size)
@@ -525,13 +525,13 @@ def _distill_args(logits, teacher_logits, teacher_indices, mask, **others):
 
 def _distill(logits, teacher_logits, teacher_indices, mask, temperature, grad_scale):
     device, rows, n, v, stride, dtype, mask, k, idx, index_bytes, t, t_dtype = _distill_args(logits, teacher_logits, teacher_indices, mask)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
+    loss = rows.new_empty((), dtype=torch.float32)
+    row_loss = rows.new_empty(logits.shape[:-1], dtype=torch.float32)
     grad = None if grad_scale is None else _like(logits)
     L = _lib.lib()
     size = L.gdpso_distill_workspace_bytes(n, v, k)
     at = (2 * n + 4) // 4 * 4  # 2 n + 1 statistics, then the call's workspace
-    stats = torch.empty(at + (size + 3) // 4, dtype=torch.float32, device=device)
+    stats = rows.new_empty(at + (size + 3) // 4, dtype=torch.float32)
     base = stats.data_ptr()
     _lib.run(device, L.gdpso_distill, n, v, k, rows.data_ptr(), stride, dtype, t.data_ptr(), t_dtype, idx.data_ptr(), index_bytes, ptr(mask), temperature,
              0.0 if grad_scale is None else grad_scale, loss.data_ptr(), row_loss.data_ptr(), base, ptr(grad), base + 4 * at, size)
