@@ -715,8 +715,9 @@ extern "C" int gdpso_distill(void *stream_, int n, int v, int k, const void *log
     float2 *parts = (float2 *)((char *)loss_part + loss_bytes(p, n));
     const bool one = dist_blocks(p, n) == 1;
     // the kept rows ahead of a gradient: by the workgroups themselves, by the segments' first launch, or by a launch of its own
+    // (no rows: neither runs, and the finishing launch counts)
     const bool ahead = mask && n > COUNT_ROWS && p.way != BY_SEGMENT && (grad || one);
-    const Kept kept = p.way == BY_SEGMENT || ahead ? KEPT_READ : (mask && (grad || one) ? KEPT_COUNT : KEPT_ALL);
+    const Kept kept = (p.way == BY_SEGMENT && n > 0) || ahead ? KEPT_READ : (mask && (grad || one) ? KEPT_COUNT : KEPT_ALL);
     const DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), grad_scale,
                         nullptr, row_stats, inv_rows, n > 0 ? (float)(1. / n) : 0.f, kept, p.way == BY_SEGMENT ? ticket : nullptr, loss, row_loss,
                         grad, loss_part, p.seg, p.segs, parts};

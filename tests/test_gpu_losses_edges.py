@@ -63,3 +63,19 @@ def test_code_products_of_whole_numbers_are_exact(eng, n, k, d, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_large_code_gradients_of_whole_numbers_are_exact(eng, dtype):
     check_whole(eng, 16411, 4099, 256, dtype)  # above 2^34 products
+
+
+# -------------------------------------------------------------------------------------------------- empty batches
+@pytest.mark.parametrize("v", [8, 3000, 20000, 200003])
+@pytest.mark.parametrize("masked", [False, True])
+def test_distill_of_no_rows(v, masked):
+    """Loss and stats are written whatever the buffers held before."""
+    lib = importlib.import_module("gan-discovery-pso_amd._lib")
+    L = lib.lib()
+    size = L.gdpso_distill_workspace_bytes(0, v, 4)
+    ws = torch.full((size // 4 + 4,), math.nan, device=DEV)
+    loss, stats = torch.full((), math.nan, device=DEV), torch.full((1,), math.nan, device=DEV)
+    mask = torch.ones(1, dtype=torch.uint8, device=DEV) if masked else None
+    lib.run(loss.device, L.gdpso_distill, 0, v, 4, None, v, 0, None, 0, None, 8, lib.ptr(mask), 1.0, 1.0, loss.data_ptr(), None, stats.data_ptr(), None,
+            ws.data_ptr(), size)
+    assert float(loss) == 0.0 and float(stats) == 0.0
