@@ -11,8 +11,7 @@
 // fp32 accuracy: a value is cut into bf16 parts, each the rounded rest of the one before, so that an fp32 value is three
 // parts (3 x 8 bits), an fp16 value two, a bf16 value itself, and the product of two values is the sum of the products of
 // their parts.  Those of order 2^-24 and below are left out: six matrix instructions for fp32 x fp32, five for fp32 x fp16,
-// three for fp32 x bf16; four and two where the logits' gradient may do with two parts (grads_kernel).  Parts multiply exactly and
-// add up in fp32.  The forward product of two 16-bit operands needs no cutting.
+// three for fp32 x bf16.  Parts multiply exactly and add up in fp32.  The forward product of two 16-bit operands needs no cutting.
 //
 // What bounds them: the fp32 logits or their gradient, [n, k], against which latents and codes are small, and with fp32 operands the
 // matrix instructions as much.  Latents 65536 x 64, 512 codes, fp32: logits 35 us (134 MB written, 3.8 TB/s, and 26 GFLOP of bf16 products), both
@@ -261,9 +260,11 @@ struct ColsOperand {
 
 // The same for the gradients of 16-bit codes and latents, from planes that planes_kernel has cut and transposed: P planes of bf16, each
 // [pitch / KT][cols][KT] with `pitch` the sum's length rounded up to whole stages, zeros behind its end.  A stage passes
-// through registers as it is.  Gathering 16-bit values anew in every workgroup took half of these gradients' time
-// (50007 x 1024 x 256, bf16: both 234 us, 181 from planes); with fp32 the six matrix instructions a product hide it, and the
-// planes' own launch is a loss (65536 x 512 x 64: 68 us, 67 from planes and 14 for those).
+// through registers as it is, where gathering takes every workgroup eight loads of two bytes a value pair and the cut (a call, gathering
+// and from planes with their launch: bf16, 20000 x 2048 x 256 171 and 157 us, 50007 x 1024 x 256 177 and 174; fp16, whose tile of 256
+// columns would leave one wave a SIMD, 374 and 231, 411 and 271; up to 128 columns there is little between them, 50007 x 512 x 128 70 and
+// 72, fp16 65536 x 512 x 64 61 and 67).  With fp32 the six matrix instructions a product hide the gathering, and the planes' own launch
+// is a loss (65536 x 512 x 64: 68 us, 67 from planes and 14 for those).
 template <int BN, int P>
 struct PlanesOperand {
     static constexpr int UNITS = BN * 4, NU = (UNITS + CL_THREADS - 1) / CL_THREADS, AHEAD = 0, PLANE = BN;
@@ -801,15 +802,14 @@ __global__ __launch_bounds__(CL_THREADS) void planes_kernel(PlanesArgs a) {
     }
 }
 
-// Both gradients in one launch, the codebook's workgroups first (they run longer).  PG: parts of the logits' gradient.  For
-// results of 16 bits two are enough where both sums are long: they leave 2^-17 of a value out, and an fp32 sum of m products may be
-// off by m 2^-24 of their magnitudes by itself, which is as much from m = 128 on; either is far below the result's own
-// rounding, 2^-9 or 2^-12.
-template <typename E, int PG, int P, int MT, int NT>
+// Both gradients in one launch, the codebook's workgroups first (they run longer).  The logits' gradient keeps all three parts also
+// for results of 16 bits: its rows sum to about nothing, so a common offset of the codes has to cancel in the products, and two parts
+// leave 2^-17 of the offset there (fp16 codes of 1024 and their neighbours: twice the result's own rounding).
+template <typename E, int P, int MT, int NT>
 __global__ __launch_bounds__(CL_THREADS, 2) void grads_kernel(ProductArgs code, int code_blocks, ProductArgs x) {
     __shared__ __attribute__((aligned(16))) char lds[tile_lds<GRAD_X, E, P, NT>()];
-    if ((int)blockIdx.x < code_blocks) product_tile<GRAD_CODE, float, E, PG, P, bf16_t, MT, NT, E>(code, blockIdx.x, lds);
-    else product_tile<GRAD_X, float, E, PG, P, bf16_t, MT, NT, E>(x, blockIdx.x - code_blocks, lds);
+    if ((int)blockIdx.x < code_blocks) product_tile<GRAD_CODE, float, E, 3, P, bf16_t, MT, NT, E>(code, blockIdx.x, lds);
+    else product_tile<GRAD_X, float, E, 3, P, bf16_t, MT, NT, E>(x, blockIdx.x - code_blocks, lds);
 }
 
 // Joins the splits' partial sums in a fixed order.  The codebook's gradient: 64 neighbouring elements a workgroup, the splits
@@ -883,8 +883,9 @@ constexpr int grad_parts() {
 // All columns in one tile up to 128, 16-bit types 256: the rows' operand, the large one, is read and cut once.  With fp32's three parts
 // 256 columns leave one wave a SIMD and are read from LDS more than the matrix instructions hide: two tiles of 128 (50000 x 512 x 256:
 // 290 us in one, 171 so).  128 rows once they fill the chip or the products are large (fp32, 64 and 128 rows: 8192 x 512 x 256 46 and
-// 56 us, 32000 x 512 x 256 136 and 109, 8192 x 8192 x 64 201 and 139); the tile of 256 columns later (bf16: 20000 x 2048 x 256 134
-// and 140 us, 50000 x 2048 x 256 294 and 272, 20000 x 8192 x 256 615 and 406; fp16's two parts would spill).  `parts` of a code: 3 for fp32,
+// 56 us, 32000 x 512 x 256 136 and 109, 8192 x 8192 x 64 201 and 139); the tile of 256 columns later (bf16: 20000 x 2048 x 256 162
+// and 167 us, 50000 x 2048 x 256 332 and 343, 8192 x 8192 x 256 290 and 249, 20000 x 8192 x 256 706 and 518; fp16's two parts would
+// spill).  `parts` of a code: 3 for fp32,
 // 2 for fp16, 1 for bf16.
 constexpr int SMALL_ROWS = 4096;
 struct Tile {
@@ -962,11 +963,23 @@ int launch_logits(hipStream_t stream, ProductArgs a) {
 }
 
 // code.out or x.out null: that gradient is not wanted
-template <typename E, int PG>
-int launch_grads(hipStream_t stream, const ProductArgs &code, const ProductArgs &x, Tile t, long code_blocks, long grid) {
+template <typename E>
+int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
+    const bool small = t.mt == 0;
+    const int tile_m = small ? 16 : 64 * t.mt, tile_n = 16 * (small ? SMALL_NT : t.nt);
+    code.tiles_m = ceil_div(code.rows, tile_m);
+    x.tiles_m = ceil_div(x.rows, tile_m);
+    code.tiles_n = x.tiles_n = ceil_div(x.cols, tile_n);
+    // the larger form deals splits and row tiles to the XCDs in eights
+    const long splits = small ? code.splits : (code.splits + 7) / 8 * 8, row_tiles = small ? x.tiles_m : (x.tiles_m + 7) / 8 * 8 * x.splits;
+    const long code_blocks = code.out ? splits * code.tiles_m * code.tiles_n : 0;
+    const long grid = code_blocks + (x.out ? row_tiles * x.tiles_n : 0);
+    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
     constexpr int P = grad_parts<E>();
-#define CL_GRADS(MT, NT) hipLaunchKernelGGL((grads_kernel<E, PG, P, MT, NT>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x)
-    if (t.mt == 2) {
+#define CL_GRADS(MT, NT) hipLaunchKernelGGL((grads_kernel<E, P, MT, NT>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x)
+    if (small) {
+        hipLaunchKernelGGL((grads_small_kernel<E, P>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x);
+    } else if (t.mt == 2) {
         if (t.nt == 2) CL_GRADS(2, 2);
         else if (t.nt == 4) CL_GRADS(2, 4);
         else if (t.nt == 8) CL_GRADS(2, 8);
@@ -980,27 +993,6 @@ int launch_grads(hipStream_t stream, const ProductArgs &code, const ProductArgs 
 #undef CL_GRADS
     GDPSO_HIP(hipGetLastError());
     return GDPSO_OK;
-}
-template <typename E>
-int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
-    const bool small = t.mt == 0;
-    const int tile_m = small ? 16 : 64 * t.mt, tile_n = 16 * (small ? SMALL_NT : t.nt);
-    code.tiles_m = ceil_div(code.rows, tile_m);
-    x.tiles_m = ceil_div(x.rows, tile_m);
-    code.tiles_n = x.tiles_n = ceil_div(x.cols, tile_n);
-    // the larger form deals splits and row tiles to the XCDs in eights
-    const long splits = small ? code.splits : (code.splits + 7) / 8 * 8, row_tiles = small ? x.tiles_m : (x.tiles_m + 7) / 8 * 8 * x.splits;
-    const long code_blocks = code.out ? splits * code.tiles_m * code.tiles_n : 0;
-    const long grid = code_blocks + (x.out ? row_tiles * x.tiles_n : 0);
-    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
-    if (small) {
-        hipLaunchKernelGGL((grads_small_kernel<E, grad_parts<E>()>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x);
-        GDPSO_HIP(hipGetLastError());
-        return GDPSO_OK;
-    }
-    if constexpr (!is_f32<E>())
-        if (x.sum >= 128 && code.sum >= 128) return launch_grads<E, 2>(stream, code, x, t, code_blocks, grid);
-    return launch_grads<E, 3>(stream, code, x, t, code_blocks, grid);
 }
 
 int code_check(const char *what, int n, int d, int k, int dtype, float temperature) {

@@ -37,7 +37,40 @@ def whole(seed, most, *shape, dtype=torch.float32):
     return torch.randint(-most, most + 1, shape, generator=generator(seed)).to(dtype).to(DEV)
 
 
-# ------------------------------------------------------------------------------------------------- code products
+# ------------------------------------------------------------------------------------------------- code gradients
+def three_entries(seed, rows, cols):
+    """[rows, cols] with three entries a row that sum to nothing, up to their own rounding."""
+    gen = generator(seed)
+    at = torch.stack([torch.randperm(cols, generator=gen)[:3] for _ in range(rows)])
+    v = torch.randn(rows, 2, generator=gen)
+    v = torch.cat([v, -v.sum(dim=1, keepdim=True)], dim=1)
+    return torch.zeros(rows, cols).scatter_(1, at, v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k,d", [(40, 30, 20), (5000, 300, 64), (4500, 1000, 130), (33000, 130, 24)])
+def test_code_gradients_of_sums_that_cancel(eng, n, k, d, dtype):
+    """Rows (columns) of three entries that sum to nothing, times codes (latents) of one large offset: what is left is 2^-10 of the
+    summands for fp16.  A sum of three whole products meets three roundings of at most one step, 2 U, of the summands' magnitudes, and
+    the result two more of its own, so it is off by at most 8 U of the magnitudes; a logits' gradient held in fewer bits than
+    its own 24 would not cancel (16 bits: 64 U)."""
+    offset = {torch.float32: 2.0 ** 20, torch.bfloat16: 128.0, torch.float16: 1024.0}[dtype]
+    code = (offset + whole(1, 3, k, d).abs()).to(dtype)
+    x = (offset + whole(2, 3, n, d).abs()).to(dtype)
+    c64, x64 = code.double().cpu(), x.double().cpu()
+    g = three_entries(3, n, k)
+    dx, _ = eng.code_logits_grad(g.to(DEV), x, code, temperature=2.0, want_codebook=False)
+    g = g.double()
+    want = g @ c64
+    assert_within(dx, want, (g.abs() @ c64.abs()) * 8 * U + store_error(want, dtype), "dx")
+    g = three_entries(4, k, n).t().contiguous()
+    _, dc = eng.code_logits_grad(g.to(DEV), x, code, temperature=2.0, want_inputs=False)
+    g = g.double()
+    want = g.t() @ x64 - g.sum(dim=0)[:, None] * c64
+    assert_within(dc, want, (g.abs().t() @ x64.abs()) * 8 * U + (g.sum(dim=0).abs() + 3 * U * g.abs().sum(dim=0))[:, None] * c64 * 2 * U
+                  + g.abs().sum(dim=0)[:, None] * c64 * 3 * U + store_error(want, dtype), "dcode")
+
+
 # Every form of the three products: sizes around the rules that choose tiles, splits and stages, with cut last tiles and sums.
 WHOLE_SIZES = [(1, 1, 1), (33, 31, 17), (512, 256, 100), (2049, 130, 65), (4097, 257, 33), (5000, 40, 300), (8193, 129, 64), (9001, 300, 150),
                (9002, 515, 180), (8195, 1025, 210), (8200, 700, 250), (8199, 333, 256), (9000, 260, 300), (9000, 1500, 256), (20001, 64, 31),
