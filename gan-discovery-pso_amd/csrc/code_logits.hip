@@ -42,7 +42,36 @@ __device__ __forceinline__ V at_bytes(const E *p, unsigned off) {
     return *(const V *)((const char *)p + off);
 }
 
-// Cuts eight values into P parts of type M: parts[p] is the rounded rest of what the parts before it leave.
+// Cuts a pair of values into P parts: words[p] holds the two p-th parts, the rounded rest of what the parts before leave.  One
+// conversion instruction packs both.  BIG: values that the first part would round up to infinity have the largest bf16 for it, and an
+// infinity is the last part alone.  A third part meets nothing but the other value's first one, which has its sign and is 0 only where
+// the value is; a 16-bit type's infinity meets second parts too, and what comes out may be NaN.
+template <int P, bool BIG>
+__device__ __forceinline__ void cut_pair(float a, float b, unsigned (&words)[P]) {
+    using f32x2 = __attribute__((ext_vector_type(2))) float;
+    using bf16x2 = __attribute__((ext_vector_type(2))) bf16_t;
+    constexpr float MOST = 3.38953139e38f;
+    f32x2 rest = {a, b};
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        f32x2 x = rest;
+        if (BIG && p == 0) {  // (a NaN stays one: comparisons with it are false)
+            x[0] = fabsf(a) > MOST ? __builtin_copysignf(MOST, a) : a;
+            x[1] = fabsf(b) > MOST ? __builtin_copysignf(MOST, b) : b;
+        }
+        words[p] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf16x2));
+        rest[0] -= __builtin_bit_cast(float, words[p] << 16);
+        rest[1] -= __builtin_bit_cast(float, words[p] & 0xffff0000u);
+    }
+    if (BIG) {
+        const unsigned low = fabsf(a) == INFINITY ? 0xffffu : 0u, high = fabsf(b) == INFINITY ? 0xffff0000u : 0u;
+#pragma unroll
+        for (int p = 0; p < P; ++p) words[p] &= ~(low | high);
+        words[P - 1] |= (low & (__builtin_bit_cast(unsigned, a) >> 16)) | (high & __builtin_bit_cast(unsigned, b));
+    }
+}
+
+// Cuts eight values into P parts of type M.
 template <int P, typename M, typename E>
 __device__ __forceinline__ void cut(const E (&v)[8], Frag<M> (&parts)[P]) {
     if constexpr (__is_same(E, M) && P == 1) {
@@ -50,32 +79,23 @@ __device__ __forceinline__ void cut(const E (&v)[8], Frag<M> (&parts)[P]) {
         for (int e = 0; e < 8; ++e) parts[0][e] = v[e];
     } else {
         static_assert(__is_same(M, bf16_t), "parts are bf16");
-        using f32x2 = __attribute__((ext_vector_type(2))) float;
-        using bf16x2 = __attribute__((ext_vector_type(2))) bf16_t;
         using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
         u32x4 words[P];
-        float most = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {  // two values at a time: one conversion instruction packs both
-            f32x2 rest = {(float)v[2 * w], (float)v[2 * w + 1]};
-            if (P > 1) most = fmaxf(most, fmaxf(fabsf(rest[0]), fabsf(rest[1])));
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const unsigned bits = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, bf16x2));
-                words[p][w] = bits;
-                rest[0] -= __builtin_bit_cast(float, bits << 16);
-                rest[1] -= __builtin_bit_cast(float, bits & 0xffff0000u);
-            }
-        }
-        if (P > 1 && most > 3.3895e38f) {  // an infinite first part (inf, or rounded up to it) has no rest: inf - inf made it NaN
+        const auto all = [&](auto huge) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const unsigned low = (words[0][w] & 0x7fffu) == 0x7f80u ? 0u : 0xffffu;
-                const unsigned high = (words[0][w] & 0x7fff0000u) == 0x7f800000u ? 0u : 0xffff0000u;
+                unsigned pair[P];
+                cut_pair<P, decltype(huge)::value>((float)v[2 * w], (float)v[2 * w + 1], pair);
 #pragma unroll
-                for (int p = 1; p < P; ++p) words[p][w] &= low | high;
+                for (int p = 0; p < P; ++p) words[p][w] = pair[p];
             }
-        }
+        };
+        float most = 0.f;
+        if (P > 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)v[e]));
+        if (P > 1 && most > 3.3895e38f) all(std::true_type{});
+        else all(std::false_type{});
 #pragma unroll
         for (int p = 0; p < P; ++p) parts[p] = __builtin_bit_cast(Frag<M>, words[p]);
     }

@@ -98,6 +98,39 @@ def test_large_code_gradients_of_whole_numbers_are_exact(eng, dtype):
     check_whole(eng, 16411, 4099, 256, dtype)  # above 2^34 products
 
 
+@pytest.mark.parametrize("n,k,d", [(70, 40, 24), (300, 64, 200), (5000, 130, 40), (9001, 70, 150), (33000, 64, 64)])
+def test_code_products_with_infinities_and_the_largest_values(eng, n, k, d):
+    """fp32 values that a 16-bit type rounds up to infinity stay finite, and an infinity reaches what the formula says."""
+    biggest = torch.finfo(torch.float32).max
+    x, code = rand(n, n, d), rand(k, k, d, scale=1e-3)
+    g = rand(d, n, k)
+    x[3, 5], x[4, 2] = math.inf, -math.inf
+    x[6], x[7, 1] = -biggest, biggest  # padding rows of the type's lowest value, with a gradient of 0
+    code[2, 7] = 0.0
+    code[11, 9] = math.inf
+    g[6:8] = 0.0
+    g[9, 4], g[10, 4] = math.inf, biggest * 1e-2
+    s = eng.code_logits(x, code).double().cpu()
+    x64, c64, g64 = x.double().cpu(), code.double().cpu(), g.double().cpu()
+    want = 2 * x64 @ c64.t() - (c64 * c64).sum(dim=1)
+    bound = (2 * x64.abs() @ c64.abs().t() + (c64 * c64).sum(dim=1)) * (d + 4) * U + store_error(want, torch.float32)
+    big = want.abs() > 2 * biggest
+    want[big] = want[big].sign() * math.inf
+
+    def check(got, want, bound, what):
+        finite = want.isfinite()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~finite].nan_to_num(nan=7.0), want[~finite].nan_to_num(nan=7.0)), what
+        assert_within(got[finite], want[finite], bound[finite], what)
+
+    check(s, want, bound, "logits")
+    dx, dc = (t.double().cpu() for t in eng.code_logits_grad(g, x, code))
+    want = 2 * g64 @ c64
+    check(dx, want, 2 * (g64.abs() @ c64.abs()) * (k + 4) * U + store_error(want, torch.float32), "dx")
+    want = 2 * (g64.t() @ x64 - g64.sum(dim=0)[:, None] * c64)
+    bound = 2 * (g64.abs().t() @ x64.abs() + g64.abs().sum(dim=0)[:, None] * c64.abs()) * (n + 8) * U + store_error(want, torch.float32)
+    check(dc, want, bound, "dcode")
+
+
 # -------------------------------------------------------------------------------------------------- empty batches
 @pytest.mark.parametrize("v", [8, 3000, 20000, 200003])
 @pytest.mark.parametrize("masked", [False, True])
