@@ -7,7 +7,8 @@
 // each.  Rows are therefore held in registers between the two: by 1 ... 64 lanes up to 2048 fp32 or 4096 16-bit columns
 // (dist_team_kernel), by a workgroup of 256 ... 1024 threads up to 131072 or 65536 (dist_row_kernel).  Longer rows,
 // and few long rows (whose workgroups would leave most CUs idle), are cut into segments: one launch leaves every
-// segment's maximum and sum, a second joins them and writes (dist_part_kernel, dist_apply_kernel).
+// segment's maximum and sum, a second joins them and writes (dist_part_kernel, dist_apply_kernel).  Rows that the teacher may name
+// whole go their own way at high temperatures (dist_full_kernel).
 //
 // The columns that a teacher names are stored a second time, behind the row's plain p; where a row names a column
 // twice (a bit per column in LDS finds out, columns folded to 65536 bits), the first of its entries adds the others' weight in
@@ -16,7 +17,7 @@
 // Measured, half the rows masked (those are only written): 65536 x 512 fp32 from 16 entries 55 us (209 MB, 3.8 TB/s), 8192 x 50007 bf16
 // from 64 entries 319 us (1.24 GB, 3.9 TB/s); a copy of 4 GiB runs at 4.76 TB/s.  12 x 131072 fp16 from 128: 3.9 + 7.2 us.
 //
-// Softmax statistics, terms and gradients are fp32, the mean over the rows fp64; the gradient is rounded once, to the logits'
+// Softmax statistics, terms and gradients are fp32 (dist_full_kernel: fp64 sums), the mean over the rows fp64; the gradient is rounded once, to the logits'
 // type, when it is stored.
 #include "loss_rows.h"
 
@@ -260,6 +261,156 @@ __global__ __launch_bounds__(THREADS) void dist_team_kernel(DistArgs a) {
         if (threadIdx.x == 0)
             for (int w = 1; w < THREADS / 64; ++w) sum += s_loss[w];
         finish_loss<THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
+    }
+}
+
+// ------------------------------------------------------------------- rows that a teacher may name whole, high temperatures
+// Both softmaxes are nearly even there, and loss and gradient are small differences of theirs: the loss is of the order of the
+// squared arguments, which t^2 makes up for, and from plain sums it would be off by t^2 2^-22 (8 of 8 columns, t = 1000: 0.2 of 0.45).
+// So exponentials near 1 go by their distance to 1, whose sums are as accurate as the arguments, and the loss is a sum in which
+// nothing cancels: with delta_j = log q_j - log p_j (p of the column that entry j names),
+//
+//   sum_j q_j delta_j = sum_j q_j (delta_j - 1 + exp(-delta_j)) + 1 - sum_j p_j        p_j - q_j = q_j (exp(-delta_j) - 1)
+//
+// Needed where the entries' columns may be the row, 2 k >= v; beside a larger share of other columns the loss is of the order of t^2.
+constexpr float FULL_TEMPERATURE = 4.f;  // below, t^2 2^-22 is lost beside the other roundings
+// Lanes of a row of v columns; what the lanes of a wave do in common is long (calls of fp32 rows at t = 4, and below:
+// 65536 x 100 from 64 132 and 61 us, 179 with a wave a row; 65536 x 512 from 256 649 and 388, 767 with sixteen lanes; 512 x 8 from 8 20 and 17).
+inline int full_team(int v) { return v <= 64 ? 8 : (v <= 256 ? 16 : 64); }
+constexpr int full_max_v(int team) { return team == 8 ? 64 : (team == 16 ? 256 : 2 * DIST_MAX_K); }
+
+// A sum of exponentials: how many are near 1, and the sum of those ones' distances to 1 and of the others.
+struct ExpSum {
+    double ones = 0., rest = 0.;
+    __device__ __forceinline__ void add(float arg) {  // exp2(arg)
+        const bool near = arg > -0.5f;
+        ones += near ? 1. : 0.;
+        rest += near ? expm1f(arg * LN2) : __builtin_amdgcn_exp2f(arg);
+    }
+    __device__ __forceinline__ double sum() const { return ones + rest; }
+    __device__ __forceinline__ double less(const ExpSum &b) const { return (ones - b.ones) + (rest - b.rest); }
+};
+__device__ __forceinline__ double exp2_of(float arg) {
+    ExpSum one;
+    one.add(arg);
+    return one.sum();
+}
+template <int TEAM>
+__device__ __forceinline__ double team_sum64(double v) {
+    for (int o = TEAM / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+template <int TEAM>
+__device__ __forceinline__ ExpSum team_sum64(ExpSum s) {
+    s.ones = team_sum64<TEAM>(s.ones);
+    s.rest = team_sum64<TEAM>(s.rest);
+    return s;
+}
+
+template <typename E, int TEAM, bool VALUE, bool GRAD>
+__global__ __launch_bounds__(TEAM_THREADS) void dist_full_kernel(DistArgs a) {
+    constexpr int TEAMS = TEAM_THREADS / TEAM, WORDS = full_max_v(TEAM) / 32;
+    constexpr double LN2_64 = 0.69314718055994531;
+    __shared__ unsigned s_bits[GRAD ? TEAMS : 1][GRAD ? WORDS : 1];
+    __shared__ double s_loss[VALUE ? TEAM_THREADS / 64 : 1];
+    const int lane = threadIdx.x & 63, pos = threadIdx.x & (TEAM - 1), team = threadIdx.x / TEAM;
+    const float inv = inv_kept<TEAM_THREADS>(a);
+    float factor = 0.f;
+    if constexpr (GRAD) {
+        factor = grad_factor(a, inv);
+        for (int w = pos; w < WORDS; w += TEAM) s_bits[team][w] = 0;
+    }
+    double sum = 0.;
+    for (long long i = (long long)blockIdx.x * TEAMS + team; i < a.n; i += (long long)gridDim.x * TEAMS) {
+        const E *row = (const E *)a.logits + i * a.row_stride;
+        E *grow = (E *)a.grad + i * a.v;
+        if (a.mask && !a.mask[i]) {
+            if (VALUE && pos == 0) {
+                a.row_loss[i] = 0.f;
+                a.stats[2 * i] = 0.f;
+                a.stats[2 * i + 1] = 0.f;
+            }
+            if constexpr (GRAD)
+                for (int c = pos; c < a.v; c += TEAM) grow[c] = (E)0.f;
+            continue;
+        }
+        const auto each = [&](auto f) {  // f(j, column, teacher's logit, student's logit) for this lane's entries
+            for (int j = pos; j < a.k; j += TEAM) {
+                int c;
+                float t;
+                entry(a, i, j, c, t);
+                if (c >= 0) f(j, c, t, (float)row[c]);
+            }
+        };
+        float m = -INFINITY, tm = -INFINITY;
+        for (int c = pos; c < a.v; c += TEAM) m = fmaxf(m, (float)row[c]);
+        each([&](int, int, float t, float) { tm = fmaxf(tm, t); });
+        m = team_max<TEAM>(m);
+        const Shift s(a.c, m), ts(a.c, team_max<TEAM>(tm));
+        ExpSum l, tl;
+        for (int c = pos; c < a.v; c += TEAM) l.add(s.arg((float)row[c]));
+        each([&](int, int, float t, float) { tl.add(ts.arg(t)); });
+        l = team_sum64<TEAM>(l);
+        tl = team_sum64<TEAM>(tl);
+        const bool empty = l.sum() == 0. || tl.sum() == 0.;
+        const double inv_l = empty ? 0. : 1. / l.sum(), inv_tl = empty ? 0. : 1. / tl.sum();
+        const double ratio = empty ? 0. : log1p(l.less(tl) * inv_tl);  // of the two sums, its logarithm
+        const auto delta = [&](float t, float x) { return LN2_64 * ((double)ts.arg(t) - (double)s.arg(x)) + ratio; };
+        if constexpr (VALUE) {
+            double terms = 0.;
+            ExpSum named;
+            each([&](int, int, float t, float x) {
+                const double q = exp2_of(ts.arg(t)) * inv_tl;
+                if (q == 0.) return;  // (a NaN is not)
+                const double d = delta(t, x);
+                terms += q * (d + expm1(-d));
+                named.add(s.arg(x));
+            });
+            terms = team_sum64<TEAM>(terms);
+            named = team_sum64<TEAM>(named);
+            if (pos == 0) {
+                const float loss = empty ? 0.f : (float)((double)a.temperature * a.temperature * (terms + l.less(named) * inv_l));
+                a.row_loss[i] = loss;
+                a.stats[2 * i] = m;
+                a.stats[2 * i + 1] = (float)l.sum();
+                sum += loss;
+            }
+        }
+        if constexpr (GRAD) {
+            for (int c = pos; c < a.v; c += TEAM) grow[c] = empty ? (E)0.f : (E)(factor * (float)(exp2_of(s.arg((float)row[c])) * inv_l));
+            if (empty) continue;
+            bool twice = false;
+            each([&](int, int c, float, float) { twice |= (atomicOr(&s_bits[team][c >> 5], 1u << (c & 31)) >> (c & 31)) & 1; });
+            __builtin_amdgcn_wave_barrier();
+            each([&](int, int c, float, float) { s_bits[team][c >> 5] = 0; });
+            __builtin_amdgcn_wave_barrier();
+            const unsigned long long team_lanes = (TEAM == 64 ? ~0ull : (1ull << (TEAM & 63)) - 1) << (lane & ~(TEAM - 1));
+            const bool repeats = (__ballot(twice) & team_lanes) != 0;
+            each([&](int j, int c, float t, float x) {
+                const double q = exp2_of(ts.arg(t)) * inv_tl;
+                double diff = q == 0. ? exp2_of(s.arg(x)) * inv_l : q * expm1(-delta(t, x));
+                if (repeats) {
+                    for (int h = 0; h < a.k; ++h) {
+                        if (h == j) continue;
+                        int ch;
+                        float th;
+                        entry(a, i, h, ch, th);
+                        if (ch != c) continue;
+                        if (h < j) return;  // an entry before this one stores for both
+                        diff -= exp2_of(ts.arg(th)) * inv_tl;
+                    }
+                }
+                grow[c] = (E)(factor * (float)diff);
+            });
+        }
+    }
+    if constexpr (VALUE) {
+        for (int o = TEAM; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);  // a team's first lane holds its rows' sum
+        if (lane == 0) s_loss[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int w = 1; w < TEAM_THREADS / 64; ++w) sum += s_loss[w];
+        finish_loss<TEAM_THREADS>(a, sum, blockIdx.x, gridDim.x, inv);
     }
 }
 
@@ -582,16 +733,23 @@ int distill_check(const char *what, int n, int v, int k, const void *logits, lon
 }
 
 // How rows of v columns are held.
-enum Way { BY_TEAM, BY_ROW, BY_SEGMENT };
+enum Way { BY_TEAM, BY_FULL, BY_ROW, BY_SEGMENT };
 struct Plan {
     Way way;
-    int team, chunks;  // BY_TEAM: lanes a row, chunks a lane
+    int team, chunks;  // BY_TEAM, BY_FULL: lanes a row; BY_TEAM: chunks a lane
     int threads;       // of a workgroup (BY_ROW: threads a row, chunks a thread in `chunks`)
     int seg, segs;
 };
-inline Plan plan_rows(int n, int v, int vec) {
+inline bool may_be_full(int v, int k) { return v <= 2ll * k; }
+inline Plan plan_rows(int n, int v, int vec, bool full) {
     Plan p = {BY_TEAM, 0, 0, 0, 0, 0};
     const int chunks = ceil_div(v, vec);
+    if (full) {
+        p.way = BY_FULL;
+        p.team = full_team(v);
+        p.threads = TEAM_THREADS;
+        return p;
+    }
     if (chunks <= TEAM_MAX_CHUNKS) {
         p.team = 1;
         while (p.team < chunks && p.team < 64) p.team <<= 1;
@@ -628,10 +786,10 @@ inline Plan plan_rows(int n, int v, int vec) {
 constexpr int DIST_TEAM_BLOCKS = 4088, DIST_ROW_BLOCKS = 16376;
 inline int dist_blocks(const Plan &p, int n) {
     if (p.way == BY_SEGMENT) return n > 0 ? n : 1;
-    const long rows = p.way == BY_TEAM ? p.threads / p.team : 1;
+    const long rows = p.way == BY_ROW ? 1 : p.threads / p.team;
     const long want = ((long)n + rows - 1) / rows;
     if (p.way == BY_TEAM && want <= 2) return 1;  // a second round of rows costs less than the launch that joins workgroups
-    return (int)(want < 1 ? 1 : std::min<long>(want, p.way == BY_TEAM ? DIST_TEAM_BLOCKS : DIST_ROW_BLOCKS));
+    return (int)(want < 1 ? 1 : std::min<long>(want, p.way == BY_ROW ? DIST_ROW_BLOCKS : DIST_TEAM_BLOCKS));
 }
 // Workspace: ticket, sums of row losses, segments
 constexpr size_t TICKET_BYTES = 16;
@@ -675,6 +833,14 @@ int launch_team(hipStream_t stream, const DistArgs &a, const Plan &p) {
 template <typename E, bool VALUE, bool GRAD>
 int launch_distill(hipStream_t stream, const DistArgs &a, const Plan &p) {
     if (p.way == BY_TEAM) return launch_team<E, VALUE, GRAD>(stream, a, p);
+    if (p.way == BY_FULL) {
+        const dim3 grid(dist_blocks(p, a.n));
+        if (p.team == 8) hipLaunchKernelGGL((dist_full_kernel<E, 8, VALUE, GRAD>), grid, dim3(TEAM_THREADS), 0, stream, a);
+        else if (p.team == 16) hipLaunchKernelGGL((dist_full_kernel<E, 16, VALUE, GRAD>), grid, dim3(TEAM_THREADS), 0, stream, a);
+        else hipLaunchKernelGGL((dist_full_kernel<E, 64, VALUE, GRAD>), grid, dim3(TEAM_THREADS), 0, stream, a);
+        GDPSO_HIP(hipGetLastError());
+        return GDPSO_OK;
+    }
     if (VALUE && p.way == BY_ROW) {
         const dim3 grid(dist_blocks(p, a.n));
         if (p.threads == 256) hipLaunchKernelGGL((dist_row_kernel<E, 256, 8, GRAD>), grid, dim3(256), 0, stream, a);
@@ -697,7 +863,8 @@ using namespace gdpso;
 
 extern "C" size_t gdpso_distill_workspace_bytes(int n, int v, int k) {
     if (n < 0 || v <= 0 || k <= 0) return 0;
-    return std::max(space_bytes(plan_rows(n, v, 4), n), space_bytes(plan_rows(n, v, 8), n));  // whatever the type
+    const size_t size = std::max(space_bytes(plan_rows(n, v, 4, false), n), space_bytes(plan_rows(n, v, 8, false), n));
+    return may_be_full(v, k) ? std::max(size, space_bytes(plan_rows(n, v, 4, true), n)) : size;  // whatever type and temperature
 }
 
 extern "C" int gdpso_distill(void *stream_, int n, int v, int k, const void *logits, long long row_stride, int dtype, const void *t_logits, int t_dtype,
@@ -709,7 +876,7 @@ extern "C" int gdpso_distill(void *stream_, int n, int v, int k, const void *log
     if (workspace_bytes < gdpso_distill_workspace_bytes(n, v, k)) return fail(GDPSO_ERR_WORKSPACE, "distill: workspace too small");
     hipStream_t stream = (hipStream_t)stream_;
     float *inv_rows = row_stats + 2 * (size_t)n;
-    const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype));
+    const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype), temperature >= FULL_TEMPERATURE && may_be_full(v, k));
     unsigned *ticket = (unsigned *)workspace;
     double *loss_part = (double *)((char *)workspace + TICKET_BYTES);
     float2 *parts = (float2 *)((char *)loss_part + loss_bytes(p, n));
@@ -741,7 +908,7 @@ extern "C" int gdpso_distill_grad(void *stream_, int n, int v, int k, const void
     if (rc) return rc;
     GDPSO_REQUIRE(n == 0 || (row_stats && upstream && grad), "distill_grad: null argument");
     if (n == 0) return GDPSO_OK;
-    const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype));
+    const Plan p = plan_rows(n, v, 16 / (int)dtype_size(dtype), temperature >= FULL_TEMPERATURE && may_be_full(v, k));
     const DistArgs a = {n, v, k, logits, row_stride, t_logits, t_dtype, t_indices, index_bytes, mask, temperature, log2e_over(temperature), 0.f, upstream,
                         (float *)row_stats, (float *)row_stats + 2 * (size_t)n, 0.f, KEPT_READ, nullptr, nullptr, nullptr, grad, nullptr, p.seg, p.segs,
                         nullptr};

@@ -405,6 +405,8 @@ int gdpso_balance_grad(void *stream, int n, int e, const void *logits, long long
  * absent (rows with fewer than k entries); an index that appears twice adds up.  A row without an entry, or without a finite
  * student logit, has loss 0 and gradient 0 but counts as kept; a teacher's entry on a column at -inf makes the loss
  * +inf; NaN propagates.  mask as for gdpso_balance.  1 <= k <= GDPSO_DISTILL_MAX_K, temperature in [1e-6, 1e6].
+ * A row loss is off by about 2^-21 t^2 at most beside its own rounding; from t = 4 on, rows that the teacher may name whole (v <= 2 k),
+ * whose loss does not grow with t, keep their relative accuracy instead, and so do their gradients.
  * Outputs: loss [1], row_loss [n] (0 for rows left out), row_stats [2 n + 1] (what gdpso_distill_grad needs: maximum and
  * sum of exponentials of every row, then one over the rows kept), grad [n, v] in `dtype`, contiguous, or NULL.
  * gdpso_distill_grad: the gradient alone, times the DEVICE scalar *upstream. */

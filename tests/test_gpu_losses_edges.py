@@ -145,3 +145,139 @@ def test_distill_of_no_rows(v, masked):
     lib.run(loss.device, L.gdpso_distill, 0, v, 4, None, v, 0, None, 0, None, 8, lib.ptr(mask), 1.0, 1.0, loss.data_ptr(), None, stats.data_ptr(), None,
             ws.data_ptr(), size)
     assert float(loss) == 0.0 and float(stats) == 0.0
+
+
+# ----------------------------------------------------------------------------------------------- high temperatures
+def distill_smooth64(logits, t_logits, t_idx, mask, t, scale):
+    """The definition in 64 bits in a form that does not cancel where both softmaxes are nearly even, and bounds.  Each row
+    sums q (delta - 1 + exp(-delta)) over its entries, delta = log q - log p, and 1 - sum of p over them; exponentials go by their distance
+    to 1.  Returns (loss, row_loss, grad, bounds of the three before they are stored).
+
+    Bounds: an argument x / t - max / t rounds once (U of itself), its temperature and its change of base 3 U more, and the distance of
+    its exponential to 1 two, which is at most 6 U of the argument: with `span` the largest argument of the row, delta is off by at most
+    e = 16 U span (two arguments and two sums of such distances), q by a factor of at most e + 2 U.  The loss changes by |1 - exp(-delta)| q e
+    for each entry and by the factor of its q; the gradient of a column by q e and by the factor of its p or q."""
+    n, v = logits.shape
+    x, tl, idx = logits.double().cpu(), t_logits.double().cpu(), t_idx.cpu().long()
+    keep = torch.ones(n, dtype=torch.bool) if mask is None else mask.cpu().bool()
+    x = torch.where(keep[:, None], x, torch.zeros_like(x))
+    there = (idx >= 0) & (idx < v) & keep[:, None]
+    tl = torch.where(there, tl, torch.full_like(tl, -math.inf))
+    col = torch.where(there, idx, torch.zeros_like(idx))
+
+    def parts(z):
+        m = z.amax(dim=1, keepdim=True)
+        m = torch.where(m == -math.inf, torch.zeros_like(m), m)
+        arg = (z - m) / t
+        live = arg > -math.inf
+        return arg, live, live.sum(dim=1).double(), torch.where(live, torch.expm1(arg), torch.zeros_like(arg))
+
+    ax, lx, nx, ex = parts(x)
+    at, lt, nt, et = parts(tl)
+    total, t_total = nx + ex.sum(dim=1), nt + et.sum(dim=1)
+    live_row = keep & (nx > 0) & (nt > 0)
+    safe, t_safe = total.clamp(min=1.0), t_total.clamp(min=1.0)
+    ratio = torch.log1p(((nx - nt) + (ex.sum(dim=1) - et.sum(dim=1))) / t_safe)
+    named = ax.gather(1, col)
+    q = torch.where(lt, (1 + et) / t_safe[:, None], torch.zeros_like(et))
+    delta = torch.where(lt, at - named + ratio[:, None], torch.zeros_like(at))
+    psi = torch.where(lt, q * (delta + torch.expm1(-delta)), torch.zeros_like(q))
+    rest_n = nx - (lt & (named > -math.inf)).sum(dim=1)
+    rest_e = ex.sum(dim=1) - torch.where(lt, ex.gather(1, col), torch.zeros_like(q)).sum(dim=1)
+    row = torch.where(live_row, t * t * (psi.sum(dim=1) + (rest_n + rest_e) / safe), torch.zeros(n, dtype=torch.float64))
+    rows = max(1, int(keep.sum()))
+    loss = row.sum() / rows
+    p = torch.where(lx, (1 + ex) / safe[:, None], torch.zeros_like(ex))
+    # a column's entries: the first one's q expm1(-delta) is p - q, the others' q come off whole
+    factor = scale * t / rows
+    big_q = torch.zeros_like(x).scatter_add_(1, col, q)
+    alone = torch.zeros_like(x).scatter_add_(1, col, lt.double()) == 1
+    smooth = torch.zeros_like(x).scatter_add_(1, col, torch.where(lt, q * torch.expm1(-delta), torch.zeros_like(q)))
+    grad = factor * torch.where(alone, smooth, p - big_q)
+    grad = torch.where(live_row[:, None], grad, torch.zeros_like(grad))
+    span = torch.maximum(torch.where(lx, ax.abs(), torch.zeros_like(ax)).amax(dim=1), torch.where(lt, at.abs(), torch.zeros_like(at)).amax(dim=1))
+    e = 16 * U * span
+    slope = torch.where(lt & (delta < math.inf), q * (1 - torch.exp(-delta)).abs(), torch.zeros_like(q)).sum(dim=1)
+    rest = ((rest_n + rest_e) / safe).abs()
+    row_bound = t * t * (slope * e + (psi.sum(dim=1) + rest) * (e + 8 * U)) + row.abs() * 4 * U
+    row_bound = torch.where(live_row, row_bound, torch.zeros_like(row))
+    grad_bound = factor * ((big_q + p) * e[:, None]) + grad.abs() * (8 * U + e[:, None])
+    several = torch.zeros_like(x).scatter_add_(1, col, lt.double()) > 1
+    grad_bound = grad_bound + torch.where(several, factor * (big_q + p) * 8 * U, torch.zeros_like(p))
+    grad_bound = torch.where(live_row[:, None], grad_bound, torch.zeros_like(grad_bound))
+    return loss, row, grad, row_bound.sum() / rows + loss.abs() * 4 * U, row_bound, grad_bound
+
+
+FULL = [(40, 2, 2), (600, 8, 8), (33, 8, 5), (70, 64, 40), (40, 65, 65), (300, 200, 130), (40, 512, 512), (9, 1000, 1024), (5, 2048, 1024), (9000, 8, 8)]
+
+
+def check_full(out, logits, t_logits, t_idx, mask, t, scale):
+    loss, row, grad = out
+    want = distill_smooth64(logits, t_logits, t_idx, mask, t, 1.0 if scale is None else scale)
+    if row is not None:
+        assert_within(row, want[1], want[4] + store_error(want[1], torch.float32), "row_loss")
+    assert_within(loss, want[0], want[3] + store_error(want[0], torch.float32), "loss")
+    if scale is not None:
+        # fp16 ends at 65504: what is half a step (16) beyond it or more rounds to infinity, e.g. 1e6 (1 / 8 - 1 / 5) = -75000
+        info = torch.finfo(logits.dtype)
+        beyond = want[2].abs() - want[5] > info.max * (1 + info.eps / 4)
+        exact = torch.where(beyond, want[2].sign() * math.inf, want[2])
+        assert_within(grad, exact, want[5] + store_error(want[2], logits.dtype), "grad")
+
+
+@pytest.mark.parametrize("t", [4.0, 10.0, 100.0, 1000.0, 1e6])
+@pytest.mark.parametrize("n,v,k", FULL)
+def test_distill_of_whole_rows_at_high_temperatures(eng, fn, n, v, k, t):
+    """A teacher that names (nearly) all columns: at high temperatures both softmaxes are nearly even, and loss and gradient are
+    small differences of theirs."""
+    for dtype in DTYPES:
+        logits = rand(n + v, n, v, scale=2.0, dtype=dtype)
+        top = (logits.float() + rand(v, n, v)).topk(min(k, v), dim=1)
+        t_logits, t_idx = top.values, top.indices
+        if k > v:  # the entries beyond the columns are absent
+            t_logits = torch.cat([t_logits, t_logits[:, : k - v]], dim=1)
+            t_idx = torch.cat([t_idx, torch.full_like(t_idx[:, : k - v], -1)], dim=1)
+        scale = float(n)
+        check_full(eng.distill(logits, t_logits, t_idx, temperature=t), logits, t_logits, t_idx, None, t, None)
+        check_full(eng.distill(logits, t_logits, t_idx, temperature=t, grad_scale=scale), logits, t_logits, t_idx, None, t, scale)
+        mask = torch.arange(n, device=DEV) % 5 != 2
+        leaf = logits.clone()
+        leaf[2] = math.nan
+        leaf.requires_grad_()
+        loss = fn.distill(leaf, t_logits, t_idx, mask, t)
+        (scale * loss).backward()
+        check_full((loss, None, leaf.grad), logits, t_logits, t_idx, mask, t, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [8, 100])
+def test_distill_of_whole_rows_with_gaps(eng, v, dtype):
+    n, t = 30, 50.0
+    logits = rand(v, n, v, dtype=dtype)
+    top = (logits.float() + rand(1, n, v)).topk(v, dim=1)
+    t_logits, t_idx = top.values.to(dtype), top.indices
+    logits[0] = -math.inf                       # nothing to teach
+    logits[1, :3] = -math.inf                   # columns that no entry names ...
+    t_idx[1][(t_idx[1] < 3)] = -1
+    logits[2] = torch.finfo(dtype).min          # even
+    t_idx[3] = -1                               # no entry
+    t_idx[4, 1:] = t_idx[4, 0]                  # one column named by all
+    t_idx[5, 2] = t_idx[5, 1]
+    t_logits[6] = -math.inf                     # entries without weight
+    t_logits[7, 3:] = -math.inf
+    t_idx[8, 0], t_idx[8, 1] = v, 2 ** 40       # out of range
+    mask = torch.ones(n, dtype=torch.bool, device=DEV)
+    mask[9:11] = False
+    dirty = logits.clone()
+    dirty[9], dirty[10] = math.nan, math.inf
+    out = eng.distill(dirty, t_logits, t_idx, mask=mask, temperature=t, grad_scale=float(n))
+    check_full(out, logits, t_logits, t_idx, mask, t, float(n))
+    again = eng.distill(dirty, t_logits, t_idx.clamp(-1, v).int(), mask=mask, temperature=t, grad_scale=float(n))
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+    assert all(torch.equal(a, b) for a, b in zip(out[:2], eng.distill(dirty, t_logits, t_idx, mask=mask, temperature=t)[:2]))
+    logits[12, 0], logits[13, 0] = math.nan, math.inf
+    t_logits[14, 0] = math.nan
+    logits[15, t_idx[15, 1]] = -math.inf        # the teacher gives weight to a column that the student cannot reach
+    loss, row, grad = eng.distill(logits, t_logits, t_idx, temperature=t, grad_scale=1.0)
+    assert bool(loss.isnan()) and [i for i in range(n) if bool(row[i].isnan())] == [12, 13, 14]
+    assert float(row[15]) == math.inf and bool(grad[15].isfinite().all())
