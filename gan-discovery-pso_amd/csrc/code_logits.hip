@@ -958,7 +958,7 @@ int launch_logits(hipStream_t stream, ProductArgs a) {
         a.tiles_n = std::min(col_tiles, std::max(ceil_div(512, a.tiles_m), more));
     }
     const long grid = (long)ceil_div(a.tiles_m, 8) * 8 * a.tiles_n;
-    GDPSO_REQUIRE(grid < (1l << 31), "code_logits: too many rows for one call");
+    GDPSO_REQUIRE(grid_fits(grid, CL_THREADS), "code_logits: too many rows for one call");
 #define CL_LOGITS(NS)                                                                                                                        \
     do {                                                                                                                                     \
         if (mt == 2) hipLaunchKernelGGL((logits_kernel<E, P, M, NS, 2>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, a);              \
@@ -994,7 +994,7 @@ int launch_grads(hipStream_t stream, ProductArgs code, ProductArgs x, Tile t) {
     const long splits = small ? code.splits : (code.splits + 7) / 8 * 8, row_tiles = small ? x.tiles_m : (x.tiles_m + 7) / 8 * 8 * x.splits;
     const long code_blocks = code.out ? splits * code.tiles_m * code.tiles_n : 0;
     const long grid = code_blocks + (x.out ? row_tiles * x.tiles_n : 0);
-    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
+    GDPSO_REQUIRE(grid_fits(grid, CL_THREADS), "code_logits_grad: too many rows for one call");
     constexpr int P = grad_parts<E>();
 #define CL_GRADS(MT, NT) hipLaunchKernelGGL((grads_kernel<E, P, MT, NT>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, code, (int)code_blocks, x)
     if (small) {
@@ -1067,7 +1067,7 @@ int launch_planes(hipStream_t stream, const PlanesArgs &a, bool codes, bool late
     const int col_tiles = ceil_div(a.cols, 64);
     b.first = codes ? ceil_div(a.rows[0], 64) * col_tiles : 0;
     const long grid = b.first + (latents ? (long)ceil_div(a.rows[1], 64) * col_tiles : 0);
-    GDPSO_REQUIRE(grid < (1l << 31), "code_logits_grad: too many rows for one call");
+    GDPSO_REQUIRE(grid_fits(grid, CL_THREADS), "code_logits_grad: too many rows for one call");
     hipLaunchKernelGGL((planes_kernel<E, grad_parts<E>()>), dim3((unsigned)grid), dim3(CL_THREADS), 0, stream, b);
     GDPSO_HIP(hipGetLastError());
     return GDPSO_OK;
@@ -1119,6 +1119,7 @@ extern "C" int gdpso_code_logits_grad(void *stream_, int n, int d, int k, const 
         const int waves = splits > 64 ? 16 : 4;  // many splits of few elements: more waves a workgroup (65536 x 64 x 64: 32 us with 4, 27)
         const long code_blocks = join_code ? ceil_div((long)k * d, 64) : 0, x_size = (long)n * d;
         const long grid = code_blocks + (join_x ? ceil_div(x_size, 64 * 4 * waves) : 0);
+        GDPSO_REQUIRE(grid_fits(grid, 64 * waves), "code_logits_grad: too many rows for one call");
         const JoinArgs a = {d, k, splits, xs, part, x_part, codebook, scale, grad_codebook, grad_inputs, x_size, (int)code_blocks};
         if (waves == 16)
             GDPSO_WITH_DTYPE(dtype, hipLaunchKernelGGL((join_kernel<E, 16>), dim3((unsigned)grid), dim3(64 * 16), 0, stream, a));

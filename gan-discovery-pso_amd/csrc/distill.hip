@@ -848,7 +848,7 @@ int launch_distill(hipStream_t stream, const DistArgs &a, const Plan &p) {
         else hipLaunchKernelGGL((dist_row_kernel<E, 1024, 16, GRAD>), grid, dim3(1024), 0, stream, a);
     } else {
         const long blocks = (long)a.n * a.segs;
-        GDPSO_REQUIRE(blocks < (1l << 31) - 1, "distill: too many rows for one call");
+        GDPSO_REQUIRE(grid_fits(blocks + 1, SEG_THREADS), "distill: too many rows for one call");
         if (VALUE) hipLaunchKernelGGL((dist_part_kernel<E>), dim3((unsigned)blocks + 1), dim3(SEG_THREADS), 0, stream, a);
         hipLaunchKernelGGL((dist_apply_kernel<E, VALUE, GRAD>), dim3((unsigned)(GRAD ? blocks : a.n)), dim3(SEG_THREADS), 0, stream, a);
     }

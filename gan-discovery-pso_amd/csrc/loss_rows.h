@@ -13,6 +13,9 @@
 
 namespace gdpso {
 
+// A launch's work items are counted in 32 bits.
+inline bool grid_fits(long blocks, int threads) { return blocks < (1l << 32) / threads; }
+
 template <typename E, int N>
 struct VecAt {  // N elements at element alignment
     typedef E type __attribute__((ext_vector_type(N), aligned(sizeof(E))));
