@@ -14,9 +14,9 @@
 // three for fp32 x bf16.  Parts multiply exactly and add up in fp32.  The forward product of two 16-bit operands needs no cutting.
 //
 // What bounds them: the fp32 logits or their gradient, [n, k], against which latents and codes are small, and with fp32 operands the
-// matrix instructions as much.  Latents 65536 x 64, 512 codes, fp32: logits 35 us (134 MB written, 3.8 TB/s, and 26 GFLOP of bf16 products), both
-// gradients 65 and the join 5 (the same 134 MB read for each, 4.1 TB/s, and 52 GFLOP).  50007 x 256 and 1024 codes, bf16: logits 71 us
-// (205 MB, 2.9 TB/s), planes 13, gradients 150 (2 x 205 MB, 2.7 TB/s, and 105 GFLOP), join 8.
+// matrix instructions as much.  Calls with inputs in rotation: latents 65536 x 64, 512 codes, fp32, logits 38 us (134 MB written, 3.6 TB/s,
+// and 26 GFLOP of bf16 products), both gradients with their join 74 (the same 134 MB read for each, and 52 GFLOP).  50007 x 256 and 1024
+// codes, bf16: logits 75 us (205 MB, 2.7 TB/s), gradients with planes and join 174 (2 x 205 MB and 157 GFLOP); fp16 77 and 274.
 #include "loss_rows.h"
 
 #include <algorithm>

@@ -5,17 +5,19 @@
 //
 // The work is one softmax over a long row and k corrections, bound by reading the logits and writing the gradient once
 // each.  Rows are therefore held in registers between the two: by 1 ... 64 lanes up to 2048 fp32 or 4096 16-bit columns
-// (dist_team_kernel), by a workgroup of 256 ... 1024 threads up to 131072 or 65536 (dist_row_kernel).  Longer rows,
-// and few long rows (whose workgroups would leave most CUs idle), are cut into segments: one launch leaves every
-// segment's maximum and sum, a second joins them and writes (dist_part_kernel, dist_apply_kernel).  Rows that the teacher may name
+// (dist_team_kernel), by a workgroup of 256 ... 1024 threads up to 65536 fp32 or 131072 16-bit columns (dist_row_kernel).  Longer
+// rows, rows of 16384 columns or more where there are fewer than 128 of them (as workgroups they would leave most CUs idle), and the
+// backward pass of all rows that lanes do not hold, are cut into segments: one launch leaves every segment's maximum and sum (the
+// backward pass is given them), a second joins them and writes (dist_part_kernel, dist_apply_kernel).  Rows that the teacher may name
 // whole go their own way at high temperatures (dist_full_kernel).
 //
 // The columns that a teacher names are stored a second time, behind the row's plain p; where a row names a column
 // twice (a bit per column in LDS finds out, columns folded to 65536 bits), the first of its entries adds the others' weight in
 // order and stores for all.  So nothing depends on the order of atomics, and the same call gives the same bits.
 //
-// Measured, half the rows masked (those are only written): 65536 x 512 fp32 from 16 entries 55 us (209 MB, 3.8 TB/s), 8192 x 50007 bf16
-// from 64 entries 319 us (1.24 GB, 3.9 TB/s); a copy of 4 GiB runs at 4.76 TB/s.  12 x 131072 fp16 from 128: 3.9 + 7.2 us.
+// Calls with inputs in rotation, half the rows masked (those are only written): 65536 x 512 fp32 from 16 entries 56 us (209 MB, 3.7 TB/s;
+// the backward pass's gradient alone 45), 8192 x 50007 bf16 from 64 entries 300 ... 320 us (1.24 GB, 4 TB/s; value alone 155, gradient
+// alone 256); a copy of 4 GiB runs at 4.76 TB/s.  12 x 131072 fp16 from 128: kernels of 4.2 + 8.2 us.
 //
 // Softmax statistics, terms and gradients are fp32 (dist_full_kernel: fp64 sums), the mean over the rows fp64; the gradient is rounded once, to the logits'
 // type, when it is stored.
