@@ -281,3 +281,36 @@ def test_distill_of_whole_rows_with_gaps(eng, v, dtype):
     loss, row, grad = eng.distill(logits, t_logits, t_idx, temperature=t, grad_scale=1.0)
     assert bool(loss.isnan()) and [i for i in range(n) if bool(row[i].isnan())] == [12, 13, 14]
     assert float(row[15]) == math.inf and bool(grad[15].isfinite().all())
+
+
+def test_distill_of_whole_rows_captured(eng):
+    """Captured calls of both forms replay on new inputs with eager work between, to the eager results' bits."""
+    def inputs(seed, n, v):
+        x = rand(seed, n, v, scale=2.0)
+        top = (x + rand(seed + 1, n, v)).topk(v, dim=1)
+        return [x, top.values, top.indices, torch.arange(n, device=DEV) % 7 != seed % 7]
+
+    def step(x, t, i, mask):
+        return [*eng.distill(x, t, i, mask=mask, temperature=20.0, grad_scale=1.0), *eng.distill(x, t, i, mask=mask, temperature=2.0, grad_scale=1.0)]
+
+    graphs = []
+    for n, v in ((700, 8), (20001, 100), (50, 600)):
+        static = inputs(n, n, v)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((n, v, static, graph, out))
+    for turn in range(3):
+        for n, v, static, graph, out in graphs:
+            fresh = inputs(100 * turn + n + 3, n, v)
+            for a, b in zip(static, fresh):
+                a.copy_(b)
+            graph.replay()
+            want = [r for r in step(*fresh) if r is not None]
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip([r for r in out if r is not None], want)), (turn, n)
